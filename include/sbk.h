@@ -282,6 +282,71 @@ int sbk_rope_kv_append(void* query, int H, int64_t q_token_stride_bytes, void* k
                        void* stream);
 
 /*
+ * The 8-bit K/V cache. Stands in for the fp8 form of the reference's cache write (kv_cache_dtype, k_scale, v_scale at
+ * vllm_hymeta/attention/meta_attention.py:790-799), with a scale per row where that has one per tensor.
+ * A token's row of one kv head (D values of K, or of V) is D codes in e4m3 and one exponent byte b, and stands for
+ *    value_d = code_d * 2^(b - 127).
+ *  k_cache,v_cache  [num_blocks, block_size, kvh, D] codes, `cache_block_stride_bytes` between blocks, rows contiguous
+ *  k_scale,v_scale  [num_blocks, kvh, block_size] exponent bytes, `scale_block_stride_bytes` between blocks
+ * All four base pointers and both strides are multiples of 16 bytes. e = b - 127 is the smallest integer in [-64, 63] with
+ * |x_d| <= 448 * 2^e over the finite values of the row; codes are rounded to nearest even; inf and NaN become the NaN code,
+ * magnitudes above 448 * 2^63 saturate. What is stored for a token depends on that token alone. Every value is a bf16 number.
+ *
+ * sbk_kv_append_q8: sbk_kv_append with the rows quantised on their way into the cache. key, value [T, kvh, D] of `dtype`
+ * (SBK_BF16 or SBK_F32), 16-byte aligned; D of 64, 128 or 256; block_size a multiple of 16; the remaining arguments as in
+ * sbk_kv_append. A slot may be named once per call (a row named twice would hold parts of both tokens).
+ *
+ * sbk_rope_kv_append_q8: the same with the rotary embedding folded in, arguments as in sbk_rope_kv_append. Unlike there
+ * the rotation is done in fp32 (every product and sum rounded once to fp32): K is quantised from the fp32 result, and the
+ * query (and the key, with key_in_place) is rounded once to `dtype`. rot_dim a multiple of 16, at most D.
+ *
+ * sbk_kv_gather_q8: sbk_kv_gather of the values, as `out_dtype` (both types hold them exactly).
+ */
+int sbk_kv_append_q8(const void* key, const void* value, int dtype, void* k_cache, void* v_cache, void* k_scale,
+                     void* v_scale, const int64_t* slot_mapping, int T, int kvh, int D,
+                     int64_t kv_token_stride_bytes, int64_t num_blocks, int block_size,
+                     int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes, int32_t* block_tables,
+                     int max_blocks, const int32_t* seq_lens, const int32_t* query_start_loc, int B,
+                     int window_left, int32_t* retired_out, int max_retired, int32_t* status, void* stream);
+int sbk_rope_kv_append_q8(void* query, int H, int64_t q_token_stride_bytes, void* key, const void* value,
+                          int key_in_place, int dtype, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                          const int64_t* slot_mapping, const int64_t* positions, const void* cos_sin_cache,
+                          int rot_dim, int64_t max_position, int T, int kvh, int D, int64_t kv_token_stride_bytes,
+                          int64_t num_blocks, int block_size, int64_t cache_block_stride_bytes,
+                          int64_t scale_block_stride_bytes, int32_t* block_tables, int max_blocks,
+                          const int32_t* seq_lens, const int32_t* query_start_loc, int B, int window_left,
+                          int32_t* retired_out, int max_retired, int32_t* status, void* stream);
+int sbk_kv_gather_q8(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                     const int32_t* block_tables, int max_blocks, const int32_t* seq_lens, int B, int kvh, int D,
+                     int64_t num_blocks, int block_size, int64_t cache_block_stride_bytes,
+                     int64_t scale_block_stride_bytes, int window_left, void* k_out, void* v_out, int out_dtype,
+                     int n_out, int32_t* status, void* stream);
+
+/*
+ * Sliding-window attention over the 8-bit cache: sbk_swa_decode (one query token per sequence) and sbk_swa_prefill (runs of
+ * query tokens) with the cache as above. q bf16; a query sees what it sees there; a sequence of length 0 gets zeros and
+ * lse -inf; a block-table entry outside the pool raises SBK_ST_BAD_BLOCK. Equal to the attention over the bf16 values that
+ * sbk_kv_gather_q8 returns, up to the rounding of the sums.
+ *  workspace    at least sbk_swa_decode_q8_workspace_bytes(B, H, D) bytes, 16-byte aligned (NULL when that is 0). Its
+ *               contents need no initialisation and mean nothing between calls. Calls that overlap on the GPU need
+ *               workspaces of their own.
+ * Supported: D == 128, H % kvh == 0, H/kvh <= 8, kvh in {1,2,4}, block_size % 16 == 0.
+ */
+size_t sbk_swa_decode_q8_workspace_bytes(int B, int H, int D);
+int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void* k_cache, const void* v_cache,
+                      const void* k_scale, const void* v_scale, const int32_t* block_tables, int max_blocks,
+                      const int32_t* seq_lens, int B, int H, int kvh, int D, int64_t num_blocks, int block_size,
+                      int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes, int window_left,
+                      float scale, void* out, int out_dtype, int64_t out_seq_stride, float* lse_out,
+                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const void* k_cache, const void* v_cache,
+                       const void* k_scale, const void* v_scale, const int32_t* block_tables, int max_blocks,
+                       const int32_t* query_start_loc, const int32_t* context_lens, int n_seqs, int max_query_len,
+                       int H, int kvh, int D, int64_t num_blocks, int block_size,
+                       int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes, int window_left,
+                       float scale, void* out, int64_t out_tok_stride, int32_t* status, void* stream);
+
+/*
  * Device-resident step planning and block allocation. State that stays on the GPU between steps:
  *    seq_lens [B] int32, block_tables [B, max_blocks] int32 (-1 = no block),
  *    ring [num_blocks] int32 (free block ids, FIFO), ctrl [4] uint64 (head, tail, lowest free

@@ -1,0 +1,120 @@
+"""The 8-bit K/V cache in 64 bits: the format by its definition (a search over exponents, the table of the 256 codes)
+and attention over the values it stands for, with the error a kernel may make on the way. Test infrastructure."""
+import math
+from typing import List, Tuple
+
+import torch
+
+MIN_EXP, MAX_EXP = -64, 63
+
+
+def code_values() -> torch.Tensor:
+    """The 256 e4m3 codes as float64 (sign, 4 exponent bits with bias 7, 3 fraction bits; 0x7f and 0xff are NaN)."""
+    v = []
+    for u in range(256):
+        e, f = (u >> 3) & 15, u & 7
+        x = math.nan if (u & 127) == 127 else ((8 + f) * 2.0 ** (e - 10) if e else f * 2.0 ** -9)
+        v.append(-x if u & 128 else x)
+    return torch.tensor(v, dtype=torch.float64)
+
+
+def values(codes: torch.Tensor, byte: torch.Tensor) -> torch.Tensor:
+    """Codes [..., D] and exponent bytes [...] -> float64 values."""
+    table = code_values().to(codes.device)
+    scale = torch.tensor([2.0 ** (b - 127) for b in range(256)], dtype=torch.float64, device=codes.device)
+    return table[codes.view(torch.uint8).long()] * scale[byte.long()].unsqueeze(-1)
+
+
+def quantise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows [..., D] of any float type -> (codes uint8, exponent bytes uint8): the smallest exponent under which every
+    finite value fits 448, the nearest code (ties to the even one), saturating; inf and NaN become NaN."""
+    x = x.double().cpu()
+    fine = torch.isfinite(x)
+    top = torch.where(fine, x.abs(), 0.0).amax(-1)
+    e = torch.full(top.shape, MAX_EXP, dtype=torch.int64)
+    for k in range(MAX_EXP - 1, MIN_EXP - 1, -1):
+        e = torch.where(top <= 448.0 * 2.0 ** k, k, e)
+    scale = torch.tensor([2.0 ** -k for k in range(MIN_EXP, MAX_EXP + 1)], dtype=torch.float64)[e - MIN_EXP]
+    y = torch.where(fine, x * scale.unsqueeze(-1), 0.0)
+    grid = code_values()[:127]                                   # 0 ... 448, ascending, code = index
+    a = y.abs().clamp(max=448.0)
+    hi = torch.searchsorted(grid, a.contiguous()).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    up, down = grid[hi] - a, a - grid[lo]
+    code = torch.where((down < up) | ((down == up) & (lo % 2 == 0)), lo, hi)
+    code = torch.where(fine, code | torch.where(torch.signbit(y), 128, 0), 127)
+    return code.to(torch.uint8), (e + 127).to(torch.uint8)
+
+
+def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor, scale: float):
+    """One sequence in float64: q [m, H, D], k and v [n, kvh, D] (values), seen [m, n]. Returns (out [m, H, D], lse [m, H],
+    err_out [m, H, D], err_lse [m, H]); the last two bound what a kernel may add before it rounds the output:
+      * scores: the query as two 4-bit pieces relative to its largest value loses at most 2^-18 of that value per product
+        (one piece in 16 bits loses less), and fp32 sums of D products 2^-20 of the sum of magnitudes;
+      * a score off by d moves every weight by at most 2 d of itself (numerator and normaliser);
+      * probabilities as two 4-bit pieces are off by at most 2^-4 * 2^-4 of themselves, and by 2^-22 of the largest
+        (probability * scale of its V row) where they are too small for the pieces; a code is at most 448;
+      * exponentials, fp32 sums and the division: 2^-18."""
+    m, H, D = q.shape
+    n, kvh, _ = k.shape
+    G = H // kvh
+    q, k, v = q.double().view(m, kvh, G, D), k.double(), v.double()
+    s = torch.einsum("mhgd,nhd->mhgn", q, k) * scale
+    s = s.masked_fill(~seen[:, None, None, :], -math.inf)
+    lse = torch.logsumexp(s, -1)
+    p = torch.where(seen[:, None, None, :], torch.exp(s - lse.clamp_min(-1e300).unsqueeze(-1)), 0.0)
+    any_seen = seen.any(-1)
+    kk = torch.where(seen.any(0)[:, None, None], k, 0.0)
+    vv = torch.where(seen.any(0)[:, None, None], v, 0.0)
+    out = torch.einsum("mhgn,nhd->mhgd", p, vv)
+    mag = torch.einsum("mhgd,nhd->mhgn", q.abs(), kk.abs()) * abs(scale)
+    floor = q.abs().amax(-1, keepdim=True) * kk.abs().sum(-1).t()[None, :, None, :] * abs(scale)
+    d = (2.0 ** -18 * floor + 2.0 ** -20 * mag).masked_fill(~seen[:, None, None, :], 0.0).amax(-1)
+    A = torch.einsum("mhgn,nhd->mhgd", p, vv.abs())
+    top = 2.0 * vv.abs().amax(-1)                                # at least 448 * 2^e of the row
+    small = n * 2.0 ** -22 * (p * top.t()[None, :, None, :]).amax(-1)
+    err = A * (2 * d + 2.0 ** -8 + 2.0 ** -18).unsqueeze(-1) + small.unsqueeze(-1)
+    zero = ~any_seen[:, None, None]
+    out = torch.where(zero.unsqueeze(-1), 0.0, out)
+    err_lse = d + 2.0 ** -18 + 2.0 ** -22 * lse.abs().clamp(max=1e300)
+    return out.reshape(m, H, D), lse.reshape(m, H), err.reshape(m, H, D), torch.where(zero, 0.0, err_lse).reshape(m, H)
+
+
+def window_values(codes: torch.Tensor, scale: torch.Tensor, table: torch.Tensor, lo: int, hi: int) -> torch.Tensor:
+    """Tokens [lo, hi) of one sequence through its block table: values [n, kvh, D]. codes [blocks, bs, kvh, D], scale
+    [blocks, kvh, bs]."""
+    bs = codes.shape[1]
+    t = torch.arange(lo, hi, device=codes.device)
+    blk = table[t // bs].long()
+    return values(codes.view(torch.uint8)[blk, t % bs], scale[blk, :, t % bs])
+
+
+def decode(q, codes, scales, table, lens: List[int], window_left: int, scale: float):
+    """codes [2, ...], scales [2, ...]; q [B, H, D] -> the four tensors of attend, rows stacked."""
+    return runs(q, codes, scales, table, [max(0, n - 1) for n in lens], [min(1, n) for n in lens], window_left, scale,
+                one_row_each=True)
+
+
+def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: int, scale: float, one_row_each=False):
+    """Runs of queries: sequence s owns the next new[s] rows of q, behind ctx[s] cached tokens."""
+    H, D = q.shape[1:]
+    dev = q.device
+    res, row = [], 0
+    for s, (c, n) in enumerate(zip(ctx, new)):
+        if n == 0:
+            if one_row_each:
+                z = torch.zeros(1, H, D, dtype=torch.float64, device=dev)
+                res.append((z, torch.full((1, H), -math.inf, dtype=torch.float64, device=dev), z, z[..., 0]))
+                row += 1
+            continue
+        lo = 0 if window_left < 0 else max(0, c - window_left)
+        k = window_values(codes[0], scales[0], table[s], lo, c + n)
+        v = window_values(codes[1], scales[1], table[s], lo, c + n)
+        for i in range(0, n, 256):
+            m = min(256, n - i)
+            qp = torch.arange(c + i, c + i + m, device=dev)[:, None]
+            kp = torch.arange(lo, c + n, device=dev)[None]
+            seen = (kp <= qp) & ((kp >= qp - window_left) if window_left >= 0 else (kp >= 0))
+            res.append(attend(q[row + i:row + i + m], k, v, seen, scale))
+        row += n
+    return tuple(torch.cat([r[j] for r in res]) for j in range(4))

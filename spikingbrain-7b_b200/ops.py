@@ -628,3 +628,235 @@ def swa_prefill_dense(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q
         _stream())
     _abi.check("sbk_swa_prefill_dense", rc)
     return out
+
+
+# ----------------------------------------------------------------- the 8-bit cache
+_Q8_CODES = (torch.float8_e4m3fn, torch.uint8)
+_Q8_SCALES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def kv_cache_q8(num_blocks: int, block_size: int, kvh: int, D: int, device="cuda") -> Tuple[torch.Tensor, torch.Tensor]:
+    """An empty 8-bit cache: codes [2, num_blocks, block_size, kvh, D] (float8_e4m3fn, K then V) and exponent bytes
+    [2, num_blocks, kvh, block_size] (uint8). Value of a code: code * 2^(byte - 127)."""
+    if block_size <= 0 or block_size % 16:
+        raise ValueError(f"Invalid block size {block_size}. Must be a multiple of 16 and at least 16.")
+    codes = torch.zeros(2, num_blocks, block_size, kvh, D, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    return codes, torch.full((2, num_blocks, kvh, block_size), 63, dtype=torch.uint8, device=device)
+
+
+def _q8_geometry(k_cache, v_cache, k_scale, v_scale) -> Tuple[int, int, int, int, int, int]:
+    """-> (num_blocks, block_size, kvh, D, bytes between cache blocks, bytes between scale blocks)."""
+    if k_cache.dtype not in _Q8_CODES or v_cache.dtype != k_cache.dtype:
+        raise ValueError("the 8-bit k_cache and v_cache are float8_e4m3fn (or uint8) tensors of one dtype")
+    nb, bs, kvh, d, stride = _cache_geometry(k_cache, v_cache)
+    for t in (k_scale, v_scale):
+        if t.dtype not in _Q8_SCALES or t.shape != (nb, kvh, bs):
+            raise ValueError(f"k_scale and v_scale must be uint8 [{nb}, {kvh}, {bs}]")
+        if nb and (t.stride(2) != 1 or (kvh > 1 and t.stride(1) != bs)):
+            raise ValueError("the rows of a scale block must be contiguous")
+    if k_scale.stride(0) != v_scale.stride(0):
+        raise ValueError("k_scale and v_scale must share one block stride")
+    return nb, bs, kvh, d, stride, k_scale.stride(0)
+
+
+def _heads_contiguous(t: torch.Tensor) -> bool:
+    """[n, heads, D] with the heads of a row one behind the other (strides of size-1 dimensions carry no meaning)."""
+    return not t.shape[0] or (t.stride(2) == 1 and (t.shape[1] < 2 or t.stride(1) == t.shape[2]))
+
+
+def _one_device(*tensors: Optional[torch.Tensor]) -> torch.device:
+    """The CUDA device that all tensors live on."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("libsbk ops take CUDA tensors only (there is no CPU path)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """C entry `name` on the current stream of `dev`, whichever device is current."""
+    if dev.index == torch.cuda.current_device():
+        rc = getattr(_abi.lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_abi.lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _abi.check(name, rc)
+
+
+def _q8_append_args(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc,
+                    retired_out):
+    nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
+    T = key.shape[0]
+    if key.shape != (T, kvh, d) or value.shape != key.shape:
+        raise ValueError(f"key/value must be [T, {kvh}, {d}], got {tuple(key.shape)} / {tuple(value.shape)}")
+    if key.dtype not in _DTYPE_CODE or value.dtype != key.dtype:
+        raise ValueError("key and value must share one dtype (bf16 or fp32)")
+    if not (_heads_contiguous(key) and _heads_contiguous(value)):
+        raise ValueError("key/value rows must be contiguous")
+    if T > 1 and value.stride(0) != key.stride(0):
+        raise ValueError("key and value must share one token stride")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous int64 tensor with one entry per token")
+    B = max_blocks = max_ret = 0
+    if block_tables is not None:
+        if seq_lens is None:
+            raise ValueError("retirement needs seq_lens")
+        B, max_blocks = block_tables.shape
+        _i32(block_tables, "block_tables")
+        _i32(seq_lens, "seq_lens", B)
+        _i32(query_start_loc, "query_start_loc", B + 1)
+        if retired_out is not None:
+            if retired_out.dtype != torch.int32 or not retired_out.is_contiguous() or retired_out.shape[0] != B:
+                raise ValueError("retired_out must be contiguous int32 [B, max_retired]")
+            max_ret = retired_out.shape[1]
+    es = key.element_size()
+    tok_stride = (key.stride(0) if T > 1 else kvh * d) * es
+    return nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, es, tok_stride
+
+
+def kv_append_q8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor, *,
+                 block_tables: Optional[torch.Tensor] = None, seq_lens: Optional[torch.Tensor] = None,
+                 query_start_loc: Optional[torch.Tensor] = None, window_left: int = -1,
+                 retired_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """kv_append into an 8-bit cache (kv_cache_q8): key/value [T, kvh, D] (bf16 or fp32) are quantised row by row as
+    they are written. A slot may be named once per call. The remaining arguments are those of kv_append."""
+    dev = _one_device(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens,
+                      query_start_loc, retired_out, status)
+    nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, _, tok_stride = _q8_append_args(
+        key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc, retired_out)
+    _call_on(dev, "sbk_kv_append_q8", _ptr(key), _ptr(value), _DTYPE_CODE[key.dtype], _ptr(k_cache), _ptr(v_cache),
+             _ptr(k_scale), _ptr(v_scale), _ptr(slot_mapping), T, kvh, d, tok_stride, nb, bs, cs, ss, _ptr(block_tables),
+             max_blocks, _ptr(seq_lens), _ptr(query_start_loc), B, window_left, _ptr(retired_out), max_ret, _ptr(status))
+
+
+def rope_kv_append_q8(query: Optional[torch.Tensor], key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor,
+                      positions: torch.Tensor, cos_sin_cache: torch.Tensor, *, key_in_place: bool = False,
+                      block_tables: Optional[torch.Tensor] = None, seq_lens: Optional[torch.Tensor] = None,
+                      query_start_loc: Optional[torch.Tensor] = None, window_left: int = -1,
+                      retired_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+    """kv_append_q8 with the NeoX rotary embedding folded in (arguments as in rope_kv_append). The rotation is done in
+    fp32: K is quantised from the fp32 result; ``query`` (and ``key`` with ``key_in_place``) is rounded once to its dtype."""
+    dev = _one_device(query, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, positions, cos_sin_cache,
+                      block_tables, seq_lens, query_start_loc, retired_out, status)
+    nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, es, tok_stride = _q8_append_args(
+        key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc, retired_out)
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype != key.dtype or not cos_sin_cache.is_contiguous():
+        raise ValueError("cos_sin_cache must be contiguous [max_position, rot_dim] in the dtype of key")
+    max_pos, rot_dim = cos_sin_cache.shape
+    if positions.dtype != torch.int64 or positions.numel() != T or not positions.is_contiguous():
+        raise ValueError("positions must be a contiguous int64 tensor with one entry per token")
+    H = q_stride = 0
+    if query is not None:
+        if query.dim() != 3 or query.shape[0] != T or query.shape[2] != d or query.dtype != key.dtype:
+            raise ValueError(f"query must be [T, H, {d}] in the dtype of key")
+        H = query.shape[1]
+        if not _heads_contiguous(query):
+            raise ValueError("query rows must be contiguous")
+        q_stride = (query.stride(0) if T > 1 else H * d) * es
+    _call_on(dev, "sbk_rope_kv_append_q8", _ptr(query), H, q_stride, _ptr(key), _ptr(value), int(key_in_place),
+             _DTYPE_CODE[key.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(slot_mapping),
+             _ptr(positions), _ptr(cos_sin_cache), rot_dim, max_pos, T, kvh, d, tok_stride, nb, bs, cs, ss,
+             _ptr(block_tables), max_blocks, _ptr(seq_lens), _ptr(query_start_loc), B, window_left, _ptr(retired_out),
+             max_ret, _ptr(status))
+
+
+def kv_gather_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 block_tables: torch.Tensor, seq_lens: torch.Tensor, n_out: int, *, window_left: int = -1,
+                 dtype: torch.dtype = torch.bfloat16,
+                 status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Dense head-first values [B, kvh, n_out, D] of every sequence's visible window, as bf16 or fp32 (both exact)."""
+    dev = _one_device(k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, status)
+    nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
+    if dtype not in _DTYPE_CODE:
+        raise ValueError("dtype must be bf16 or fp32")
+    B, max_blocks = block_tables.shape
+    _i32(block_tables, "block_tables")
+    _i32(seq_lens, "seq_lens", B)
+    k_out = torch.empty((B, kvh, n_out, d), dtype=dtype, device=dev)
+    v_out = torch.empty_like(k_out)
+    _call_on(dev, "sbk_kv_gather_q8", _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables),
+             max_blocks, _ptr(seq_lens), B, kvh, d, nb, bs, cs, ss, window_left, _ptr(k_out), _ptr(v_out),
+             _DTYPE_CODE[dtype], n_out, _ptr(status))
+    return k_out, v_out
+
+
+def swa_decode_q8_workspace(B: int, H: int, D: int, device) -> Optional[torch.Tensor]:
+    """Scratch for swa_decode_q8 (None when it needs none). Its contents need no initialisation and mean nothing between
+    calls; calls that can overlap on the GPU (other streams) need one each."""
+    n = _abi.lib.sbk_swa_decode_q8_workspace_bytes(B, H, D)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor, *, window_left: int,
+                  scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                  out_dtype: Optional[torch.dtype] = None, lse: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Single-query sliding-window attention over the 8-bit paged cache; q [B, H, D] bf16. ``lse`` [B, H] fp32 receives the
+    log-sum-exp of the scaled scores. ``workspace`` (swa_decode_q8_workspace): kept by callers that must not allocate."""
+    dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, out, lse, workspace, status)
+    nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != d or q.dtype != torch.bfloat16:
+        raise ValueError(f"q must be bf16 [B, H, {d}]")
+    B, H, _ = q.shape
+    if not _heads_contiguous(q):
+        raise ValueError("the heads of q must be contiguous")
+    if block_tables.dim() != 2 or block_tables.shape[0] != B:
+        raise ValueError("block_tables needs one row per query")
+    _i32(block_tables, "block_tables")
+    _i32(seq_lens, "seq_lens", B)
+    if out is None:
+        out = torch.empty((B, H, d), dtype=out_dtype or torch.bfloat16, device=dev)
+    elif out.shape != (B, H, d) or not _heads_contiguous(out):
+        raise ValueError("out must be [B, H, D] with contiguous heads")
+    if out.dtype not in _DTYPE_CODE:
+        raise ValueError("out must be bf16 or fp32")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
+        raise ValueError("lse must be contiguous fp32 [B, H]")
+    if workspace is None:
+        workspace = swa_decode_q8_workspace(B, H, d, dev)
+    _call_on(dev, "sbk_swa_decode_q8", _ptr(q), q.stride(0) if B > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+             _ptr(v_scale), _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), B, H, kvh, d, nb, bs, cs, ss,
+             window_left, d ** -0.5 if scale is None else float(scale), _ptr(out), _DTYPE_CODE[out.dtype],
+             out.stride(0) if B > 1 else H * d, _ptr(lse), _ptr(workspace),
+             workspace.numel() * workspace.element_size() if workspace is not None else 0, _ptr(status))
+    return out
+
+
+def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                   v_scale: torch.Tensor, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
+                   context_lens: torch.Tensor, max_query_len: int, *, window_left: int, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sliding-window attention of runs of query tokens (q [T, H, D] bf16, token-major) over the 8-bit paged cache, the
+    runs' own K/V already appended; arguments as in swa_prefill."""
+    dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, query_start_loc, context_lens, out, status)
+    nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != d or q.dtype != torch.bfloat16:
+        raise ValueError(f"q must be bf16 [T, H, {d}]")
+    T, H, _ = q.shape
+    if not _heads_contiguous(q):
+        raise ValueError("the heads of q must be contiguous")
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables needs one row per sequence")
+    n_seqs = block_tables.shape[0]
+    _i32(block_tables, "block_tables")
+    _i32(query_start_loc, "query_start_loc", n_seqs + 1)
+    _i32(context_lens, "context_lens", n_seqs)
+    if out is None:
+        out = torch.empty((T, H, d), dtype=torch.bfloat16, device=dev)
+    elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not _heads_contiguous(out):
+        raise ValueError("out must be bf16 [T, H, D] with contiguous heads")
+    _call_on(dev, "sbk_swa_prefill_q8", _ptr(q), q.stride(0) if T > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+             _ptr(v_scale), _ptr(block_tables), block_tables.shape[1], _ptr(query_start_loc), _ptr(context_lens), n_seqs,
+             int(max_query_len), H, kvh, d, nb, bs, cs, ss, window_left, d ** -0.5 if scale is None else float(scale),
+             _ptr(out), out.stride(0) if T > 1 else H * d, _ptr(status))
+    return out
