@@ -291,6 +291,7 @@ int sbk_rope_kv_append(void* query, int H, int64_t q_token_stride_bytes, void* k
  * All four base pointers and both strides are multiples of 16 bytes. e = b - 127 is the smallest integer in [-64, 63] with
  * |x_d| <= 448 * 2^e over the finite values of the row; codes are rounded to nearest even; inf and NaN become the NaN code,
  * magnitudes above 448 * 2^63 saturate. What is stored for a token depends on that token alone. Every value is a bf16 number.
+ * Exponent bytes outside [63, 190] are never written here; what the readers make of them is unspecified.
  *
  * sbk_kv_append_q8: sbk_kv_append with the rows quantised on their way into the cache. key, value [T, kvh, D] of `dtype`
  * (SBK_BF16 or SBK_F32), 16-byte aligned; D of 64, 128 or 256; block_size a multiple of 16; the remaining arguments as in

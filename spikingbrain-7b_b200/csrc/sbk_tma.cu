@@ -28,14 +28,15 @@ static bool encode_map(CUtensorMap* m, const MapKey& k, bool tile_copy) {
   const cuuint64_t row_bytes = k.tok_stride ? (cuuint64_t)k.tok_stride : (cuuint64_t)k.kvh * 256;
   cuuint64_t dim[4], stride[3];
   cuuint32_t box[4], estr[4] = {1, 1, 1, 1};
+  const cuuint64_t rows = k.rows ? (cuuint64_t)k.rows : (cuuint64_t)(2 * k.kvh);
   dim[0] = 64; dim[3] = (cuuint64_t)k.num_blocks;
   stride[2] = (cuuint64_t)k.block_stride;
   if (tile_copy) {
-    dim[1] = (cuuint64_t)k.block_size; dim[2] = 2 * k.kvh;
+    dim[1] = (cuuint64_t)k.block_size; dim[2] = rows;
     stride[0] = row_bytes; stride[1] = 128;
     box[0] = 64; box[1] = 16; box[2] = (cuuint32_t)k.box_rows; box[3] = 1;
   } else {
-    dim[1] = 2 * k.kvh; dim[2] = (cuuint64_t)k.block_size;
+    dim[1] = rows; dim[2] = (cuuint64_t)k.block_size;
     stride[0] = 128; stride[1] = row_bytes;
     box[0] = 64; box[1] = 1; box[2] = 16; box[3] = 1;
   }

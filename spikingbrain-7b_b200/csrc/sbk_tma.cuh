@@ -20,9 +20,11 @@ struct MapKey {
   const void* base; int kvh; int64_t num_blocks; int block_size; int64_t block_stride;
   int box_rows;   // 128-byte rows per tile copy: 2*kvh (all kv heads), 2 (one kv head) or 1 (64 dims)
   int64_t tok_stride = 0;   // bytes between tokens; 0: kvh*256 (rows of a block contiguous)
+  int rows = 0;             // 128-byte rows per token; 0: 2*kvh (bf16, 128 dims). An 8-bit cache has kvh.
   bool operator==(const MapKey& o) const {
     return base == o.base && kvh == o.kvh && num_blocks == o.num_blocks && block_size == o.block_size &&
-           block_stride == o.block_stride && box_rows == o.box_rows && tok_stride == o.tok_stride;
+           block_stride == o.block_stride && box_rows == o.box_rows && tok_stride == o.tok_stride &&
+           rows == o.rows;
   }
 };
 

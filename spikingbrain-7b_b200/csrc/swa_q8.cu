@@ -161,44 +161,6 @@ static int check(const char* who, const Params& P, int D, int n_q, int out_dtype
 }  // namespace attn_q8
 }  // namespace sbk
 
-extern "C" size_t sbk_swa_decode_q8_workspace_bytes(int B, int H, int D) {
-  (void)B; (void)H; (void)D;
-  return 0;
-}
-
-extern "C" int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void* k_cache, const void* v_cache,
-                                 const void* k_scale, const void* v_scale, const int32_t* block_tables, int max_blocks,
-                                 const int32_t* seq_lens, int B, int H, int kvh, int D, int64_t num_blocks,
-                                 int block_size, int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes,
-                                 int window_left, float scale, void* out, int out_dtype, int64_t out_seq_stride,
-                                 float* lse_out, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  using namespace sbk;
-  using namespace sbk::attn_q8;
-  (void)workspace; (void)workspace_bytes;
-  Params P = {};
-  P.q = (const __nv_bfloat16*)q; P.q_stride = q_seq_stride;
-  P.k_cache = (const uint8_t*)k_cache; P.v_cache = (const uint8_t*)v_cache; P.k_scale = (const uint8_t*)k_scale;
-  P.v_scale = (const uint8_t*)v_scale; P.cache_block_stride = cache_block_stride_bytes;
-  P.scale_block_stride = scale_block_stride_bytes; P.block_tables = block_tables; P.max_blocks = max_blocks;
-  P.seq_lens = seq_lens; P.n_seqs = B; P.H = H; P.kvh = kvh; P.num_blocks = num_blocks; P.block_size = block_size;
-  P.window_left = window_left; P.scale_log2 = scale * kLog2e; P.out = out; P.out_stride = out_seq_stride;
-  P.lse_out = lse_out; P.status = status;
-  const int rc = check("sbk_swa_decode_q8", P, D, 1, out_dtype);
-  if (rc != SBK_OK || B == 0) return rc;
-  if (!seq_lens) {
-    set_error("sbk_swa_decode_q8: null pointer");
-    return SBK_E_ARG;
-  }
-  if (B > 65535) {
-    set_error("sbk_swa_decode_q8: B=%d exceeds 65535", B);
-    return SBK_E_ARG;
-  }
-  const dim3 grid(1, kvh, B);
-  if (out_dtype == SBK_BF16) attend_kernel<__nv_bfloat16><<<grid, kTile, 0, (cudaStream_t)stream>>>(P);
-  else attend_kernel<float><<<grid, kTile, 0, (cudaStream_t)stream>>>(P);
-  return check_launch("sbk_swa_decode_q8");
-}
-
 extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const void* k_cache, const void* v_cache,
                                   const void* k_scale, const void* v_scale, const int32_t* block_tables, int max_blocks,
                                   const int32_t* query_start_loc, const int32_t* context_lens, int n_seqs,
