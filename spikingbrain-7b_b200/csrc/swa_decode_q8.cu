@@ -4,21 +4,20 @@
 //
 // Bound by HBM: 2 kvh (D + 1) bytes per visible token, at 14 flops a byte.
 //
-// Products. The codes go into the tensor cores as they are stored (mma.sync m16n8k32, e4m3 x e4m3, exact products and
-//   fp32 sums: measured, no product is cut). The other operand is made 8-bit without losing bits: a bf16 number is the sum of two
-//   e4m3 numbers of four significant bits each, and a kv group has at most eight query heads, so the sixteen rows of the MMA are
-//   the upper parts of eight heads and their remainders:
-//       S[2 x 8, tokens] = [q_hi; q_lo] . K^T        O[2 x 8, dims] = [p_hi; 16 p_lo] . V
-//   and one thread holds both rows of a head. q is scaled by the power of two that takes its largest value under 448; elements far
-//   below it lose what lies under 2^-18 of that value. The padding of the group to eight heads is the only work beyond the formula.
-//   Converting K and V to 16 bits instead would be two thirds of the kernel's instructions.
+// Products. Both run on mma.sync m16n8k16 in fp16, the codes converted in registers on their way into the A operand (exact, two codes
+//   per instruction), K and V taking the 16-row side and the query heads of a kv group (at most eight) the other:
+//       S^T[16 tokens, 8 heads] = K . Q^T            O^T[16 dims, 8 heads] = V^T . W^T
+//   q is scaled by the power of two that takes its largest value under 448: a bf16 number is an fp16 number then (elements below
+//   2^-23 of the largest lose bits no score shows). Feeding the codes to the e4m3 MMA as they are, with query and
+//   probabilities split into two 4-bit parts, takes three times the instructions: the compiler expands that MMA into
+//   conversions of both operands and two fp16 ones (64 mixed sequences: 67 us against 5x us).
 // Softmax. The V scale belongs to the probability's exponent: with m the running maximum of s, the normaliser sums 2^(s_j - m) and
-//   the product takes w_j = 2^(s_j - m + ev_j - r + 8), r the running maximum of s_j - m + ev_j: w <= 256, and its two 4-bit parts
-//   reach down to 2^-13. At the end O * 2^(r - 8) / l.
-// Fragments. Column n of a score tile may be any token, as long as the rows of V come in the order of the probabilities' fragment:
-//   thread t of a quad takes tokens 4t ... 4t+3 of every sixteen, which makes the probabilities the A operand of the second
-//   product without any exchange, the scale bytes of a thread one 32-bit word, and all shared-memory reads conflict-free (eight
-//   rows of a read lie in eight different 16-byte columns of the 128-byte swizzle).
+//   the product takes w_j = 2^(s_j - m + ev_j - r + 8), r the running maximum of s_j - m + ev_j: w <= 256, rounded to fp16's eleven
+//   bits (2^-24 at the least). At the end O * 2^(r - 8) / l.
+// Fragments. The order of tokens inside a tile is free as long as K, the exponents and V agree on it, and so is the order of
+//   dims inside a K = 16 step: a 4-byte word of a row is two adjacent pairs, which become columns 2t, 2t+1 and 2t+8, 2t+9 of the
+//   fragment. Row r of a tile is token r (r < 8) or 8 + (r - 8 ^ 4): the rows of K (plain ldmatrix) and of V (the transposing
+//   8-bit one) then come from eight different 16-byte columns of the 128-byte swizzle, eight rows at a time.
 // Data movement. One producer warp walks the block table and issues a TMA tensor copy per 16 tokens (kvh * 2 KiB of K, the same of V)
 //   and sixteen 16-byte bulk copies of exponents per stage, into a ring of three 32.25 KiB stages; two CTAs per SM. A stage holds 32
 //   tokens per consumer warp: warp w serves kv head w % kvh and the 32-token part w / kvh.
@@ -80,11 +79,22 @@ __device__ __forceinline__ Span span_of(int L, int window_left) {
   return s;
 }
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// words of four codes of rows g (lo) and g + 8 (hi) -> one product: each word holds columns 2t, 2t+1, then 2t+8, 2t+9
+__device__ __forceinline__ void mma_codes(float (&c)[4], uint32_t lo, uint32_t hi, uint32_t b0, uint32_t b1) {
+  mma_f16(c, q8::e4m3x2_to_f16x2(lo & 0xffffu), q8::e4m3x2_to_f16x2(hi & 0xffffu), q8::e4m3x2_to_f16x2(lo >> 16),
+          q8::e4m3x2_to_f16x2(hi >> 16), b0, b1);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 // two 16 x 16 byte matrices, transposed: lane 4g + t gets column g (r0) and g + 8 (r1) of the first, rows 4t ... 4t+3, and the
 // same of the second (r2, r3); lanes 0-15 name the rows of the first matrix, 16-31 those of the second
@@ -95,14 +105,6 @@ __device__ __forceinline__ void ldmatrix_b8_trans(uint32_t (&r)[4], uint32_t add
                : "memory");
 }
 __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
-
-// four floats -> codes of their upper parts and of their remainders * up
-__device__ __forceinline__ void split4(float a, float b, float c, float d, float up, uint32_t& hi, uint32_t& lo) {
-  const uint32_t h0 = q8::pack_e4m3x2(a, b), h1 = q8::pack_e4m3x2(c, d);
-  const float2 f0 = q8::e4m3x2_to_float2(h0), f1 = q8::e4m3x2_to_float2(h1);
-  hi = h0 | (h1 << 16);
-  lo = q8::pack_e4m3x2((a - f0.x) * up, (b - f0.y) * up) | (q8::pack_e4m3x2((c - f1.x) * up, (d - f1.y) * up) << 16);
-}
 
 template <typename TO> __device__ __forceinline__ void store2(TO* p, float a, float b);
 template <> __device__ __forceinline__ void store2<float>(float* p, float a, float b) { p[0] = a; p[1] = b; }
@@ -348,25 +350,21 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   // ================================== consumers ==================================
   const int hk = warp % KVH, sub = warp / KVH, G = P.H / KVH;
   const int g = lane >> 2, t = lane & 3;
-  const bool head_ok = g < G;
   TO* const out = reinterpret_cast<TO*>(P.out);
 
-  // Rows of a [16 tokens][128 B] tile, 16-byte column c of token r at r * 128 + ((c ^ (r & 7)) << 4).
-  // K: lane 8i + n names token tau(tile, n) and column i (+ 4): tile 0 takes tokens 0 1 4 5 10 11 14 15, tile 1 the others
-  const int n8 = lane & 7, i4 = lane >> 3;
-  const int tok0 = 4 * (n8 >> 1) + ((n8 >> 1) & 2) + (n8 & 1), tok1 = tok0 ^ 2;
-  // V: lane r names row kappa = r & 15 of the product, token 4 (kappa / 4) + ..., of the first or second sixteen
-  const int kap = lane & 15;
-  const int tokv = 4 * (kap >> 2) + ((((kap >> 1) & 1) ? 2 : 0) ^ ((kap >> 2) & 2)) + (kap & 1);
+  // A tile is [16 tokens][128 B], 16-byte column c of token r at r * 128 + ((c ^ (r & 7)) << 4).
+  // K: lanes 0-7 and 8-15 name rows 0-7 and 8-15 at column c, lanes 16-31 the same rows at column c + 1
+  const int rk = lane & 15, tokk = rk < 8 ? rk : 8 + ((rk - 8) ^ 4);
+  // V: lane r (of each sixteen) names row r of the product, whose words run over rows 2t, 2t+1, 8+2t, 9+2t of the scores
+  const int rv = 2 * (rk >> 2) + (rk & 1) + ((rk & 2) << 2), tokv = rv < 8 ? rv : 8 + ((rv - 8) ^ 4);
   const uint32_t tile0 = (uint32_t)(sub * 2 * kChunkBytes + hk * 2048);        // this warp's first sixteen tokens, its head
-  const uint32_t k0 = tile0 + tok0 * 128, k1 = tile0 + tok1 * 128;
-  const uint32_t v0 = kTileBytes + tile0 + (lane >> 4) * kChunkBytes + tokv * 128;
-  const int pa = 4 * t + (t & 2), pb = pa ^ 2;     // a thread's tokens in score tile 0 (pa, pa + 1) and tile 1 (pb, pb + 1)
-  const int sh = t & 2 ? 16 : 0;                   // bit position of tile 0's pair in the thread's word of exponents
+  const uint32_t k0 = tile0 + tokk * 128, v0 = kTileBytes + tile0 + tokv * 128;
+  const int xk = (tokk & 7) ^ (lane >> 4), xv = (tokv & 7) ^ (lane >> 4);
+  const int ta = g, tb8 = 8 + (g ^ 4);             // a thread's tokens in every sixteen
 
-  uint32_t qf[4][4];
-  float acc[16][4];
-  float m = -INFINITY, l = 0.f, r = -INFINITY, qs = 0.f;
+  uint32_t qf[8][2];
+  float acc[8][4];
+  float m[2], l[2], r[2], qs[2];                   // of heads 2t, 2t + 1
   for (int it = 0;; ++it) {
     const int s = it % kStages;
     if (!mbar_wait_bounded(bar_full + 8 * s, (it / kStages) & 1)) {
@@ -378,13 +376,14 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     const uint32_t stage = ring + s * kStageBytes;
 
     if (si.flags & kFirst) {
-      // q of head g, dims 32 kk + 4t ... + 3 and 32 kk + 16 + 4t ... + 3
+      // q of head g: dims 16c + 4t ... + 3
+      const bool head_ok = g < G;
       const __nv_bfloat16* qp = P.q + (int64_t)si.b * P.q_stride + (int64_t)(hk * G + (head_ok ? g : 0)) * kD + 4 * t;
       uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[2 * i] = *reinterpret_cast<const uint32_t*>(qp + 16 * i);
-        w[2 * i + 1] = *reinterpret_cast<const uint32_t*>(qp + 16 * i + 2);
+      for (int c = 0; c < 8; ++c) {
+        w[2 * c] = *reinterpret_cast<const uint32_t*>(qp + 16 * c);
+        w[2 * c + 1] = *reinterpret_cast<const uint32_t*>(qp + 16 * c + 2);
       }
       float top = 0.f;
 #pragma unroll
@@ -396,20 +395,18 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = q8::row_exponent(top);
-      const float inv = q8::pow2i(-e);
-      qs = P.scale_log2 * q8::pow2i(e);
+      const float inv = q8::pow2i(-e), mine = P.scale_log2 * q8::pow2i(e);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float x[4] = {__uint_as_float(w[2 * i] << 16), __uint_as_float(w[2 * i] & 0xffff0000u),
-                      __uint_as_float(w[2 * i + 1] << 16), __uint_as_float(w[2 * i + 1] & 0xffff0000u)};
+      for (int i = 0; i < 16; ++i)           // (an infinity stays one, or becomes one: the head's scores are NaN or infinite)
+        qf[i >> 1][i & 1] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = q8::finite(x[j]) ? x[j] * inv : __uint_as_float(0x7fffffffu);
-        split4(x[0], x[1], x[2], x[3], 1.f, qf[i >> 1][2 * (i & 1)], qf[i >> 1][2 * (i & 1) + 1]);
+      for (int i = 0; i < 2; ++i) {
+        qs[i] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + i));
+        m[i] = r[i] = -INFINITY;
+        l[i] = 0.f;
       }
 #pragma unroll
-      for (int nt = 0; nt < 16; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-      m = r = -INFINITY;
-      l = 0.f;
+      for (int mt = 0; mt < 8; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
     }
 
     const int tb = si.tok_base + 32 * sub;                      // my 32 tokens
@@ -418,172 +415,161 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       const bool ragged = vlo > tb || vhi < tb + 32;
       if (ragged) {
         // rows outside the visible range hold anything, or older data: a zero probability must not meet a NaN code
-        for (int r = lane >> 3; r < 32; r += 4)
-          if (tb + r < vlo || tb + r >= vhi)
-            *reinterpret_cast<uint4*>(smem + s * kStageBytes + kTileBytes + tile0 + (r >> 4) * kChunkBytes + (r & 15) * 128 +
+        for (int row = lane >> 3; row < 32; row += 4)
+          if (tb + row < vlo || tb + row >= vhi)
+            *reinterpret_cast<uint4*>(smem + s * kStageBytes + kTileBytes + tile0 + (row >> 4) * kChunkBytes + (row & 15) * 128 +
                                       (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
-      // ---- scores of 32 tokens: tiles 0, 1 of the first sixteen, 2, 3 of the second ----
-      float sc[8];                                              // [16-token half][tile][pair]
+      // ---- scores: [16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
+      float sc[2][4], ev[2][2];
+      const uint8_t* se = smem + kScaleOff + s * kScaleBytes + (sub * KVH + hk) * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+        float ca[4] = {0.f, 0.f, 0.f, 0.f}, cb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          uint32_t b[4];
-          ldmatrix_x4(b, stage + h * kChunkBytes + k0 + (((4 * f + i4) ^ (tok0 & 7)) << 4));
-          mma_e4m3(c0, qf[2 * f], b[0], b[1]);
-          mma_e4m3(c0, qf[2 * f + 1], b[2], b[3]);
-          ldmatrix_x4(b, stage + h * kChunkBytes + k1 + (((4 * f + i4) ^ (tok1 & 7)) << 4));
-          mma_e4m3(c1, qf[2 * f], b[0], b[1]);
-          mma_e4m3(c1, qf[2 * f + 1], b[2], b[3]);
+        for (int c = 0; c < 8; c += 2) {
+          uint32_t w[4];
+          ldmatrix_x4(w, stage + h * kChunkBytes + k0 + ((c ^ xk) << 4));
+          mma_codes(ca, w[0], w[1], qf[c][0], qf[c][1]);
+          mma_codes(cb, w[2], w[3], qf[c + 1][0], qf[c + 1][1]);
         }
-        sc[4 * h] = c0[0] + c0[2]; sc[4 * h + 1] = c0[1] + c0[3];
-        sc[4 * h + 2] = c1[0] + c1[2]; sc[4 * h + 3] = c1[1] + c1[3];
-      }
-      float ev[8];
-      {
-        const uint8_t* se = smem + kScaleOff + s * kScaleBytes + (sub * KVH + hk) * 32 + 4 * t;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t kb = *reinterpret_cast<const uint32_t*>(se + 16 * h);
-          const uint32_t vb = *reinterpret_cast<const uint32_t*>(se + 128 + 16 * h);
-          const uint32_t kw[2] = {kb >> sh, kb >> (16 - sh)}, vw[2] = {vb >> sh, vb >> (16 - sh)};
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            sc[4 * h + 2 * i] *= qs * __uint_as_float((kw[i] & 255u) << 23);
-            sc[4 * h + 2 * i + 1] *= qs * __uint_as_float((kw[i] & 0xff00u) << 15);
-            // byte - 127, through the low bits of a float: 2^23 + byte
-            ev[4 * h + 2 * i] = __uint_as_float(0x4b000000u | (vw[i] & 255u)) - 8388735.f;
-            ev[4 * h + 2 * i + 1] = __uint_as_float(0x4b000000u | ((vw[i] >> 8) & 255u)) - 8388735.f;
-          }
+        const float ka = __uint_as_float((uint32_t)se[16 * h + ta] << 23), kb = __uint_as_float((uint32_t)se[16 * h + tb8] << 23);
+        sc[h][0] = (ca[0] + cb[0]) * (qs[0] * ka); sc[h][1] = (ca[1] + cb[1]) * (qs[1] * ka);
+        sc[h][2] = (ca[2] + cb[2]) * (qs[0] * kb); sc[h][3] = (ca[3] + cb[3]) * (qs[1] * kb);
+        // byte - 127, through the low bits of a float: 2^23 + byte
+        ev[h][0] = __uint_as_float(0x4b000000u | se[128 + 16 * h + ta]) - 8388735.f;
+        ev[h][1] = __uint_as_float(0x4b000000u | se[128 + 16 * h + tb8]) - 8388735.f;
+        if (ragged) {
+          const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
+          if (a < vlo || a >= vhi) { sc[h][0] = sc[h][1] = -INFINITY; ev[h][0] = 0.f; }
+          if (b < vlo || b >= vhi) { sc[h][2] = sc[h][3] = -INFINITY; ev[h][1] = 0.f; }
         }
       }
-      if (ragged) {
+      // ---- running maxima: m of s, and r of (s - m) + ev, which moves with m (s + ev itself would lose ev beside a large s) ----
+      float mx[2], back[2], w[2][4], mx2[2], al2[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mx[i] = fmaxf(fmaxf(sc[0][i], sc[0][2 + i]), fmaxf(sc[1][i], sc[1][2 + i]));
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float mn = fmaxf(m[i], mx[i]), ms = fmaxf(mn, kNegBig);
+        back[i] = m[i] - ms;
+        m[i] = mn;
+        float ls = 0.f;
+        mx2[i] = -INFINITY;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int tok = tb + 16 * h + (i < 2 ? pa : pb) + (i & 1);
-            if (tok < vlo || tok >= vhi) { sc[4 * h + i] = -INFINITY; ev[4 * h + i] = 0.f; }
+          for (int k = 0; k < 2; ++k) {
+            const float d = sc[h][2 * k + i] - ms;
+            w[h][2 * k + i] = d + ev[h][k];
+            mx2[i] = fmaxf(mx2[i], w[h][2 * k + i]);
+            ls += fast_exp2(d);
           }
-      }
-      // ---- running maxima: m of s, and r of (s - m) + ev, which moves with m (s + ev itself would lose ev beside a large s) ----
-      float mx = sc[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i]);
-#pragma unroll
-      for (int off = 1; off < 4; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-      const float mn = fmaxf(m, mx), ms = fmaxf(mn, kNegBig);
-      const float back = m - ms;
-      const float al = fast_exp2(back);
-      m = mn;
-      float w[8], mx2 = -INFINITY, ls = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = sc[i] - ms;
-        w[i] = d + ev[i];
-        mx2 = fmaxf(mx2, w[i]);
-        ls += fast_exp2(d);
+        l[i] = l[i] * fast_exp2(back[i]) + ls;
       }
 #pragma unroll
-      for (int off = 1; off < 4; off <<= 1) mx2 = fmaxf(mx2, __shfl_xor_sync(0xffffffffu, mx2, off));
-      const float ro = r + back, rn = fmaxf(fmaxf(ro, mx2), kNegBig);
-      const float al2 = fast_exp2(ro - rn);
-      r = rn;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = fast_exp2(w[i] - (rn - 8.f));
-      l = l * al + ls;
-      if (__any_sync(0xffffffffu, al2 != 1.f)) {
-#pragma unroll
-        for (int nt = 0; nt < 16; ++nt) { acc[nt][0] *= al2; acc[nt][1] *= al2; acc[nt][2] *= al2; acc[nt][3] *= al2; }
+      for (int off = 4; off < 32; off <<= 1) {
+        mx2[0] = fmaxf(mx2[0], __shfl_xor_sync(0xffffffffu, mx2[0], off));
+        mx2[1] = fmaxf(mx2[1], __shfl_xor_sync(0xffffffffu, mx2[1], off));
       }
-      uint32_t pf[4];
-      split4(w[0], w[1], w[2], w[3], 16.f, pf[0], pf[1]);
-      split4(w[4], w[5], w[6], w[7], 16.f, pf[2], pf[3]);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t b[4];
-        ldmatrix_b8_trans(b, stage + v0 + ((c ^ (tokv & 7)) << 4));
-        mma_e4m3(acc[2 * c], pf, b[0], b[2]);
-        mma_e4m3(acc[2 * c + 1], pf, b[1], b[3]);
+      for (int i = 0; i < 2; ++i) {
+        const float ro = r[i] + back[i], rn = fmaxf(fmaxf(ro, mx2[i]), kNegBig);
+        al2[i] = fast_exp2(ro - rn);
+        r[i] = rn;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          w[h][i] = fast_exp2(w[h][i] - (rn - 8.f));
+          w[h][2 + i] = fast_exp2(w[h][2 + i] - (rn - 8.f));
+        }
+      }
+      if (__any_sync(0xffffffffu, al2[0] != 1.f || al2[1] != 1.f)) {
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) { acc[mt][0] *= al2[0]; acc[mt][1] *= al2[1]; acc[mt][2] *= al2[0]; acc[mt][3] *= al2[1]; }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t p0 = movmatrix_trans(pack_f16x2(w[h][0], w[h][1])), p1 = movmatrix_trans(pack_f16x2(w[h][2], w[h][3]));
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+          uint32_t v[4];
+          ldmatrix_b8_trans(v, stage + h * kChunkBytes + v0 + ((c ^ xv) << 4));
+          mma_codes(acc[c], v[0], v[1], p0, p1);
+          mma_codes(acc[c + 1], v[2], v[3], p0, p1);
+        }
       }
       if (ragged) fence_proxy_async_smem();   // my zero fill precedes the next copy into these rows
     }
     __syncwarp();
-    const bool keep_stage = kSub > 1 && (si.flags & kLast);     // becomes the merge scratch first
-    if (lane == 0 && !keep_stage) mbar_arrive(bar_empty + 8 * s);
+    // the last stage of an item becomes the scratch of its output before it goes back to the producer
+    if (lane == 0 && !(si.flags & kLast)) mbar_arrive(bar_empty + 8 * s);
     if (!(si.flags & kLast)) continue;
 
     // ================= end of an item: its output row, or its partial =================
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
     // O relative to m (0 where nothing was visible; a NaN score has made O and l NaN already)
-    const float fix = r > kNegBig ? exp2f(r - 8.f) : 0.f;
-    const int64_t prow = (int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * P.H;
-    if constexpr (kSub == 1) {
-      if (head_ok) {
-        const int h = hk * G + g;
-        if (si.part < 0) {
-          const float f = fix * inverse(l);
-          TO* op = out + (int64_t)si.b * P.out_stride + (int64_t)h * kD + 2 * t;
+    float fix[2];
 #pragma unroll
-          for (int nt = 0; nt < 16; ++nt)
-            store2(op + 8 * nt, (acc[nt][0] + acc[nt][2] * 0.0625f) * f, (acc[nt][1] + acc[nt][3] * 0.0625f) * f);
-          if (P.lse_out && t == 0) P.lse_out[(int64_t)si.b * P.H + h] = row_lse(m, l);
-        } else {
-          float* wp = P.ws_o + (prow + h) * kD + 2 * t;
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-          for (int nt = 0; nt < 16; ++nt)
-            *reinterpret_cast<float2*>(wp + 8 * nt) =
-                make_float2((acc[nt][0] + acc[nt][2] * 0.0625f) * fix, (acc[nt][1] + acc[nt][3] * 0.0625f) * fix);
-          if (t == 0) P.ws_ml[prow + h] = make_float2(m, l);
-        }
-      }
-    } else {
-      // several warps share a kv head (each took other tokens): merge through the stage just consumed
-      uint8_t* mbuf = smem + s * kStageBytes;
-      float* wo = reinterpret_cast<float*>(mbuf + warp * kMergeWarpBytes);
-      float* wml = wo + kMaxG * kHeadStride;
-      consumer_bar();                       // every warp is done reading this stage
-#pragma unroll
-      for (int nt = 0; nt < 16; ++nt)
-        *reinterpret_cast<float2*>(wo + g * kHeadStride + 8 * nt + 2 * t) =
-            make_float2((acc[nt][0] + acc[nt][2] * 0.0625f) * fix, (acc[nt][1] + acc[nt][3] * 0.0625f) * fix);
-      if (t == 0) { wml[g] = m; wml[8 + g] = l; }
-      consumer_bar();
-      for (int h = warp; h < P.H; h += kConsumerWarps) {
-        const int kh = h / G, r = h - kh * G;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w2 = 0; w2 < kSub; ++w2)
-          M = fmaxf(M, reinterpret_cast<const float*>(mbuf + (kh + KVH * w2) * kMergeWarpBytes)[kMaxG * kHeadStride + r]);
-        const float Ms = fmaxf(M, kNegBig);
-        float L = 0.f;
-        float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w2 = 0; w2 < kSub; ++w2) {
-          const float* po = reinterpret_cast<const float*>(mbuf + (kh + KVH * w2) * kMergeWarpBytes);
-          const float wgt = fast_exp2(po[kMaxG * kHeadStride + r] - Ms);
-          const float4 o = *reinterpret_cast<const float4*>(po + r * kHeadStride + 4 * lane);
-          L += po[kMaxG * kHeadStride + 8 + r] * wgt;
-          O.x += o.x * wgt; O.y += o.y * wgt; O.z += o.z * wgt; O.w += o.w * wgt;
-        }
-        if (si.part < 0) {
-          const float f = inverse(L);
-          store4(out + (int64_t)si.b * P.out_stride + (int64_t)h * kD + 4 * lane,
-                 make_float4(O.x * f, O.y * f, O.z * f, O.w * f));
-          if (P.lse_out && lane == 0) P.lse_out[(int64_t)si.b * P.H + h] = row_lse(M, L);
-        } else {
-          *reinterpret_cast<float4*>(P.ws_o + (prow + h) * kD + 4 * lane) = O;
-          if (lane == 0) P.ws_ml[prow + h] = make_float2(M, L);
-        }
-      }
-      fence_proxy_async_smem();             // these writes precede the copies that refill the stage
-      consumer_bar();
-      if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+      for (int off = 4; off < 32; off <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
+      fix[i] = r[i] > kNegBig ? exp2f(r[i] - 8.f) : 0.f;
     }
+    const int64_t prow = (int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * P.H;
+    // [head][dim] floats of every warp in shared memory; warps that share a kv head (each took other tokens) are added up here
+    uint8_t* mbuf = smem + s * kStageBytes;
+    float* wo = reinterpret_cast<float*>(mbuf + warp * kMergeWarpBytes);
+    float* wml = wo + kMaxG * kHeadStride;
+    consumer_bar();                         // every warp is done reading this stage
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        wo[(2 * t + i) * kHeadStride + 16 * mt + g] = acc[mt][i] * fix[i];
+        wo[(2 * t + i) * kHeadStride + 16 * mt + g + 8] = acc[mt][2 + i] * fix[i];
+      }
+    if (g == 0) {
+      wml[2 * t] = m[0]; wml[2 * t + 1] = m[1];
+      wml[8 + 2 * t] = l[0]; wml[8 + 2 * t + 1] = l[1];
+    }
+    if constexpr (kSub > 1) consumer_bar(); else __syncwarp();
+    // heads go round the warps (one warp to a kv head: its own heads), a lane takes four dims
+    const int h_lo = kSub > 1 ? warp : hk * G, h_hi = kSub > 1 ? P.H : hk * G + G, h_step = kSub > 1 ? kConsumerWarps : 1;
+#pragma unroll 2
+    for (int h = h_lo; h < h_hi; h += h_step) {
+      const int kh = h / G, row = h - kh * G;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w2 = 0; w2 < kSub; ++w2)
+        M = fmaxf(M, reinterpret_cast<const float*>(mbuf + (kh + KVH * w2) * kMergeWarpBytes)[kMaxG * kHeadStride + row]);
+      const float Ms = fmaxf(M, kNegBig);
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w2 = 0; w2 < kSub; ++w2) {
+        const float* po = reinterpret_cast<const float*>(mbuf + (kh + KVH * w2) * kMergeWarpBytes);
+        const float wgt = kSub > 1 ? fast_exp2(po[kMaxG * kHeadStride + row] - Ms) : 1.f;
+        const float4 o = *reinterpret_cast<const float4*>(po + row * kHeadStride + 4 * lane);
+        L += po[kMaxG * kHeadStride + 8 + row] * wgt;
+        O.x += o.x * wgt; O.y += o.y * wgt; O.z += o.z * wgt; O.w += o.w * wgt;
+      }
+      if (si.part < 0) {
+        const float f = inverse(L);
+        store4(out + (int64_t)si.b * P.out_stride + (int64_t)h * kD + 4 * lane, make_float4(O.x * f, O.y * f, O.z * f, O.w * f));
+        if (P.lse_out && lane == 0) P.lse_out[(int64_t)si.b * P.H + h] = row_lse(M, L);
+      } else {
+        *reinterpret_cast<float4*>(P.ws_o + (prow + h) * kD + 4 * lane) = O;
+        if (lane == 0) P.ws_ml[prow + h] = make_float2(M, L);
+      }
+    }
+    fence_proxy_async_smem();               // these accesses precede the copies that refill the stage
+    if constexpr (kSub > 1) consumer_bar(); else __syncwarp();
+    if (lane == 0) mbar_arrive(bar_empty + 8 * s);
   }
 }
 
