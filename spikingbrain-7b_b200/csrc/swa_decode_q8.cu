@@ -11,21 +11,25 @@
 //   2^-23 of the largest lose bits no score shows). Feeding the codes to the e4m3 MMA as they are, with query and
 //   probabilities split into two 4-bit parts, takes three times the instructions: the compiler expands that MMA into
 //   conversions of both operands and two fp16 ones (64 mixed sequences: 67 us against 5x us).
-// Softmax. The V scale belongs to the probability's exponent: with m the running maximum of s, the normaliser sums 2^(s_j - m) and
-//   the product takes w_j = 2^(s_j - m + ev_j - r + 8), r the running maximum of s_j - m + ev_j: w <= 256, rounded to fp16's eleven
-//   bits (2^-24 at the least). At the end O * 2^(r - 8) / l.
+// Softmax. The V scale belongs to the probability's exponent: with an offset m per head the normaliser sums p_j = 2^(s_j - m), and
+//   the product takes w_j = p_j 2^(ev_j - r), rounded to fp16's eleven bits. m and r are not the running maxima: they move only
+//   when a w would leave fp16 (or p grow past 2^40), to put the largest w of the item between 2^6 and 2^7; until the
+//   next move w may grow to 2^15, and the smallest fp16 number is 2^-30 of the largest w at the most. So a step costs one
+//   vote where maxima over the tokens would cost twelve shuffles. At the end O * 2^r / l.
 // Fragments. The order of tokens inside a tile is free as long as K, the exponents and V agree on it, and so is the order of
 //   dims inside a K = 16 step: a 4-byte word of a row is two adjacent pairs, which become columns 2t, 2t+1 and 2t+8, 2t+9 of the
 //   fragment. Row r of a tile is token r (r < 8) or 8 + (r - 8 ^ 4): the rows of K (plain ldmatrix) and of V (the transposing
 //   8-bit one) then come from eight different 16-byte columns of the 128-byte swizzle, eight rows at a time.
 // Data movement. One producer warp walks the block table and issues a TMA tensor copy per 16 tokens (kvh * 2 KiB of K, the same of V)
-//   and sixteen 16-byte bulk copies of exponents per stage, into a ring of three 32.25 KiB stages; two CTAs per SM. A stage holds 32
+//   into a ring of three 32 KiB stages; two CTAs per SM. The exponents, 16 bytes per head and 16 tokens, come beside them through
+//   the load path (cp.async): as bulk copies they took four of five requests of the copy engine (XX us). A stage holds 32
 //   tokens per consumer warp: warp w serves kv head w % kvh and the 32-token part w / kvh.
 // Partition. The units (one stage of tokens each) of all sequences, laid end to end with a fixed charge per sequence, are cut
 //   into one equal run per CTA. Only the first and the last sequence of a run can be cut, so a CTA writes at most two partial results
 //   (m, l, O): the workspace is indexed by CTA, holds nothing between calls and needs no clearing. A second kernel, launched
 //   ahead of the first one's end (programmatic dependent launch), folds the partials: no counters, no waits between CTAs.
 #include "kv_q8.cuh"
+#include "sbk_tcgen05.cuh"
 #include "sbk_tma.cuh"
 
 namespace sbk {
@@ -43,6 +47,7 @@ constexpr int kScaleBytes = 256;      // exponents of a stage: 128 of K, 128 of 
 constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kHeadStride = 132;      // floats per head row of the merge scratch (bank skew)
 constexpr int kMergeWarpBytes = kMaxG * kHeadStride * 4 + 64;
+constexpr float kMostW = 32768.f, kMostP = 1.099511627776e12f;   // 2^15, 2^40: where the offsets of the softmax move
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kNegBig = -1.0e30f;
 enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8 };
 
@@ -104,6 +109,13 @@ __device__ __forceinline__ void ldmatrix_b8_trans(uint32_t (&r)[4], uint32_t add
                : "r"(addr)
                : "memory");
 }
+// 16 bytes global -> shared through the load path, and the arrival of a lane's copies on a barrier
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
 
 template <typename TO> __device__ __forceinline__ void store2(TO* p, float a, float b);
@@ -144,7 +156,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_full + 8 * s, 1 + 32);   // the stage's bytes, and each producer lane's exponents
       mbar_init(bar_empty + 8 * s, kConsumerWarps);
     }
     misc[0] = 0;
@@ -258,7 +270,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           si.flags = (j == 0 ? kFirst : 0) | (j == n - 1 ? kLast : 0) | (bad ? kBad : 0);
           info[s] = si;
           if (bad) raise_status(P.status, SBK_ST_BAD_BLOCK);
-          mbar_arrive_expect_tx(bar_full + 8 * s, bad ? 0u : (uint32_t)(cb - ca) * 2u * (kChunkBytes + KVH * kChunk));
+          mbar_arrive_expect_tx(bar_full + 8 * s, bad ? 0u : (uint32_t)(cb - ca) * 2u * kChunkBytes);
         }
         __syncwarp();
         if (!bad && in) {
@@ -269,8 +281,8 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
             const int64_t at = pb * P.scale_block_stride + (int64_t)h * P.block_size + tin;
             const uint32_t dst = ring + kScaleOff + s * kScaleBytes + (((c >> 1) * KVH + h) * 2 + (c & 1)) * 16;
             if (x < kChunks * KVH) {
-              bulk_g2s(dst, P.k_scale + at, 16, bar);
-              bulk_g2s(dst + 128, P.v_scale + at, 16, bar);
+              cp_async16(dst, P.k_scale + at);
+              cp_async16(dst + 128, P.v_scale + at);
             }
           } else if (x < kChunks) {
             const uint32_t dst = ring + s * kStageBytes + c * kChunkBytes;
@@ -285,6 +297,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
             }
           }
         }
+        cp_async_arrive(bar_full + 8 * s);
       }
     };
 
@@ -332,10 +345,10 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       // the end marker travels through the ring like any stage
       const int s = it % kStages, use = it / kStages;
       if (use == 0 || mbar_wait_bounded(bar_empty + 8 * s, (use - 1) & 1)) {
-        if (lane == 0) {
-          info[s].flags = kEnd;
-          mbar_arrive_expect_tx(bar_full + 8 * s, 0u);
-        }
+        if (lane == 0) info[s].flags = kEnd;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bar_full + 8 * s, 0u);
+        mbar_arrive(bar_full + 8 * s);
       } else if (lane == 0) {
         raise_status(P.status, SBK_ST_WAIT_TIMEOUT);
         misc[0] = 1;
@@ -364,7 +377,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 
   uint32_t qf[8][2];
   float acc[8][4];
-  float m[2], l[2], r[2], qs[2];                   // of heads 2t, 2t + 1
+  float m[2], l[2], rs[2], qs[2];                  // of heads 2t, 2t + 1 (rs = 2^-r)
   for (int it = 0;; ++it) {
     const int s = it % kStages;
     if (!mbar_wait_bounded(bar_full + 8 * s, (it / kStages) & 1)) {
@@ -402,8 +415,9 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         qs[i] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + i));
-        m[i] = r[i] = -INFINITY;
+        m[i] = kNegBig;
         l[i] = 0.f;
+        rs[i] = 1.f;
       }
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
@@ -421,11 +435,15 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                                       (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
-      // ---- scores: [16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
-      float sc[2][4], ev[2][2];
+      // ---- scores (without the scales): [16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
+      float sc[2][4], kv[2][2], ve[2][2];
       const uint8_t* se = smem + kScaleOff + s * kScaleBytes + (sub * KVH + hk) * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        kv[h][0] = __uint_as_float((uint32_t)se[16 * h + ta] << 23);
+        kv[h][1] = __uint_as_float((uint32_t)se[16 * h + tb8] << 23);
+        ve[h][0] = __uint_as_float((uint32_t)se[128 + 16 * h + ta] << 23);
+        ve[h][1] = __uint_as_float((uint32_t)se[128 + 16 * h + tb8] << 23);
         float ca[4] = {0.f, 0.f, 0.f, 0.f}, cb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
@@ -434,64 +452,77 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           mma_codes(ca, w[0], w[1], qf[c][0], qf[c][1]);
           mma_codes(cb, w[2], w[3], qf[c + 1][0], qf[c + 1][1]);
         }
-        const float ka = __uint_as_float((uint32_t)se[16 * h + ta] << 23), kb = __uint_as_float((uint32_t)se[16 * h + tb8] << 23);
-        sc[h][0] = (ca[0] + cb[0]) * (qs[0] * ka); sc[h][1] = (ca[1] + cb[1]) * (qs[1] * ka);
-        sc[h][2] = (ca[2] + cb[2]) * (qs[0] * kb); sc[h][3] = (ca[3] + cb[3]) * (qs[1] * kb);
-        // byte - 127, through the low bits of a float: 2^23 + byte
-        ev[h][0] = __uint_as_float(0x4b000000u | se[128 + 16 * h + ta]) - 8388735.f;
-        ev[h][1] = __uint_as_float(0x4b000000u | se[128 + 16 * h + tb8]) - 8388735.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[h][i] = (ca[i] + cb[i]) * (qs[i & 1] * kv[h][i >> 1]);
         if (ragged) {
           const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
-          if (a < vlo || a >= vhi) { sc[h][0] = sc[h][1] = -INFINITY; ev[h][0] = 0.f; }
-          if (b < vlo || b >= vhi) { sc[h][2] = sc[h][3] = -INFINITY; ev[h][1] = 0.f; }
+          if (a < vlo || a >= vhi) { sc[h][0] = sc[h][1] = -INFINITY; ve[h][0] = 0.f; }
+          if (b < vlo || b >= vhi) { sc[h][2] = sc[h][3] = -INFINITY; ve[h][1] = 0.f; }
         }
       }
-      // ---- running maxima: m of s, and r of (s - m) + ev, which moves with m (s + ev itself would lose ev beside a large s) ----
-      float mx[2], back[2], w[2][4], mx2[2], al2[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) mx[i] = fmaxf(fmaxf(sc[0][i], sc[0][2 + i]), fmaxf(sc[1][i], sc[1][2 + i]));
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float mn = fmaxf(m[i], mx[i]), ms = fmaxf(mn, kNegBig);
-        back[i] = m[i] - ms;
-        m[i] = mn;
-        float ls = 0.f;
-        mx2[i] = -INFINITY;
+      // ---- p = 2^(s - m), w = p * 2^(ev - r) with the offsets in use; they move only when a w leaves fp16 ----
+      float p[2][4], w[2][4], wtop, ptop;
+      auto weigh = [&]() {
+        wtop = ptop = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float d = sc[h][2 * k + i] - ms;
-            w[h][2 * k + i] = d + ev[h][k];
-            mx2[i] = fmaxf(mx2[i], w[h][2 * k + i]);
-            ls += fast_exp2(d);
+          for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+            for (int j = i; j < i + 2; ++j) {
+              p[h][j] = fast_exp2(sc[h][j] - m[j & 1]);
+              w[h][j] = p[h][j] * (ve[h][j >> 1] * rs[j & 1]);
+            }
+            wtop = tc5::fmax3(wtop, w[h][i], w[h][i + 1]);
+            ptop = tc5::fmax3(ptop, p[h][i], p[h][i + 1]);
           }
-        l[i] = l[i] * fast_exp2(back[i]) + ls;
-      }
+      };
+      weigh();
+      if (__any_sync(0xffffffffu, wtop > kMostW || ptop > kMostP)) {
+        // (rare: the first tokens of an item, and where a score or a V row outgrows all before it by 2^8)
+        float mx[2], ne[2];
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        mx2[0] = fmaxf(mx2[0], __shfl_xor_sync(0xffffffffu, mx2[0], off));
-        mx2[1] = fmaxf(mx2[1], __shfl_xor_sync(0xffffffffu, mx2[1], off));
-      }
+        for (int i = 0; i < 2; ++i) mx[i] = fmaxf(fmaxf(sc[0][i], sc[0][2 + i]), fmaxf(sc[1][i], sc[1][2 + i]));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float ro = r[i] + back[i], rn = fmaxf(fmaxf(ro, mx2[i]), kNegBig);
-        al2[i] = fast_exp2(ro - rn);
-        r[i] = rn;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          w[h][i] = fast_exp2(w[h][i] - (rn - 8.f));
-          w[h][2 + i] = fast_exp2(w[h][2 + i] - (rn - 8.f));
+        for (int off = 4; off < 32; off <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
         }
-      }
-      if (__any_sync(0xffffffffu, al2[0] != 1.f || al2[1] != 1.f)) {
 #pragma unroll
-        for (int mt = 0; mt < 8; ++mt) { acc[mt][0] *= al2[0]; acc[mt][1] *= al2[1]; acc[mt][2] *= al2[0]; acc[mt][3] *= al2[1]; }
+        for (int i = 0; i < 2; ++i) {
+          const float mn = fmaxf(m[i], mx[i]);
+          ne[i] = fast_exp2(m[i] - mn);
+          l[i] *= ne[i];
+          m[i] = mn;
+          mx[i] = 0.f;                        // from here on: the largest p * 2^ev
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            mx[i] = fmaxf(mx[i], fast_exp2(sc[h][i] - mn) * ve[h][0]);
+            mx[i] = fmaxf(mx[i], fast_exp2(sc[h][2 + i] - mn) * ve[h][1]);
+          }
+        }
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // 2^-r: the power of two that takes the largest w so far to [2^6, 2^7) (those before had one of 2^6 at least)
+          const float had = ne[i] * 64.f / rs[i];
+          int e = (int)(__float_as_uint(fmaxf(mx[i], had)) >> 23) - 127;
+          e = e < -64 ? -64 : (e > 63 ? 63 : e);
+          const float rn = q8::pow2i(6 - e), al = ne[i] * (rn / rs[i]);
+          rs[i] = rn;
+#pragma unroll
+          for (int mt = 0; mt < 8; ++mt) { acc[mt][i] *= al; acc[mt][2 + i] *= al; }
+        }
+        weigh();
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[0] += p[h][0] + p[h][2];
+        l[1] += p[h][1] + p[h][3];
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -512,13 +543,13 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     if (!(si.flags & kLast)) continue;
 
     // ================= end of an item: its output row, or its partial =================
-    // O relative to m (0 where nothing was visible; a NaN score has made O and l NaN already)
+    // (where nothing was visible m is kNegBig, l and O are 0)
     float fix[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-      fix[i] = r[i] > kNegBig ? exp2f(r[i] - 8.f) : 0.f;
+      fix[i] = 1.f / rs[i];
     }
     const int64_t prow = (int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * P.H;
     // [head][dim] floats of every warp in shared memory; warps that share a kv head (each took other tokens) are added up here
