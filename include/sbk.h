@@ -328,10 +328,13 @@ int sbk_kv_gather_q8(const void* k_cache, const void* v_cache, const void* k_sca
  * query tokens) with the cache as above. q bf16; a query sees what it sees there; a sequence of length 0 gets zeros and
  * lse -inf; a block-table entry outside the pool raises SBK_ST_BAD_BLOCK. Equal to the attention over the bf16 values that
  * sbk_kv_gather_q8 returns, up to the rounding of the sums.
- *  workspace    at least sbk_swa_decode_q8_workspace_bytes(B, H, D) bytes, 16-byte aligned (NULL when that is 0). Its
- *               contents need no initialisation and mean nothing between calls. Calls that overlap on the GPU need
- *               workspaces of their own.
- * Supported: D == 128, H % kvh == 0, H/kvh <= 8, kvh in {1,2,4}, block_size % 16 == 0.
+ *  workspace    at least sbk_swa_decode_q8_workspace_bytes(B, H, D) or sbk_swa_prefill_q8_workspace_bytes(...) bytes,
+ *               16-byte aligned (may be NULL when that is 0). Its contents need no initialisation and mean nothing between calls.
+ *               Calls that overlap on the GPU need workspaces of their own. For runs of queries it holds the visible
+ *               keys as dense bf16 rows: up to 256 MiB, or one sequence's worth where that is more (its sequences take
+ *               turns).
+ * Supported: D == 128, H % kvh == 0, H/kvh <= 8, block_size % 16 == 0; sbk_swa_decode_q8: kvh in {1,2,4}; sbk_swa_prefill_q8:
+ * q, out 16-byte aligned with token strides that are multiples of 8 elements.
  */
 size_t sbk_swa_decode_q8_workspace_bytes(int B, int H, int D);
 int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void* k_cache, const void* v_cache,
@@ -340,12 +343,15 @@ int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void* k_cache, 
                       int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes, int window_left,
                       float scale, void* out, int out_dtype, int64_t out_seq_stride, float* lse_out,
                       void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+size_t sbk_swa_prefill_q8_workspace_bytes(int n_seqs, int max_query_len, int max_blocks, int kvh, int D,
+                                          int block_size, int window_left);
 int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const void* k_cache, const void* v_cache,
                        const void* k_scale, const void* v_scale, const int32_t* block_tables, int max_blocks,
                        const int32_t* query_start_loc, const int32_t* context_lens, int n_seqs, int max_query_len,
                        int H, int kvh, int D, int64_t num_blocks, int block_size,
                        int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes, int window_left,
-                       float scale, void* out, int64_t out_tok_stride, int32_t* status, void* stream);
+                       float scale, void* out, int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
+                       int32_t* status, void* stream);
 
 /*
  * Device-resident step planning and block allocation. State that stays on the GPU between steps:

@@ -85,10 +85,11 @@ SIGNATURES = {
         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
         c_int, c_int, c_int64, c_int, c_int64, c_int64, c_int, c_float, c_void_p, c_int, c_int64, c_void_p,
         c_void_p, c_size_t, c_void_p, c_void_p]),
+    "sbk_swa_prefill_q8_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "sbk_swa_prefill_q8": (c_int, [
         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
         c_int, c_int, c_int, c_int, c_int64, c_int, c_int64, c_int64, c_int, c_float, c_void_p, c_int64, c_void_p,
-        c_void_p]),
+        c_size_t, c_void_p, c_void_p]),
     "sbk_pool_init": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "sbk_plan_step": (c_int, [
         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,

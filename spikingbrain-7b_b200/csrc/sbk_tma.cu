@@ -45,6 +45,17 @@ static bool encode_map(CUtensorMap* m, const MapKey& k, bool tile_copy) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_rows_map(CUtensorMap* m, const void* base, int64_t rows, int heads) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dim[3] = {128, (cuuint64_t)rows, (cuuint64_t)heads};
+  const cuuint64_t stride[2] = {256, (cuuint64_t)rows * 256};
+  const cuuint32_t box[3] = {64, 128, 1}, estr[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dim, stride, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static int g_copy_mode = -1;
 int copy_mode() { return g_copy_mode; }
 

@@ -33,6 +33,9 @@ struct MapKey {
 // asked once per process with a fixed geometry -- and every key can be expressed in it), else 0
 // for row copies. False when some key cannot be encoded in either form.
 bool get_maps(CUtensorMap* out, const MapKey* keys, int n, int* tile_copy);
+// A map over dense rows [heads][rows][128] bf16: boxes of 64 dims x 128 rows of one head, 128-byte swizzle. Not cached (its
+// base is a scratch that comes and goes).
+bool encode_rows_map(CUtensorMap* m, const void* base, int64_t rows, int heads);
 int copy_mode();   // -1 unknown, 1 tile copies, 0 row copies
 
 // 4-D tensor copy global -> shared (TMA), completion in bytes on an mbarrier

@@ -39,7 +39,7 @@ constexpr int kD = 128, kChunk = 16, kMaxG = 8;
 constexpr int kConsumerWarps = 4, kThreads = 32 * (kConsumerWarps + 1), kConsumers = 32 * kConsumerWarps;
 constexpr int kMaxSeqs = 1024;        // sequences per launch (lengths and prefix in shared memory)
 constexpr int kMaxCtas = 320;         // two per SM, as many as the workspace is laid out for
-constexpr int kItemCost = 8;          // what starting and finishing a sequence is charged, in units
+constexpr int kItemCost = 2;          // what starting and finishing a sequence is charged, in units
 constexpr int kMinRun = 1;            // shortest run of a CTA, in units
 constexpr int kStages = 3;
 constexpr int kTileBytes = 16384;     // K, or V, of a stage
@@ -69,7 +69,9 @@ struct Params {
   const int32_t* block_tables; int max_blocks; const int32_t* seq_lens;
   int B, H; int64_t num_blocks; int block_size, window_left; float scale_log2;
   void* out; int64_t out_stride; float* lse_out;
-  int2* cut;            // [grid]: the sequence that begins in this CTA's run and goes on in the next ones, and its pieces (0: none)
+  int4* cut;            // (sequence, first CTA, pieces; pieces <= 1: not cut), an entry per sequence where there are fewer of them
+                        // than CTAs, else per CTA: the sequence that begins in its run and goes on
+  int cut_by_seq;
   float* ws_o; float2* ws_ml;   // partials [2 * CTA + slot][H][D] and [..][H]: slot 0 a sequence that began before, 1 one that goes on
   int32_t* status; int tile_copy;
 };
@@ -301,9 +303,8 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       }
     };
 
-    int2 cut = make_int2(-1, 0);
     if (whole) {
-      if (lane == 0) P.cut[me] = cut;
+      if (lane == 0) P.cut[me] = make_int4(-1, 0, 0, 0);      // (a whole batch has as many sequences as CTAs at least)
       for (int b = me; b < P.B && !aborted; b += n_cta) {
         const Span sp = span_of<kUnit>(lens[b], P.window_left);
         stream_item(b, sp.first, sp.units, -1);
@@ -312,6 +313,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       const int64_t g0 = (int64_t)me * per;
       const int64_t g1 = g0 + per < total ? g0 + per : total;
       int b0 = 0;
+      int4 cut = make_int4(-1, 0, 0, 0);
       if (g0 < total) {
         int hi_b = P.B;                 // largest b with pre[b] <= g0
         while (hi_b - b0 > 1) {
@@ -325,9 +327,15 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           if (pre[mid] <= g1 - 1) e = mid; else he = mid;
         }
         const int cr = lens[e] > 0 ? span_of<kUnit>(lens[e], P.window_left).units : 1;
-        if (pre[e] >= g0 && pre[e] + cr > g1) cut = make_int2(e, (pre[e] + cr - 1) / per - me + 1);
+        if (pre[e] >= g0 && pre[e] + cr > g1) cut = make_int4(e, me, (pre[e] + cr - 1) / per - me + 1, 0);
       }
-      if (lane == 0) P.cut[me] = cut;
+      // (before anything is streamed: the folding kernel reads every entry, also of a launch that gave up on a wait)
+      if (P.cut_by_seq) {
+        for (int b = b0 + lane; g0 < total && b < P.B && pre[b] < g1; b += 32)
+          if (pre[b] >= g0) P.cut[b] = b == cut.x ? cut : make_int4(-1, 0, 0, 0);
+      } else if (lane == 0) {
+        P.cut[me] = cut;
+      }
       if (g0 < total) {
         for (int b = b0; b < P.B && pre[b] < g1 && !aborted; ++b) {
           const Span sp = span_of<kUnit>(lens[b], P.window_left);
@@ -604,32 +612,34 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   }
 }
 
-// Folds the partials of the sequence that begins in CTA c's run and goes on: one block per (c, four heads), four warps per
-// head, each taking every fourth piece with its loads issued eight at a time.
-constexpr int kFoldThreads = 512;
-template <typename TO>
-__global__ void __launch_bounds__(kFoldThreads) fold_kernel(const Params P) {
-  __shared__ float part[16][32][6];
+// Folds the partials of the sequences that were cut. Block (x, y): entry x of `cut`, heads HPC y ...; WPH warps share a head,
+// each taking every WPH-th piece with its loads issued eight at a time.
+template <int WPH, int HPC, typename TO>
+__global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P) {
+  __shared__ float4 part_o[WPH * HPC][32];
+  __shared__ float2 part_ml[WPH * HPC];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x;
-  const int2 cut = P.cut[c];
-  if (cut.y <= 1) return;
+  const int4 cut = P.cut[blockIdx.x];                    // sequence, first CTA, pieces
+  if (cut.z <= 1) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y * 4 + (warp >> 2), w = warp & 3;
+  const int h = blockIdx.y * HPC + warp / WPH, w = warp % WPH;
   const bool on = h < P.H;
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kU = 8;
-  for (int i0 = w; on && i0 < cut.y; i0 += 4 * kU) {
+  for (int i0 = w; on && i0 < cut.z; i0 += WPH * kU) {
     float2 ml[kU];
     float4 o[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      const int i = i0 + 4 * u < cut.y ? i0 + 4 * u : i0;
-      const int64_t row = (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)) * P.H + h;
-      ml[u] = __ldcg(P.ws_ml + row);
-      o[u] = __ldcg(reinterpret_cast<const float4*>(P.ws_o + row * kD) + lane);
-      if (i0 + 4 * u >= cut.y) ml[u] = make_float2(-INFINITY, 0.f);
+      const int i = i0 + WPH * u;
+      ml[u] = make_float2(-INFINITY, 0.f);
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < cut.z) {
+        const int64_t row = (int64_t)(2 * (cut.y + i) + (i == 0 ? 1 : 0)) * P.H + h;
+        ml[u] = __ldcg(P.ws_ml + row);
+        o[u] = __ldcg(reinterpret_cast<const float4*>(P.ws_o + row * kD) + lane);
+      }
     }
     float Mn = M;
 #pragma unroll
@@ -638,29 +648,29 @@ __global__ void __launch_bounds__(kFoldThreads) fold_kernel(const Params P) {
     L *= resc; O.x *= resc; O.y *= resc; O.z *= resc; O.w *= resc;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (i0 + 4 * u >= cut.y) break;
       const float wgt = fast_exp2(ml[u].x - Ms);
       L += ml[u].y * wgt;
       O.x += o[u].x * wgt; O.y += o[u].y * wgt; O.z += o[u].z * wgt; O.w += o[u].w * wgt;
     }
     M = Mn;
   }
-  float* mine = part[warp][lane];
-  mine[0] = M; mine[1] = L; mine[2] = O.x; mine[3] = O.y; mine[4] = O.z; mine[5] = O.w;
+  part_o[warp][lane] = O;
+  if (lane == 0) part_ml[warp] = make_float2(M, L);
   __syncthreads();
   if (w != 0 || !on) return;
   float Mt = -INFINITY;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) Mt = fmaxf(Mt, part[warp + q][lane][0]);
+  for (int q = 0; q < WPH; ++q) Mt = fmaxf(Mt, part_ml[warp + q].x);
   const float Ms = fmaxf(Mt, kNegBig);
   float Lt = 0.f;
   float4 Ot = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const float* p = part[warp + q][lane];
-    const float wgt = fast_exp2(p[0] - Ms);
-    Lt += p[1] * wgt;
-    Ot.x += p[2] * wgt; Ot.y += p[3] * wgt; Ot.z += p[4] * wgt; Ot.w += p[5] * wgt;
+  for (int q = 0; q < WPH; ++q) {
+    const float2 ml = part_ml[warp + q];
+    const float4 o = part_o[warp + q][lane];
+    const float wgt = fast_exp2(ml.x - Ms);
+    Lt += ml.y * wgt;
+    Ot.x += o.x * wgt; Ot.y += o.y * wgt; Ot.z += o.z * wgt; Ot.w += o.w * wgt;
   }
   const float f = inverse(Lt);
   store4(reinterpret_cast<TO*>(P.out) + (int64_t)cut.x * P.out_stride + (int64_t)h * kD + 4 * lane,
@@ -668,7 +678,7 @@ __global__ void __launch_bounds__(kFoldThreads) fold_kernel(const Params P) {
   if (P.lse_out && lane == 0) P.lse_out[(int64_t)cut.x * P.H + h] = row_lse(Mt, Lt);
 }
 
-static size_t cut_bytes() { return (size_t)kMaxCtas * sizeof(int2); }
+static size_t cut_bytes() { return (size_t)kMaxCtas * sizeof(int4); }
 
 template <int KVH, typename TO>
 static int launch(const Params& P0, int B_total, int sms, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
@@ -701,19 +711,22 @@ static int launch(const Params& P0, int B_total, int sms, const CUtensorMap& map
     int grid = (int)(most < n_ctas ? most : n_ctas);
     // a batch between one and two sequences per SM: one CTA each, so that every SM has work either way of cutting
     if (2 * P.B >= n_ctas && P.B < n_ctas) grid = P.B;
+    P.cut_by_seq = P.B < grid;
     kern<<<grid, kThreads, kSmemBytes, st>>>(P, map_k, map_v);
     int rc = check_launch("sbk_swa_decode_q8");
     if (rc != SBK_OK) return rc;
+    // Few sequences are cut into many pieces: sixteen warps to a head. Else four heads to a block of eight warps.
+    const bool few = P.B <= 32;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, (P.H + 3) / 4);
-    cfg.blockDim = dim3(kFoldThreads);
+    cfg.gridDim = dim3(P.cut_by_seq ? P.B : grid, few ? P.H : (P.H + 3) / 4);
+    cfg.blockDim = dim3(few ? 512 : 256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fold_kernel<TO>, P);
+    const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, fold_kernel<16, 1, TO>, P) : cudaLaunchKernelEx(&cfg, fold_kernel<2, 4, TO>, P);
     if (e != cudaSuccess) {
       set_error("sbk_swa_decode_q8: launch of the folding kernel failed: %s", cudaGetErrorString(e));
       return SBK_E_LAUNCH;
@@ -785,7 +798,7 @@ extern "C" int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void
   P.block_tables = block_tables; P.max_blocks = max_blocks; P.seq_lens = seq_lens;
   P.H = H; P.num_blocks = num_blocks; P.block_size = block_size; P.window_left = window_left;
   P.scale_log2 = scale * kLog2e; P.out = out; P.out_stride = out_seq_stride; P.lse_out = lse_out; P.status = status;
-  P.cut = (int2*)workspace;
+  P.cut = (int4*)workspace;
   P.ws_o = (float*)((uint8_t*)workspace + cut_bytes());
   P.ws_ml = (float2*)(P.ws_o + (size_t)kMaxCtas * 2 * H * D);
   static int sm_count[64] = {};

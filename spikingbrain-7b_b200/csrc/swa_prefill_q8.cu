@@ -1,0 +1,562 @@
+// Sliding-window attention for runs of query tokens over the 8-bit paged K/V cache (format: kv_q8.cuh), in two launches.
+//
+// 1. unpack: the keys that a run sees become dense bf16 rows, K and V [head][row][128], once. Every value of the cache is
+//    a bf16 number, so nothing is rounded. A run's rows start at a multiple of 128 and its last 128 are filled up with
+//    zeros. Each key serves (window / queries of a tile) query tiles, so expanding it in every CTA that reads it would repeat that work
+//    a hundred times over in the kernel that is short of instructions; written out once it is 3 (D + 1) kvh bytes a token,
+//    under 2 % of the time of a long run.
+// 2. attend: tcgen05, two query tiles per CTA taking turns, as in swa_prefill_tc2.cu: a CTA owns 2 x (128 / G) consecutive queries of a
+//    run and one kv head as two MMA tiles A and B of 128 rows (row = query * G + head); both read the same K / V tiles in shared
+//    memory; one thread owns one row, and while the warps of A work on their scores the tensor core computes for B:
+//        tensor core:  S_A(0) S_B(0) | P_A(0).V S_A(1) | P_B(0).V S_B(1) | ...
+//        warps 0-3  :  softmax A(0)  |                 | softmax A(1)    ...
+//        warps 4-7  :                | softmax B(0)    |                 ...
+//    Unlike there P and V are bf16 (a V row may have any exponent, which fp16 does not hold; P loses 2^-9 of itself, half of what
+//    the output's own rounding does), nothing has to be converted, and a tile of 128 keys is one copy per 64 dims.
+//    Tensor memory (512 columns): S_A / P_A [0,128), S_B / P_B [128,256), O_A [256,384), O_B [384,512). The softmax offset of a row
+//    moves only when its maximum has grown by more than 2^8, so O is rescaled in tensor memory almost only on the first tile.
+//    Roles (352 threads): warps 0-3 softmax / epilogue of tile A, 4-7 of tile B, 8 producer of the K ring, 9 of the V ring, 10 tensor
+//    memory and MMA issue. Every wait is bounded.
+#include <math.h>
+
+#include "kv_q8.cuh"
+#include "sbk_tcgen05.cuh"
+#include "sbk_tma.cuh"
+
+namespace sbk {
+namespace prefill_q8 {
+
+using namespace tc5;
+
+constexpr int kD = 128, kTile = 128;
+constexpr int kPanelBytes = 128 * 128;           // [128 rows][128 B]: 64 bf16 of every row
+constexpr int kOperandBytes = 2 * kPanelBytes;
+constexpr int kStagesK = 2, kStagesV = 3;
+constexpr int kQOff = 0, kKOff = 2 * kOperandBytes, kVOff = kKOff + kStagesK * kOperandBytes;
+constexpr int kBarOff = kVOff + kStagesV * kOperandBytes;
+constexpr int kSmemBytes = kBarOff + 256 + 1024;
+constexpr int kSoftmaxWarps = 8, kThreads = 32 * (kSoftmaxWarps + 3);
+constexpr int kTmemCols = 512, kOCol = 256;
+constexpr float kLog2e = 1.4426950408889634f, kNegBig = -1.0e30f;
+constexpr int64_t kScratchTarget = (int64_t)1 << 28;   // 256 MiB of dense rows at a time, or one sequence's where that is more
+
+struct Params {
+  const __nv_bfloat16* q; int64_t q_tok_stride;
+  const int32_t* query_start_loc; const int32_t* context_lens;
+  int seq0;               // first sequence of this launch; its dense rows start at row 0
+  int rows_per_seq;       // dense rows of a sequence, a multiple of 128
+  int pairs;              // query tile pairs per sequence
+  int max_query_len, H, G, bq, window_left; float scale_log2;   // >= 0: a negative scale's sign goes into q
+  uint32_t q_sign;
+  __nv_bfloat16* out; int64_t out_tok_stride; int32_t* status;
+};
+
+// what a sequence's run sees: keys [first, first + n) of its token axis
+struct Keys { int first, n, n_q; };
+__device__ __forceinline__ Keys keys_of(const int32_t* qsl, const int32_t* ctx_lens, int s, int window_left, int max_query_len) {
+  Keys k;
+  k.n_q = qsl[s + 1] - qsl[s];
+  if (k.n_q > max_query_len) k.n_q = max_query_len;
+  if (k.n_q < 0) k.n_q = 0;
+  int ctx = ctx_lens[s];
+  ctx = ctx < 0 ? 0 : (ctx > (1 << 30) ? (1 << 30) : ctx);
+  k.first = window_left < 0 || ctx <= window_left ? 0 : ctx - window_left;
+  k.n = k.n_q > 0 ? ctx - k.first + k.n_q : 0;
+  return k;
+}
+
+// ---- 1. the visible keys of sequences seq0 ... as dense rows; 16 lanes per row, eight values each ----
+__global__ void __launch_bounds__(256)
+unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const uint8_t* __restrict__ k_scale,
+              const uint8_t* __restrict__ v_scale, const int32_t* __restrict__ block_tables, int max_blocks,
+              const int32_t* __restrict__ query_start_loc, const int32_t* __restrict__ context_lens, int seq0, int kvh,
+              int64_t num_blocks, int block_size, int64_t cache_block_stride, int64_t scale_block_stride, int window_left,
+              int max_query_len, int rows_per_seq, int64_t rows_total, uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out,
+              int32_t* status) {
+  const int s = seq0 + (int)blockIdx.y;
+  Keys ks = keys_of(query_start_loc, context_lens, s, window_left, max_query_len);
+  if (ks.n > rows_per_seq) {             // a run that goes past its row of the block table
+    if (blockIdx.x == 0 && threadIdx.x == 0) raise_status(status, SBK_ST_BAD_BLOCK);
+    ks.n = rows_per_seq;
+  }
+  const int n_pad = (ks.n + kTile - 1) / kTile * kTile;
+  const int l = threadIdx.x & 15;
+  const int32_t* table = block_tables + (int64_t)s * max_blocks;
+  // consecutive groups of lanes walk the heads of a token: the rows of a token are contiguous in the cache
+  for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < (int64_t)n_pad * kvh; i += (int64_t)gridDim.x * 16) {
+    const int r = (int)(i / kvh), h = (int)(i - (int64_t)r * kvh);
+    uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
+    if (r < ks.n) {
+      const int tok = ks.first + r, lb = tok / block_size, off = tok - lb * block_size;
+      const int32_t pb = lb < max_blocks ? table[lb] : -1;
+      if (pb < 0 || pb >= num_blocks) {
+        if (l == 0) raise_status(status, SBK_ST_BAD_BLOCK);
+      } else {
+        const int64_t at = (int64_t)pb * cache_block_stride + ((int64_t)off * kvh + h) * kD + 8 * l;
+        const int64_t sa = (int64_t)pb * scale_block_stride + (int64_t)h * block_size + off;
+        const uint2 kc = *reinterpret_cast<const uint2*>(k_cache + at), vc = *reinterpret_cast<const uint2*>(v_cache + at);
+        const float kf = q8::byte_scale(k_scale[sa]), vf = q8::byte_scale(v_scale[sa]);
+        auto two = [](uint32_t w, float f) {
+          const float2 x = q8::e4m3x2_to_float2(w);
+          return pack_bf16x2(x.x * f, x.y * f);
+        };
+        kw = make_uint4(two(kc.x & 0xffffu, kf), two(kc.x >> 16, kf), two(kc.y & 0xffffu, kf), two(kc.y >> 16, kf));
+        vw = make_uint4(two(vc.x & 0xffffu, vf), two(vc.x >> 16, vf), two(vc.y & 0xffffu, vf), two(vc.y >> 16, vf));
+      }
+    }
+    const int64_t o = (((int64_t)h * rows_total + (int64_t)blockIdx.y * rows_per_seq + r) * kD + 8 * l) * 2;
+    *reinterpret_cast<uint4*>(k_out + o) = kw;
+    *reinterpret_cast<uint4*>(v_out + o) = vw;
+  }
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+// ---- 2. attention of the runs over the dense rows ----
+__global__ void __launch_bounds__(kThreads, 1)
+attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t sbase = smem_u32(smem);
+  // barriers: K ring full / empty, V ring full / empty; per tile: S ready, P ready (two halves of the keys); Q staged; all done.
+  // S and P of a tile take turns strictly, so one barrier each and phase t & 1.
+  const uint32_t bar_kf = sbase + kBarOff, bar_ke = bar_kf + 8 * kStagesK;
+  const uint32_t bar_vf = bar_ke + 8 * kStagesK, bar_ve = bar_vf + 8 * kStagesV;
+  const uint32_t bar_s = bar_ve + 8 * kStagesV, bar_p = bar_s + 16, bar_q = bar_p + 32, bar_done = bar_q + 8;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kBarOff + 192);
+  volatile uint8_t* abort_flag = smem + kBarOff + 208;
+
+  const int sl = blockIdx.x / P.pairs, s = P.seq0 + sl;
+  // later queries see more keys: they are launched first, so the long items do not start last
+  const int j = P.pairs - 1 - (int)(blockIdx.x - sl * P.pairs);
+  const int hk = blockIdx.y, kBQ = P.bq, G = P.G;
+  const Keys ks = keys_of(P.query_start_loc, P.context_lens, s, P.window_left, P.max_query_len);
+  if (j * 2 * kBQ >= ks.n_q) return;   // whole CTA, before anything is allocated
+  const int nq_pair = ks.n_q - j * 2 * kBQ < 2 * kBQ ? ks.n_q - j * 2 * kBQ : 2 * kBQ;
+  const bool has_b = nq_pair > kBQ;
+  const int qs = P.query_start_loc[s] + j * 2 * kBQ;       // row of the pair's first query
+  // in dense rows (row 0 = key ks.first): the last key of the pair's first query, the first key it sees, one past the last key
+  const int p0 = ks.n - ks.n_q + j * 2 * kBQ;
+  const int lo = P.window_left < 0 || p0 <= P.window_left ? 0 : p0 - P.window_left;
+  const int t_lo = lo / kTile, n_tiles = (p0 + nq_pair - 1) / kTile - t_lo + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStagesK; ++i) { mbar_init(bar_kf + 8 * i, 1); mbar_init(bar_ke + 8 * i, 1); }
+    for (int i = 0; i < kStagesV; ++i) { mbar_init(bar_vf + 8 * i, 1); mbar_init(bar_ve + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) mbar_init(bar_s + 8 * i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(bar_p + 8 * i, 4);      // one arrival per warp of the tile
+    mbar_init(bar_q, kSoftmaxWarps);
+    mbar_init(bar_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kSoftmaxWarps + 2) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
+    tmem_relinquish();
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == kSoftmaxWarps || warp == kSoftmaxWarps + 1) {
+    // ===== producers: one warp per ring, a tile is two copies of [128 rows][64 dims] =====
+    const int kind = warp - kSoftmaxWarps;
+    const int stages = kind ? kStagesV : kStagesK;
+    bool ok = true;
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      const int slot = t % stages, use = t / stages;
+      const uint32_t bar_e = (kind ? bar_ve : bar_ke) + 8 * slot, bar_f = (kind ? bar_vf : bar_kf) + 8 * slot;
+      if (use > 0 && !mbar_wait_bounded(bar_e, (use - 1) & 1)) ok = false;
+      if (*abort_flag) ok = false;
+      if (!ok) break;
+      if (lane == 0) {
+        const uint32_t dst = sbase + (kind ? kVOff : kKOff) + slot * kOperandBytes;
+        const CUtensorMap* map = kind ? &map_v : &map_k;
+        const int row = sl * P.rows_per_seq + (t_lo + t) * kTile;
+        mbar_arrive_expect_tx(bar_f, kOperandBytes);
+        tma_load_3d(dst, map, 0, row, hk, bar_f);
+        tma_load_3d(dst + kPanelBytes, map, 64, row, hk, bar_f);
+      }
+      __syncwarp();
+    }
+    if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+  } else if (warp == kSoftmaxWarps + 2) {
+    // ================================= MMA issuer =================================
+    const uint32_t idesc_qk = instr_desc(0), idesc_pv = instr_desc(1);
+    auto issue_s = [&](int X, int t) {     // S_X(t) = Q_X . K(t)^T
+      if (lane == 0) {
+        const uint32_t q_addr = sbase + kQOff + X * kOperandBytes;
+        const uint32_t k_addr = sbase + kKOff + (t % kStagesK) * kOperandBytes;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t off = (k >> 2) * kPanelBytes + (k & 3) * 32;
+          umma_bf16(tmem + X * 128, smem_desc(q_addr + off, 16), smem_desc(k_addr + off, 16), idesc_qk, k > 0);
+        }
+        umma_commit(bar_s + 8 * X);
+      }
+      __syncwarp();
+    };
+    // O_X += P_X(t) . V(t) for one half of the keys: steps of 16 keys, whose P is 8 columns of packed pairs at the head of
+    // the 32 columns its scores came from
+    auto issue_pv = [&](int X, int t, int half) {
+      if (lane == 0) {
+        const uint32_t v_addr = sbase + kVOff + (t % kStagesV) * kOperandBytes;
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int k = 4 * half + k4;
+          umma_bf16_ts(tmem + kOCol + X * 128, tmem + X * 128 + 32 * (k >> 1) + 8 * (k & 1), smem_desc(v_addr + k * 2048, kPanelBytes),
+                       idesc_pv, (t > 0) || (k > 0));
+        }
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint32_t bar) {
+      if (lane == 0) umma_commit(bar);
+      __syncwarp();
+    };
+    auto k_full = [&](int t) { return mbar_wait_bounded(bar_kf + 8 * (t % kStagesK), (t / kStagesK) & 1) && !*abort_flag; };
+    bool ok = mbar_wait_bounded(bar_q, 0) && k_full(0);
+    if (ok) {
+      tc_fence_after();
+      issue_s(0, 0);
+      if (has_b) issue_s(1, 0);
+      commit(bar_ke);
+    }
+    for (int t = 0; ok && t < n_tiles; ++t) {
+      const int vslot = t % kStagesV;
+      const bool more = t + 1 < n_tiles;
+      for (int X = 0; ok && X < (has_b ? 2 : 1); ++X) {
+        const bool last = X == (has_b ? 1 : 0);
+        // P_X(t), the first 64 keys and then the rest: the product of the first half runs while the threads work on the second;
+        // with the second S_X(t) has been read, so S_X(t + 1) may follow
+        ok = mbar_wait_bounded(bar_p + 16 * X, t & 1) && mbar_wait_bounded(bar_vf + 8 * vslot, (t / kStagesV) & 1);
+        if (!ok || *abort_flag) break;
+        tc_fence_after();
+        issue_pv(X, t, 0);
+        ok = mbar_wait_bounded(bar_p + 16 * X + 8, t & 1);
+        if (!ok || *abort_flag) break;
+        tc_fence_after();
+        issue_pv(X, t, 1);
+        if (last) commit(bar_ve + 8 * vslot);
+        if (more) {
+          if (X == 0) {
+            ok = k_full(t + 1);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          issue_s(X, t + 1);
+          if (last) commit(bar_ke + 8 * ((t + 1) % kStagesK));
+        }
+      }
+      if (*abort_flag) ok = false;
+    }
+    if (ok) commit(bar_done);
+    if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+  } else {
+    // ====================== softmax / epilogue: one thread per row ======================
+    const int X = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;        // row of the MMA tile = tensor-memory lane
+    const int ql = r / G, slot_h = r - ql * G;   // rows past bq * G land on ql == bq: never a query of the tile
+    const int nq_tile = X ? nq_pair - kBQ : (nq_pair < kBQ ? nq_pair : kBQ);
+    const bool row_ok = ql < nq_tile;
+    const int64_t q_row = qs + X * kBQ + ql;
+    const int p_row = p0 + X * kBQ + ql;         // the row's last visible key
+    const int lo_row = P.window_left < 0 || p_row <= P.window_left ? 0 : p_row - P.window_left;
+    {
+      const uint4* qp = reinterpret_cast<const uint4*>(P.q + q_row * P.q_tok_stride + (int64_t)(hk * G + slot_h) * kD);
+      uint4 v[16];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        v[c] = row_ok ? qp[c] : make_uint4(0, 0, 0, 0);
+        v[c].x ^= P.q_sign; v[c].y ^= P.q_sign; v[c].z ^= P.q_sign; v[c].w ^= P.q_sign;
+      }
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        *reinterpret_cast<uint4*>(smem + kQOff + X * kOperandBytes + (c >> 3) * kPanelBytes + swz(r, c & 7)) = v[c];
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q);
+    }
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_col = t_lane + X * 128, o_col = t_lane + kOCol + X * 128;
+    float m_run = -INFINITY, mr = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    if (X == 0 || has_b) {
+      for (int t = 0; t < n_tiles; ++t) {
+        ok = mbar_wait_bounded(bar_s + 8 * X, t & 1);
+        if (!ok || *abort_flag) break;
+        tc_fence_after();
+        const int tb = (t_lo + t) * kTile;
+        int v_lo = lo_row - tb, v_hi = p_row + 1 - tb;            // columns this row may see: [v_lo, v_hi)
+        v_lo = v_lo < 0 ? 0 : v_lo;
+        v_hi = v_hi > kTile ? kTile : v_hi;
+        const bool full = __all_sync(0xffffffffu, v_lo == 0 && v_hi == kTile);   // the warp takes one path
+        // ---- first pass: the row maximum, 64 columns at a time ----
+        float both;
+        {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t s0[32], s1[32];
+            tmem_ld32_issue(s_col + 64 * hf, s0);
+            tmem_ld32_issue(s_col + 64 * hf + 32, s1);
+            tmem_ld_fence(s0); tmem_ld_fence(s1);
+            if (full) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                mx[0] = fmax3(mx[0], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
+                mx[1] = fmax3(mx[1], __uint_as_float(s0[i + 2]), __uint_as_float(s0[i + 3]));
+                mx[2] = fmax3(mx[2], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
+                mx[3] = fmax3(mx[3], __uint_as_float(s1[i + 2]), __uint_as_float(s1[i + 3]));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const int col = 64 * hf + i;
+                if (col >= v_lo && col < v_hi) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s0[i]));
+                if (col + 32 >= v_lo && col + 32 < v_hi) mx[2 + (i & 1)] = fmaxf(mx[2 + (i & 1)], __uint_as_float(s1[i]));
+              }
+            }
+          }
+          both = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        }
+        const float cand = fmaxf(m_run, both * P.scale_log2);
+        const bool move = cand > m_run + 8.f;   // also the first visible key of a row (m_run = -inf)
+        const float mr_new = move ? both : mr;  // the offset as a score, and in the exponent's units
+        const float m_s = move ? cand : fmaxf(m_run, kNegBig);
+        const float alpha = !move ? 1.f : (mr == -INFINITY ? 0.f : fast_exp2((mr - mr_new) * P.scale_log2));
+        if (move) m_run = cand;
+        mr = mr_new;
+        // One multiply-add per score where the offset is of ordinary size: all of a row's exponents are off by the rounding of the
+        // offset, which cancels against l. Beyond 2^20 that rounding is no longer small against the exponent itself.
+        const bool fast = full && __all_sync(0xffffffffu, fabsf(m_s) <= 1048576.f);
+        // O moves with the offset. The products that wrote it are done: S_X(t) was issued behind P_X(t-1).V.
+        if (__any_sync(0xffffffffu, t > 0 && alpha != 1.f)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t orr[32];
+            tmem_ld32_issue(o_col + 32 * c, orr);
+            tmem_ld_fence(orr);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * alpha);
+            tmem_st32(o_col + 32 * c, orr);
+          }
+        }
+        // ---- second pass: probabilities in place of the scores, each half reported as soon as it is stored ----
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+        const f32x2 sc2 = pack2(P.scale_log2, P.scale_log2), nm2 = pack2(-m_s, -m_s);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t sa[32], sb[32];
+          tmem_ld32_issue(s_col + 64 * hf, sa);
+          tmem_ld32_issue(s_col + 64 * hf + 32, sb);
+          tmem_ld_fence(sa); tmem_ld_fence(sb);
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            uint32_t (&sr)[32] = cc ? sb : sa;
+            const int col0 = 64 * hf + 32 * cc;
+            uint32_t ph[16];               // packed bf16 pairs, key 2e in the low half
+            if (fast) {
+              f32x2 la = 0ull, lb = 0ull;
+#pragma unroll
+              for (int i = 0; i < 32; i += 4) {
+                float x0, x1, x2, x3;
+                unpack2(ffma2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), sc2, nm2), x0, x1);
+                unpack2(ffma2(pack2(__uint_as_float(sr[i + 2]), __uint_as_float(sr[i + 3])), sc2, nm2), x2, x3);
+                const float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
+                la = fadd2(la, pack2(e0, e1));
+                lb = fadd2(lb, pack2(e2, e3));
+                ph[i >> 1] = pack_bf16x2(e0, e1);
+                ph[(i >> 1) + 1] = pack_bf16x2(e2, e3);
+              }
+              float a0, a1, b0, b1;
+              unpack2(la, a0, a1);
+              unpack2(lb, b0, b1);
+              ls[0] += a0; ls[1] += a1; ls[2] += b0; ls[3] += b1;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float pa = fast_exp2((__uint_as_float(sr[i]) - mr) * P.scale_log2);
+                float pb = fast_exp2((__uint_as_float(sr[i + 1]) - mr) * P.scale_log2);
+                if (col0 + i < v_lo || col0 + i >= v_hi) pa = 0.f;
+                if (col0 + i + 1 < v_lo || col0 + i + 1 >= v_hi) pb = 0.f;
+                ls[i & 3] += pa;
+                ls[(i + 1) & 3] += pb;
+                ph[i >> 1] = pack_bf16x2(pa, pb);
+              }
+            }
+            tmem_st16(s_col + col0, ph);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p + 16 * X + 8 * hf);
+        }
+        l_run = l_run * alpha + (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      }
+      if (ok && !*abort_flag) {
+        ok = mbar_wait_bounded(bar_done, 0);
+        if (ok) {
+          tc_fence_after();
+          const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
+          uint4* op = reinterpret_cast<uint4*>(P.out + q_row * P.out_tok_stride + (int64_t)(hk * G + slot_h) * kD);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t orr[32];
+            tmem_ld32_issue(o_col + 32 * c, orr);
+            tmem_ld_fence(orr);
+            if (row_ok) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                op[c * 4 + e] = make_uint4(
+                    pack_bf16x2(__uint_as_float(orr[e * 8 + 0]) * inv, __uint_as_float(orr[e * 8 + 1]) * inv),
+                    pack_bf16x2(__uint_as_float(orr[e * 8 + 2]) * inv, __uint_as_float(orr[e * 8 + 3]) * inv),
+                    pack_bf16x2(__uint_as_float(orr[e * 8 + 4]) * inv, __uint_as_float(orr[e * 8 + 5]) * inv),
+                    pack_bf16x2(__uint_as_float(orr[e * 8 + 6]) * inv, __uint_as_float(orr[e * 8 + 7]) * inv));
+            }
+          }
+        }
+      }
+    }
+    if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+  }
+
+  // ---- everyone meets here, then the allocating warp returns the tensor memory ----
+  if (*abort_flag) {
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies and MMAs in flight land
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftmaxWarps + 2) tmem_dealloc(tmem, kTmemCols);
+}
+
+// dense rows of a sequence, and sequences that share one scratch
+struct Layout { int64_t rows_per_seq; int group; };
+static Layout layout_of(int n_seqs, int max_query_len, int max_blocks, int kvh, int block_size, int window_left) {
+  Layout y;
+  const int64_t width = (int64_t)max_blocks * block_size;
+  int64_t n = width;
+  if (window_left >= 0 && (int64_t)window_left + max_query_len < width) n = (int64_t)window_left + max_query_len;
+  y.rows_per_seq = (n + kTile - 1) / kTile * kTile;
+  const int64_t bytes = y.rows_per_seq * kvh * kD * 4;      // K and V in bf16
+  int64_t g = kScratchTarget / bytes;
+  if (g < 1) g = 1;
+  y.group = (int)(g < n_seqs ? g : n_seqs);
+  return y;
+}
+
+}  // namespace prefill_q8
+}  // namespace sbk
+
+extern "C" size_t sbk_swa_prefill_q8_workspace_bytes(int n_seqs, int max_query_len, int max_blocks, int kvh, int D, int block_size,
+                                                     int window_left) {
+  using namespace sbk::prefill_q8;
+  if (n_seqs <= 0 || max_query_len <= 0 || max_blocks <= 0 || kvh <= 0 || D <= 0 || block_size <= 0) return 0;
+  const Layout y = layout_of(n_seqs, max_query_len, max_blocks, kvh, block_size, window_left);
+  return (size_t)(y.rows_per_seq * y.group) * kvh * D * 4;
+}
+
+extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const void* k_cache, const void* v_cache,
+                                  const void* k_scale, const void* v_scale, const int32_t* block_tables, int max_blocks,
+                                  const int32_t* query_start_loc, const int32_t* context_lens, int n_seqs,
+                                  int max_query_len, int H, int kvh, int D, int64_t num_blocks, int block_size,
+                                  int64_t cache_block_stride_bytes, int64_t scale_block_stride_bytes, int window_left,
+                                  float scale, void* out, int64_t out_tok_stride, void* workspace, size_t workspace_bytes,
+                                  int32_t* status, void* stream) {
+  using namespace sbk;
+  using namespace sbk::prefill_q8;
+  if (n_seqs < 0 || max_query_len < 0 || H <= 0 || kvh <= 0 || H % kvh != 0 || num_blocks < 0) {
+    set_error("sbk_swa_prefill_q8: bad sizes n_seqs=%d max_query_len=%d H=%d kvh=%d", n_seqs, max_query_len, H, kvh);
+    return SBK_E_ARG;
+  }
+  if (D != kD || H / kvh > 8) {
+    set_error("sbk_swa_prefill_q8: unsupported shape D=%d H/kvh=%d (need D=128, at most 8 query heads per kv head)", D, H / kvh);
+    return SBK_E_ARG;
+  }
+  if (block_size <= 0 || block_size % 16 != 0) {
+    set_error("sbk_swa_prefill_q8: block_size=%d must be a positive multiple of 16", block_size);
+    return SBK_E_ARG;
+  }
+  if (n_seqs == 0 || max_query_len == 0) return SBK_OK;
+  if (max_blocks <= 0 || !q || !k_cache || !v_cache || !k_scale || !v_scale || !block_tables || !query_start_loc || !context_lens || !out) {
+    set_error("sbk_swa_prefill_q8: null pointer or max_blocks=%d", max_blocks);
+    return SBK_E_ARG;
+  }
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_scale) || !aligned16(v_scale) ||
+      cache_block_stride_bytes % 16 || scale_block_stride_bytes % 16 || !aligned16(q) || !aligned16(out) || q_tok_stride % 8 ||
+      out_tok_stride % 8) {
+    set_error("sbk_swa_prefill_q8: caches, scales, their block strides, q, out and their token strides must be 16-byte multiples");
+    return SBK_E_ALIGN;
+  }
+  if (cache_block_stride_bytes < (int64_t)kvh * D * block_size || scale_block_stride_bytes < (int64_t)kvh * block_size) {
+    set_error("sbk_swa_prefill_q8: a block stride is smaller than the block it spans");
+    return SBK_E_ARG;
+  }
+  const Layout y = layout_of(n_seqs, max_query_len, max_blocks, kvh, block_size, window_left);
+  const int64_t rows = y.rows_per_seq * y.group;
+  const int bq = 128 / (H / kvh);
+  const int pairs = (max_query_len + 2 * bq - 1) / (2 * bq);
+  if (rows > 2147483647LL || (int64_t)y.group * pairs > 2147483647LL || kvh > 65535 || y.group > 65535) {
+    set_error("sbk_swa_prefill_q8: grid or scratch too large");
+    return SBK_E_ARG;
+  }
+  const size_t half = (size_t)rows * kvh * D * 2;
+  if (!workspace || workspace_bytes < 2 * half) {
+    set_error("sbk_swa_prefill_q8: workspace of %zu bytes given, %zu needed", workspace ? workspace_bytes : 0, 2 * half);
+    return SBK_E_WORKSPACE;
+  }
+  if (!aligned16(workspace)) {
+    set_error("sbk_swa_prefill_q8: workspace must be 16-byte aligned");
+    return SBK_E_ALIGN;
+  }
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    if (!encode_rows_map(&maps[i], (uint8_t*)workspace + i * half, rows, kvh)) {
+      set_error("sbk_swa_prefill_q8: cuTensorMapEncodeTiled rejected the scratch (%lld rows, %d heads)", (long long)rows, kvh);
+      return SBK_E_ARG;
+    }
+  }
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) {
+      set_error("sbk_swa_prefill_q8: cannot opt in to %d bytes of shared memory: %s", kSmemBytes, cudaGetErrorString(e));
+      return SBK_E_LAUNCH;
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  Params P = {};
+  P.q = (const __nv_bfloat16*)q; P.q_tok_stride = q_tok_stride;
+  P.query_start_loc = query_start_loc; P.context_lens = context_lens;
+  P.rows_per_seq = (int)y.rows_per_seq; P.pairs = pairs; P.max_query_len = max_query_len; P.H = H; P.G = H / kvh; P.bq = bq;
+  P.window_left = window_left; P.scale_log2 = fabsf(scale) * kLog2e; P.q_sign = scale < 0.f ? 0x80008000u : 0u;
+  P.out = (__nv_bfloat16*)out; P.out_tok_stride = out_tok_stride; P.status = status;
+  // groups of sequences share the scratch, one after the other on the stream
+  for (int s0 = 0; s0 < n_seqs; s0 += y.group) {
+    const int n = n_seqs - s0 < y.group ? n_seqs - s0 : y.group;
+    const int64_t ctas = (y.rows_per_seq * kvh + 63) / 64;           // four rows per group of lanes
+    unpack_kernel<<<dim3((unsigned)(ctas < 65535 ? ctas : 65535), n), 256, 0, st>>>(
+        (const uint8_t*)k_cache, (const uint8_t*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_tables,
+        max_blocks, query_start_loc, context_lens, s0, kvh, num_blocks, block_size, cache_block_stride_bytes,
+        scale_block_stride_bytes, window_left, max_query_len, P.rows_per_seq, rows, (uint8_t*)workspace,
+        (uint8_t*)workspace + half, status);
+    int rc = check_launch("sbk_swa_prefill_q8");
+    if (rc != SBK_OK) return rc;
+    P.seq0 = s0;
+    attend_kernel<<<dim3(n * pairs, kvh), kThreads, kSmemBytes, st>>>(P, maps[0], maps[1]);
+    rc = check_launch("sbk_swa_prefill_q8");
+    if (rc != SBK_OK) return rc;
+  }
+  return SBK_OK;
+}

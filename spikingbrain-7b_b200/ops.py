@@ -646,9 +646,19 @@ def kv_cache_q8(num_blocks: int, block_size: int, kvh: int, D: int, device="cuda
 
 def _q8_geometry(k_cache, v_cache, k_scale, v_scale) -> Tuple[int, int, int, int, int, int]:
     """-> (num_blocks, block_size, kvh, D, bytes between cache blocks, bytes between scale blocks)."""
+    shape, stride = k_cache.shape, k_cache.stride()
+    if len(shape) == 4:
+        nb, bs, kvh, d = shape
+        ss = k_scale.stride()
+        if (v_cache.shape == shape and v_cache.stride() == stride and stride[1:] == (kvh * d, d, 1)
+                and k_scale.shape == (nb, kvh, bs) and v_scale.shape == (nb, kvh, bs) and v_scale.stride() == ss
+                and ss[1:] == (bs, 1) and k_cache.dtype in _Q8_CODES and v_cache.dtype == k_cache.dtype
+                and k_scale.dtype in _Q8_SCALES and v_scale.dtype in _Q8_SCALES):
+            return nb, bs, kvh, d, stride[0], ss[0]
+    # everything else that is allowed (strides of size-1 dimensions, empty pools), and the errors
     if k_cache.dtype not in _Q8_CODES or v_cache.dtype != k_cache.dtype:
         raise ValueError("the 8-bit k_cache and v_cache are float8_e4m3fn (or uint8) tensors of one dtype")
-    nb, bs, kvh, d, stride = _cache_geometry(k_cache, v_cache)
+    nb, bs, kvh, d, cs = _cache_geometry(k_cache, v_cache)
     for t in (k_scale, v_scale):
         if t.dtype not in _Q8_SCALES or t.shape != (nb, kvh, bs):
             raise ValueError(f"k_scale and v_scale must be uint8 [{nb}, {kvh}, {bs}]")
@@ -656,7 +666,7 @@ def _q8_geometry(k_cache, v_cache, k_scale, v_scale) -> Tuple[int, int, int, int
             raise ValueError("the rows of a scale block must be contiguous")
     if k_scale.stride(0) != v_scale.stride(0):
         raise ValueError("k_scale and v_scale must share one block stride")
-    return nb, bs, kvh, d, stride, k_scale.stride(0)
+    return nb, bs, kvh, d, cs, k_scale.stride(0)
 
 
 def _heads_contiguous(t: torch.Tensor) -> bool:
@@ -664,28 +674,24 @@ def _heads_contiguous(t: torch.Tensor) -> bool:
     return not t.shape[0] or (t.stride(2) == 1 and (t.shape[1] < 2 or t.stride(1) == t.shape[2]))
 
 
-def _one_device(*tensors: Optional[torch.Tensor]) -> torch.device:
-    """The CUDA device that all tensors live on."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("libsbk ops take CUDA tensors only (there is no CPU path)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """Index of the CUDA device that all tensors live on."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if dev < 0:
+        raise RuntimeError("libsbk ops take CUDA tensors only (there is no CPU path)")
     return dev
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """C entry `name` on the current stream of `dev`, whichever device is current."""
-    if dev.index == torch.cuda.current_device():
-        rc = getattr(_abi.lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+def _call_on(dev: int, name: str, *args) -> None:
+    """C entry `name` on the current stream of device `dev`, whichever device is current."""
+    if dev == torch._C._cuda_getDevice():
+        rc = getattr(_abi.lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = getattr(_abi.lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = getattr(_abi.lib, name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _abi.check(name, rc)
 
@@ -745,7 +751,7 @@ def rope_kv_append_q8(query: Optional[torch.Tensor], key: torch.Tensor, value: t
                       retired_out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
     """kv_append_q8 with the NeoX rotary embedding folded in (arguments as in rope_kv_append). The rotation is done in
     fp32: K is quantised from the fp32 result; ``query`` (and ``key`` with ``key_in_place``) is rounded once to its dtype."""
-    dev = _one_device(query, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, positions, cos_sin_cache,
+    dev = _one_device(key, query, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, positions, cos_sin_cache,
                       block_tables, seq_lens, query_start_loc, retired_out, status)
     nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, es, tok_stride = _q8_append_args(
         key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc, retired_out)
@@ -781,8 +787,7 @@ def kv_gather_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Te
     B, max_blocks = block_tables.shape
     _i32(block_tables, "block_tables")
     _i32(seq_lens, "seq_lens", B)
-    k_out = torch.empty((B, kvh, n_out, d), dtype=dtype, device=dev)
-    v_out = torch.empty_like(k_out)
+    k_out, v_out = torch.empty((2, B, kvh, n_out, d), dtype=dtype, device=k_cache.device).unbind()
     _call_on(dev, "sbk_kv_gather_q8", _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables),
              max_blocks, _ptr(seq_lens), B, kvh, d, nb, bs, cs, ss, window_left, _ptr(k_out), _ptr(v_out),
              _DTYPE_CODE[dtype], n_out, _ptr(status))
@@ -815,7 +820,7 @@ def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     _i32(block_tables, "block_tables")
     _i32(seq_lens, "seq_lens", B)
     if out is None:
-        out = torch.empty((B, H, d), dtype=out_dtype or torch.bfloat16, device=dev)
+        out = torch.empty((B, H, d), dtype=out_dtype or torch.bfloat16, device=q.device)
     elif out.shape != (B, H, d) or not _heads_contiguous(out):
         raise ValueError("out must be [B, H, D] with contiguous heads")
     if out.dtype not in _DTYPE_CODE:
@@ -823,7 +828,7 @@ def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous fp32 [B, H]")
     if workspace is None:
-        workspace = swa_decode_q8_workspace(B, H, d, dev)
+        workspace = swa_decode_q8_workspace(B, H, d, q.device)
     _call_on(dev, "sbk_swa_decode_q8", _ptr(q), q.stride(0) if B > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
              _ptr(v_scale), _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), B, H, kvh, d, nb, bs, cs, ss,
              window_left, d ** -0.5 if scale is None else float(scale), _ptr(out), _DTYPE_CODE[out.dtype],
@@ -832,13 +837,23 @@ def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     return out
 
 
+def swa_prefill_q8_workspace(n_seqs: int, max_query_len: int, max_blocks: int, kvh: int, D: int, device, *, block_size: int,
+                             window_left: int) -> Optional[torch.Tensor]:
+    """Scratch for swa_prefill_q8 calls of these sizes (None when it needs none): the visible keys as dense bf16 rows. Its
+    contents need no initialisation; calls that can overlap on the GPU need one each."""
+    n = _abi.lib.sbk_swa_prefill_q8_workspace_bytes(n_seqs, max_query_len, max_blocks, kvh, D, block_size, window_left)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
 def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                    v_scale: torch.Tensor, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
                    context_lens: torch.Tensor, max_query_len: int, *, window_left: int, scale: Optional[float] = None,
-                   out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Sliding-window attention of runs of query tokens (q [T, H, D] bf16, token-major) over the 8-bit paged cache, the
-    runs' own K/V already appended; arguments as in swa_prefill."""
-    dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, query_start_loc, context_lens, out, status)
+    runs' own K/V already appended; arguments as in swa_prefill. ``workspace`` (swa_prefill_q8_workspace): kept by callers
+    that must not allocate."""
+    dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, query_start_loc, context_lens, out, workspace, status)
     nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != d or q.dtype != torch.bfloat16:
         raise ValueError(f"q must be bf16 [T, H, {d}]")
@@ -852,11 +867,16 @@ def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _i32(query_start_loc, "query_start_loc", n_seqs + 1)
     _i32(context_lens, "context_lens", n_seqs)
     if out is None:
-        out = torch.empty((T, H, d), dtype=torch.bfloat16, device=dev)
+        out = torch.empty((T, H, d), dtype=torch.bfloat16, device=q.device)
     elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not _heads_contiguous(out):
         raise ValueError("out must be bf16 [T, H, D] with contiguous heads")
+    max_query_len = int(max_query_len)
+    if workspace is None and n_seqs:
+        workspace = swa_prefill_q8_workspace(n_seqs, max_query_len, block_tables.shape[1], kvh, d, q.device, block_size=bs,
+                                             window_left=window_left)
     _call_on(dev, "sbk_swa_prefill_q8", _ptr(q), q.stride(0) if T > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
              _ptr(v_scale), _ptr(block_tables), block_tables.shape[1], _ptr(query_start_loc), _ptr(context_lens), n_seqs,
-             int(max_query_len), H, kvh, d, nb, bs, cs, ss, window_left, d ** -0.5 if scale is None else float(scale),
-             _ptr(out), out.stride(0) if T > 1 else H * d, _ptr(status))
+             max_query_len, H, kvh, d, nb, bs, cs, ss, window_left, d ** -0.5 if scale is None else float(scale),
+             _ptr(out), out.stride(0) if T > 1 else H * d, _ptr(workspace),
+             workspace.numel() * workspace.element_size() if workspace is not None else 0, _ptr(status))
     return out

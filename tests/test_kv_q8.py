@@ -165,7 +165,8 @@ def test_decode_refusals(sb, over, code):
 def test_prefill_refusals(sb, over, code):
     from spikingbrain_7b_b200 import _abi
     a = dict(q=A, qs=3584, k=A, v=A, ks=A, vs=A, tables=A, max_blocks=4, qsl=A, ctx=A, n=2, mq=5, H=28, kvh=4, D=128, nb=8,
-             bs=16, cs=8192, ss=64, wl=-1, scale=ctypes.c_float(0.1), out=A, os=3584, status=None, stream=None)
+             bs=16, cs=8192, ss=64, wl=-1, scale=ctypes.c_float(0.1), out=A, os=3584, ws=A, wsb=1 << 40, status=None,
+             stream=None)
     a.update(over)
     assert _abi.lib.sbk_swa_prefill_q8(*a.values()) == code
     assert b"sbk_swa_prefill_q8" in _abi.lib.sbk_last_error()
