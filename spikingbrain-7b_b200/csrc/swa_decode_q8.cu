@@ -31,72 +31,86 @@
 #include "kv_q8.cuh"
 #include "sbk_tcgen05.cuh"
 #include "sbk_tma.cuh"
+#include "swa_decode_q8.cuh"
 
 namespace sbk {
 namespace decode_q8 {
 
 constexpr int kD = 128, kChunk = 16, kMaxG = 8;
-constexpr int kConsumerWarps = 4, kThreads = 32 * (kConsumerWarps + 1), kConsumers = 32 * kConsumerWarps;
-constexpr int kMaxSeqs = 1024;        // sequences per launch (lengths and prefix in shared memory)
-constexpr int kMaxCtas = 320;         // two per SM, as many as the workspace is laid out for
-constexpr int kItemCost = 2;          // what starting and finishing a sequence is charged, in units
-constexpr int kMinRun = 1;            // shortest run of a CTA, in units
-constexpr int kStages = 3;
+constexpr int kMaxSeqs = 1024;        // items (sequences, or groups of queries of one) per launch: lengths and prefix in shared memory
+constexpr int kMaxSms = 160;          // as many as the workspace is laid out for
+constexpr int kItemCost = 2;          // what starting and finishing an item is charged, in units
 constexpr int kTileBytes = 16384;     // K, or V, of a stage
 constexpr int kScaleBytes = 256;      // exponents of a stage: 128 of K, 128 of V
 constexpr int kStageBytes = 2 * kTileBytes;
-constexpr int kHeadStride = 132;      // floats per head row of the merge scratch (bank skew)
-constexpr int kMergeWarpBytes = kMaxG * kHeadStride * 4 + 64;
+constexpr int kMergeWarpBytes = kMaxG * kD * 4;
 constexpr float kMostW = 32768.f, kMostP = 1.099511627776e12f;   // 2^15, 2^40: where the offsets of the softmax move
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kNegBig = -1.0e30f;
 enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8 };
 
-struct StageInfo { int b, tok_base, lo, hi, flags, part; };   // part: partial slot of the item's result, or -1 (direct)
+// row: the item's first query row; n_q: its queries; top: one past the last key of the last of them;
+// part: partial slot of the item's result, or -1 (direct)
+struct StageInfo { int row, n_q, top, tok_base, lo, hi, flags, part; };
 
-constexpr int kScaleOff = kStages * kStageBytes;
-constexpr int kInfoOff = kScaleOff + kStages * kScaleBytes;
-constexpr int kPreOff = kInfoOff + ((kStages * (int)sizeof(StageInfo) + 15) / 16) * 16;
-constexpr int kLensOff = kPreOff + (kMaxSeqs + 4) * 4;
-constexpr int kBarOff = kLensOff + kMaxSeqs * 4;
-constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
-constexpr int kSmemBytes = kMiscOff + 48 + 1024;      // + slack to align the ring to 1 KiB
-static_assert(kSmemBytes <= 115200, "two CTAs must fit one SM");
-static_assert(kConsumerWarps * kMergeWarpBytes <= kStageBytes, "the merge scratch lives inside one stage");
+// QG groups of four consumer warps, each with NQ queries of an item: one group and two CTAs per SM for single tokens, two
+// groups that read the same stages for runs of a few
+template <int QG>
+struct Cfg {
+  static constexpr int kWarps = 4 * QG, kThreads = 32 * (kWarps + 1), kConsumers = 32 * kWarps;
+  static constexpr int kCtasPerSm = QG == 1 ? 2 : 1;
+  static constexpr int kMaxCtas = kMaxSms * kCtasPerSm;
+  static constexpr int kStages = 3 * QG;
+  static constexpr int kScaleOff = kStages * kStageBytes;
+  static constexpr int kInfoOff = kScaleOff + kStages * kScaleBytes;
+  static constexpr int kPreOff = kInfoOff + kStages * (int)sizeof(StageInfo);
+  static constexpr int kLensOff = kPreOff + (kMaxSeqs + 4) * 4;
+  static constexpr int kCntOff = kLensOff + kMaxSeqs * 4;
+  static constexpr int kMlOff = kCntOff + kMaxSeqs;              // (m, l) of every warp's heads at the end of an item
+  static constexpr int kBarOff = kMlOff + kWarps * 64;
+  static constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
+  static constexpr int kSmemBytes = kMiscOff + 64 + 1024;        // + slack to align the ring to 1 KiB
+  static_assert(kSmemBytes * kCtasPerSm <= 230400, "the CTAs of an SM must fit its shared memory");
+  static_assert(kWarps * kMergeWarpBytes <= kStageBytes, "the merge scratch lives inside one stage");
+};
 
 struct Params {
   const __nv_bfloat16* q; int64_t q_stride;
   const uint8_t* k_scale; const uint8_t* v_scale; int64_t scale_block_stride;
-  const int32_t* block_tables; int max_blocks; const int32_t* seq_lens;
-  int B, H; int64_t num_blocks; int block_size, window_left; float scale_log2;
+  const int32_t* block_tables; int max_blocks;
+  const int32_t* seq_lens;                                    // single tokens; NULL: runs, whose item v is queries
+  const int32_t* query_start_loc; const int32_t* context_lens; // cap * (v % per_seq) ... of sequence v / per_seq
+  int per_seq, max_query_len;
+  int item0, B;         // items [item0, item0 + B) of the call
+  int H; int64_t num_blocks; int block_size, window_left; float scale_log2;
   void* out; int64_t out_stride; float* lse_out;
-  int4* cut;            // (sequence, first CTA, pieces; pieces <= 1: not cut), an entry per sequence where there are fewer of them
-                        // than CTAs, else per CTA: the sequence that begins in its run and goes on
-  int cut_by_seq;
-  float* ws_o; float2* ws_ml;   // partials [2 * CTA + slot][H][D] and [..][H]: slot 0 a sequence that began before, 1 one that goes on
+  int4* cut;            // (first query row, first CTA, pieces, queries; pieces <= 1: not cut), an entry per item where there are
+                        // fewer of them than CTAs, else per CTA: the item that begins in its run and goes on
+  int cut_by_item;
+  float* ws_o; float2* ws_ml;   // partials [2 * CTA + slot][query][H][D] and [..][H]: slot 0 an item that began before, 1 one that goes on
   int32_t* status; int tile_copy;
 };
 
 struct Span { int first, units; };    // units [first, first + units) of the token axis hold the visible tokens
 template <int UNIT>
-__device__ __forceinline__ Span span_of(int L, int window_left) {
+__device__ __forceinline__ Span span_of(int top, int n_q, int window_left) {
   Span s;
-  if (L <= 0) { s.first = 0; s.units = 0; return s; }
-  s.first = first_visible(L, 1, window_left) / UNIT;
-  s.units = (L - 1) / UNIT - s.first + 1;
+  if (top <= 0) { s.first = 0; s.units = 0; return s; }
+  s.first = first_visible(top, n_q, window_left) / UNIT;
+  s.units = (top - 1) / UNIT - s.first + 1;
   return s;
 }
 
 // D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// words of four codes of rows g (lo) and g + 8 (hi) -> one product: each word holds columns 2t, 2t+1, then 2t+8, 2t+9
-__device__ __forceinline__ void mma_codes(float (&c)[4], uint32_t lo, uint32_t hi, uint32_t b0, uint32_t b1) {
-  mma_f16(c, q8::e4m3x2_to_f16x2(lo & 0xffffu), q8::e4m3x2_to_f16x2(hi & 0xffffu), q8::e4m3x2_to_f16x2(lo >> 16),
-          q8::e4m3x2_to_f16x2(hi >> 16), b0, b1);
+// words of four codes of rows g (lo) and g + 8 (hi) -> an A fragment: each word holds columns 2t, 2t+1, then 2t+8, 2t+9
+__device__ __forceinline__ void widen(uint32_t (&a)[4], uint32_t lo, uint32_t hi) {
+  a[0] = q8::e4m3x2_to_f16x2(lo & 0xffffu); a[1] = q8::e4m3x2_to_f16x2(hi & 0xffffu);
+  a[2] = q8::e4m3x2_to_f16x2(lo >> 16); a[3] = q8::e4m3x2_to_f16x2(hi >> 16);
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
@@ -118,7 +132,8 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers) : "memory"); }
+template <int N>
+__device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
 
 template <typename TO> __device__ __forceinline__ void store2(TO* p, float a, float b);
 template <> __device__ __forceinline__ void store2<float>(float* p, float a, float b) { p[0] = a; p[1] = b; }
@@ -136,22 +151,27 @@ __device__ __forceinline__ void store4(TO* p, float4 v) { store2(p, v.x, v.y); s
 __device__ __forceinline__ float row_lse(float m, float l) { return l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY; }
 __device__ __forceinline__ float inverse(float l) { return l != 0.f ? 1.f / l : 0.f; }
 
-template <int KVH, typename TO>
-__global__ void __launch_bounds__(kThreads, 2)
-decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-  constexpr int kSub = kConsumerWarps / KVH;          // 32-token parts of a stage
+template <int KVH, int NQ, int QG, typename TO>
+__global__ void __launch_bounds__(Cfg<QG>::kThreads, Cfg<QG>::kCtasPerSm)
+stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+  using C = Cfg<QG>;
+  constexpr int kStages = C::kStages, kThreads = C::kThreads;
+  constexpr int kCap = NQ * QG;                       // queries of an item
+  constexpr int kSub = 4 / KVH;                       // 32-token parts of a stage
   constexpr int kUnit = 32 * kSub;                    // tokens of a stage
   constexpr int kChunks = kUnit / kChunk;             // 16-token chunks of a stage
   constexpr int kChunkBytes = KVH * kChunk * kD;      // one chunk of K or of V: [head][token][128 B]
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t ring = smem_u32(smem);
-  StageInfo* info = reinterpret_cast<StageInfo*>(smem + kInfoOff);
-  int* pre = reinterpret_cast<int*>(smem + kPreOff);
-  int* lens = reinterpret_cast<int*>(smem + kLensOff);
-  const uint32_t bar_full = ring + kBarOff, bar_empty = bar_full + 8 * kStages;
-  volatile int* misc = reinterpret_cast<volatile int*>(smem + kMiscOff);   // [0] abort, [1] longest, [2..6] scan
+  StageInfo* info = reinterpret_cast<StageInfo*>(smem + C::kInfoOff);
+  int* pre = reinterpret_cast<int*>(smem + C::kPreOff);
+  int* tops = reinterpret_cast<int*>(smem + C::kLensOff);
+  uint8_t* cnts = smem + C::kCntOff;
+  const uint32_t bar_full = ring + C::kBarOff, bar_empty = bar_full + 8 * kStages;
+  volatile int* misc = reinterpret_cast<volatile int*>(smem + C::kMiscOff);   // [0] abort, [1] longest, [2..] scan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int4 kNotCut = make_int4(-1, 0, 0, 0);
 
   // the folding kernel may be set up while this one runs (it waits for this one's end before it reads anything)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -159,7 +179,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1 + 32);   // the stage's bytes, and each producer lane's exponents
-      mbar_init(bar_empty + 8 * s, kConsumerWarps);
+      mbar_init(bar_empty + 8 * s, C::kWarps);
     }
     misc[0] = 0;
     misc[1] = 0;
@@ -167,7 +187,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     fence_mbar_init();
   }
   __syncthreads();
-  // ---- what every sequence costs, as an exclusive prefix: units of b occupy [pre[b], pre[b] + units), its charge follows ----
+  // ---- what every item costs, as an exclusive prefix: units of b occupy [pre[b], pre[b] + units), its charge follows ----
   {
     constexpr int kRun = (kMaxSeqs + kThreads - 1) / kThreads;
     const int run_len = (P.B + kThreads - 1) / kThreads;
@@ -178,16 +198,33 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       const int b = b_lo + i;
       int c = 0;
       if (i < run_len && b < P.B) {
-        int L = P.seq_lens[b];
+        int top, n = 1;
+        if (P.seq_lens) {
+          top = P.seq_lens[P.item0 + b];
+        } else {
+          const int v = P.item0 + b, s = v / P.per_seq, q0 = (v - s * P.per_seq) * kCap;
+          n = P.query_start_loc[s + 1] - P.query_start_loc[s];
+          n = (n < P.max_query_len ? n : P.max_query_len) - q0;
+          n = n > kCap ? kCap : n;
+          int ctx = P.context_lens[s];
+          ctx = ctx < 0 ? 0 : (ctx > (1 << 30) ? (1 << 30) : ctx);
+          top = n > 0 ? ctx + q0 + n : -1;   // -1: no such queries, nothing to write
+        }
         const int64_t width = (int64_t)P.max_blocks * P.block_size;
-        if (L > width) {                   // tokens that the table has no entry for
-          L = (int)width;
+        if (top > width) {                   // tokens that the table has no entry for
+          top = (int)width;
           if (blockIdx.x == 0) raise_status(P.status, SBK_ST_BAD_BLOCK);
         }
-        lens[b] = L;
-        c = L > 0 ? span_of<kUnit>(L, P.window_left).units : 1;   // an empty sequence keeps one: somebody writes its zeros
-        mx = max(mx, c);
-        c += kItemCost;
+        tops[b] = top;
+        cnts[b] = (uint8_t)(n > 0 ? n : 0);
+        if (top < 0 && P.seq_lens) tops[b] = top = 0;
+        if (top >= 0) {
+          c = top > 0 ? span_of<kUnit>(top, n, P.window_left).units : 1;   // an empty one keeps a unit: somebody writes its zeros
+          mx = max(mx, c);
+          c += kItemCost;
+        } else if (blockIdx.x == 0 && P.cut_by_item) {
+          P.cut[b] = kNotCut;
+        }
       }
       cnt[i] = c;
       sum += c;
@@ -219,20 +256,27 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   }
   const int total = pre[P.B], n_cta = (int)gridDim.x, me = (int)blockIdx.x;
   int per = (total + n_cta - 1) / n_cta;
-  if (per < kMinRun) per = kMinRun;
-  // A batch of near-equal sequences that fills the CTAs evenly streams fastest as whole sequences: no partials to write and fold.
+  if (per < 1) per = 1;
+  // A batch of near-equal items that fills the CTAs evenly streams fastest as whole items: no partials to write and fold.
   const int rounds = (P.B + n_cta - 1) / n_cta;
   const bool whole = 2 * P.B >= n_cta && (P.B <= n_cta || 10 * rounds * n_cta <= 11 * P.B) &&
                      (int64_t)misc[1] * P.B <= ((int64_t)total - (int64_t)kItemCost * P.B) / 8 * 9;
+  auto first_row = [&](int b) {
+    if (P.seq_lens) return P.item0 + b;
+    const int v = P.item0 + b, s = v / P.per_seq;
+    return P.query_start_loc[s] + (v - s * P.per_seq) * kCap;
+  };
 
-  if (warp == kConsumerWarps) {
+  if (warp == C::kWarps) {
     // ================================= producer =================================
     int it = 0;
     bool aborted = false;
     auto stream_item = [&](int b, int unit0, int n_units, int part) {
-      const int L = lens[b];
-      const int t0 = first_visible(L, 1, P.window_left);
-      const int32_t* table = P.block_tables + (int64_t)b * P.max_blocks;
+      const int top = tops[b], n_q = cnts[b];
+      const int t0 = first_visible(top, n_q, P.window_left);
+      const int seq = (P.item0 + b) / P.per_seq;
+      const int row = first_row(b);
+      const int32_t* table = P.block_tables + (int64_t)seq * P.max_blocks;
       int64_t pb_lane = -1;            // physical block of chunk (batch0 + lane): one table read per 32 chunks
       int batch0 = 0;
       const int n = n_units > 0 ? n_units : 1;
@@ -241,7 +285,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         if (n_units > 0 && (j == 0 || c0 + kChunks > batch0 + 32)) {
           batch0 = c0;
           const int lb = (c0 + lane) * kChunk / P.block_size;
-          pb_lane = (c0 + lane) * kChunk < L && lb < P.max_blocks ? (int64_t)table[lb] : -1;
+          pb_lane = (c0 + lane) * kChunk < top && lb < P.max_blocks ? (int64_t)table[lb] : -1;
         }
         const int s = it % kStages, use = it / kStages;
         if (use > 0 && !mbar_wait_bounded(bar_empty + 8 * s, (use - 1) & 1)) {
@@ -252,7 +296,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         if (misc[0]) { aborted = true; return; }
         const int base = c0 * kChunk;
         const int lo = base > t0 ? base : t0;
-        int hi = base + kUnit < L ? base + kUnit : L;
+        int hi = base + kUnit < top ? base + kUnit : top;
         if (n_units == 0 || hi < lo) hi = lo;
         // chunks of this stage that hold visible tokens: [ca, cb)
         const int ca = (lo - base) / kChunk, cb = hi > lo ? (hi - 1 - base) / kChunk + 1 : ca;
@@ -260,7 +304,6 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         const int x = lane & 15;
         const bool is_tile = lane >= 16;
         const int c = is_tile ? x % kChunks : x / KVH % kChunks;
-        // every lane reads its chunk's block; what it issues is decided below
         int src = c0 + c - batch0;
         src = src < 0 ? 0 : (src > 31 ? 31 : src);
         const int64_t pb = __shfl_sync(0xffffffffu, pb_lane, src);
@@ -268,7 +311,7 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         const bool bad = __any_sync(0xffffffffu, in && (pb < 0 || pb >= P.num_blocks));
         if (lane == 0) {
           StageInfo si;
-          si.b = b; si.tok_base = base; si.lo = lo; si.hi = hi; si.part = part;
+          si.row = row; si.n_q = n_q; si.top = top; si.tok_base = base; si.lo = lo; si.hi = hi; si.part = part;
           si.flags = (j == 0 ? kFirst : 0) | (j == n - 1 ? kLast : 0) | (bad ? kBad : 0);
           info[s] = si;
           if (bad) raise_status(P.status, SBK_ST_BAD_BLOCK);
@@ -279,10 +322,10 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           const int tin = (base + c * kChunk) % P.block_size;
           const uint32_t bar = bar_full + 8 * s;
           if (!is_tile) {
-            const int h = x % KVH;
-            const int64_t at = pb * P.scale_block_stride + (int64_t)h * P.block_size + tin;
-            const uint32_t dst = ring + kScaleOff + s * kScaleBytes + (((c >> 1) * KVH + h) * 2 + (c & 1)) * 16;
             if (x < kChunks * KVH) {
+              const int h = x % KVH;
+              const int64_t at = pb * P.scale_block_stride + (int64_t)h * P.block_size + tin;
+              const uint32_t dst = ring + C::kScaleOff + s * kScaleBytes + (((c >> 1) * KVH + h) * 2 + (c & 1)) * 16;
               cp_async16(dst, P.k_scale + at);
               cp_async16(dst + 128, P.v_scale + at);
             }
@@ -304,41 +347,45 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     };
 
     if (whole) {
-      if (lane == 0) P.cut[me] = make_int4(-1, 0, 0, 0);      // (a whole batch has as many sequences as CTAs at least)
+      if (lane == 0) P.cut[me] = kNotCut;      // (a whole batch has as many items as CTAs at least: entries are per CTA)
       for (int b = me; b < P.B && !aborted; b += n_cta) {
-        const Span sp = span_of<kUnit>(lens[b], P.window_left);
+        if (tops[b] < 0) continue;
+        const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left);
         stream_item(b, sp.first, sp.units, -1);
       }
     } else {
       const int64_t g0 = (int64_t)me * per;
       const int64_t g1 = g0 + per < total ? g0 + per : total;
       int b0 = 0;
-      int4 cut = make_int4(-1, 0, 0, 0);
+      int e = -1;
+      int4 cut = kNotCut;
       if (g0 < total) {
         int hi_b = P.B;                 // largest b with pre[b] <= g0
         while (hi_b - b0 > 1) {
           const int mid = (b0 + hi_b) >> 1;
           if (pre[mid] <= g0) b0 = mid; else hi_b = mid;
         }
-        // the sequence that holds the run's last slot: does it begin here and go on?
-        int e = b0, he = P.B;
+        // the item that holds the run's last slot: does it begin here and go on?
+        int he = P.B;
+        e = b0;
         while (he - e > 1) {
           const int mid = (e + he) >> 1;
           if (pre[mid] <= g1 - 1) e = mid; else he = mid;
         }
-        const int cr = lens[e] > 0 ? span_of<kUnit>(lens[e], P.window_left).units : 1;
-        if (pre[e] >= g0 && pre[e] + cr > g1) cut = make_int4(e, me, (pre[e] + cr - 1) / per - me + 1, 0);
+        const int cr = tops[e] > 0 ? span_of<kUnit>(tops[e], cnts[e], P.window_left).units : 1;
+        if (pre[e] >= g0 && pre[e] + cr > g1) cut = make_int4(first_row(e), me, (pre[e] + cr - 1) / per - me + 1, cnts[e]);
       }
       // (before anything is streamed: the folding kernel reads every entry, also of a launch that gave up on a wait)
-      if (P.cut_by_seq) {
+      if (P.cut_by_item) {
         for (int b = b0 + lane; g0 < total && b < P.B && pre[b] < g1; b += 32)
-          if (pre[b] >= g0) P.cut[b] = b == cut.x ? cut : make_int4(-1, 0, 0, 0);
+          if (pre[b] >= g0 && tops[b] >= 0) P.cut[b] = b == e ? cut : kNotCut;
       } else if (lane == 0) {
         P.cut[me] = cut;
       }
       if (g0 < total) {
         for (int b = b0; b < P.B && pre[b] < g1 && !aborted; ++b) {
-          const Span sp = span_of<kUnit>(lens[b], P.window_left);
+          if (tops[b] < 0) continue;
+          const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left);
           const int cr = sp.units > 0 ? sp.units : 1;
           const int va = (int)(g0 > pre[b] ? g0 - pre[b] : 0);
           if (va >= cr) continue;                               // only charged slots of b fall into this run
@@ -369,7 +416,8 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   }
 
   // ================================== consumers ==================================
-  const int hk = warp % KVH, sub = warp / KVH, G = P.H / KVH;
+  const int qg = warp >> 2, w4 = warp & 3;            // query group, warp of the group
+  const int hk = w4 % KVH, sub = w4 / KVH, G = P.H / KVH;
   const int g = lane >> 2, t = lane & 3;
   TO* const out = reinterpret_cast<TO*>(P.out);
 
@@ -383,9 +431,9 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   const int xk = (tokk & 7) ^ (lane >> 4), xv = (tokv & 7) ^ (lane >> 4);
   const int ta = g, tb8 = 8 + (g ^ 4);             // a thread's tokens in every sixteen
 
-  uint32_t qf[8][2];
-  float acc[8][4];
-  float m[2], l[2], rs[2], qs[2];                  // of heads 2t, 2t + 1 (rs = 2^-r)
+  uint32_t qf[NQ][8][2];
+  float acc[NQ][8][4];
+  float m[NQ][2], l[NQ][2], rs[NQ][2], qs[NQ][2];  // of heads 2t, 2t + 1 (rs = 2^-r)
   for (int it = 0;; ++it) {
     const int s = it % kStages;
     if (!mbar_wait_bounded(bar_full + 8 * s, (it / kStages) & 1)) {
@@ -397,233 +445,288 @@ decode_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     const uint32_t stage = ring + s * kStageBytes;
 
     if (si.flags & kFirst) {
-      // q of head g: dims 16c + 4t ... + 3
-      const bool head_ok = g < G;
-      const __nv_bfloat16* qp = P.q + (int64_t)si.b * P.q_stride + (int64_t)(hk * G + (head_ok ? g : 0)) * kD + 4 * t;
-      uint32_t w[16];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        w[2 * c] = *reinterpret_cast<const uint32_t*>(qp + 16 * c);
-        w[2 * c + 1] = *reinterpret_cast<const uint32_t*>(qp + 16 * c + 2);
+      for (int n = 0; n < NQ; ++n) {
+        // q of head g: dims 16c + 4t ... + 3 (zeros for a head or a query that is not there)
+        const int qi = qg * NQ + n;
+        const bool head_ok = g < G && qi < si.n_q;
+        const __nv_bfloat16* qp =
+            P.q + (int64_t)(si.row + (head_ok ? qi : 0)) * P.q_stride + (int64_t)(hk * G + (head_ok ? g : 0)) * kD + 4 * t;
+        uint32_t w[16];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          w[2 * c] = *reinterpret_cast<const uint32_t*>(qp + 16 * c);
+          w[2 * c + 1] = *reinterpret_cast<const uint32_t*>(qp + 16 * c + 2);
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (!head_ok) w[i] = 0u;
+          const float a = fabsf(__uint_as_float(w[i] << 16)), b = fabsf(__uint_as_float(w[i] & 0xffff0000u));
+          top = fmaxf(top, fmaxf(q8::finite(a) ? a : 0.f, q8::finite(b) ? b : 0.f));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = q8::row_exponent(top);
+        const float inv = q8::pow2i(-e), mine = P.scale_log2 * q8::pow2i(e);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)         // (an infinity stays one: the head's scores are NaN or infinite)
+          qf[n][i >> 1][i & 1] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          qs[n][i] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + i));
+          m[n][i] = kNegBig;
+          l[n][i] = 0.f;
+          rs[n][i] = 1.f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) acc[n][mt][0] = acc[n][mt][1] = acc[n][mt][2] = acc[n][mt][3] = 0.f;
       }
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (!head_ok) w[i] = 0u;
-        const float a = fabsf(__uint_as_float(w[i] << 16)), b = fabsf(__uint_as_float(w[i] & 0xffff0000u));
-        top = fmaxf(top, fmaxf(q8::finite(a) ? a : 0.f, q8::finite(b) ? b : 0.f));
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = q8::row_exponent(top);
-      const float inv = q8::pow2i(-e), mine = P.scale_log2 * q8::pow2i(e);
-#pragma unroll
-      for (int i = 0; i < 16; ++i)           // (an infinity stays one, or becomes one: the head's scores are NaN or infinite)
-        qf[i >> 1][i & 1] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        qs[i] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + i));
-        m[i] = kNegBig;
-        l[i] = 0.f;
-        rs[i] = 1.f;
-      }
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) acc[mt][0] = acc[mt][1] = acc[mt][2] = acc[mt][3] = 0.f;
     }
 
     const int tb = si.tok_base + 32 * sub;                      // my 32 tokens
     const int vlo = si.lo > tb ? si.lo : tb, vhi = si.hi < tb + 32 ? si.hi : tb + 32;
-    if (!(si.flags & kBad) && vhi > vlo) {
-      const bool ragged = vlo > tb || vhi < tb + 32;
-      if (ragged) {
+    if (!(si.flags & kBad) && vhi > vlo && (QG == 1 || qg * NQ < si.n_q)) {
+      const bool edge = vlo > tb || vhi < tb + 32;
+      if (edge) {
         // rows outside the visible range hold anything, or older data: a zero probability must not meet a NaN code
+        // (groups of warps that share the tile all write the same zeros)
         for (int row = lane >> 3; row < 32; row += 4)
           if (tb + row < vlo || tb + row >= vhi)
             *reinterpret_cast<uint4*>(smem + s * kStageBytes + kTileBytes + tile0 + (row >> 4) * kChunkBytes + (row & 15) * 128 +
                                       (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
-      // ---- scores (without the scales): [16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
-      float sc[2][4], kv[2][2], ve[2][2];
-      const uint8_t* se = smem + kScaleOff + s * kScaleBytes + (sub * KVH + hk) * 32;
+      // ---- scores: [query][16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
+      float sc[NQ][2][4], ve[2][2];
+      const uint8_t* se = smem + C::kScaleOff + s * kScaleBytes + (sub * KVH + hk) * 32;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        kv[h][0] = __uint_as_float((uint32_t)se[16 * h + ta] << 23);
-        kv[h][1] = __uint_as_float((uint32_t)se[16 * h + tb8] << 23);
+        const float ka = __uint_as_float((uint32_t)se[16 * h + ta] << 23), kb = __uint_as_float((uint32_t)se[16 * h + tb8] << 23);
         ve[h][0] = __uint_as_float((uint32_t)se[128 + 16 * h + ta] << 23);
         ve[h][1] = __uint_as_float((uint32_t)se[128 + 16 * h + tb8] << 23);
-        float ca[4] = {0.f, 0.f, 0.f, 0.f}, cb[4] = {0.f, 0.f, 0.f, 0.f};
+        float ca[NQ][4], cb[NQ][4];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ca[n][i] = cb[n][i] = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
-          uint32_t w[4];
+          uint32_t w[4], a[4];
           ldmatrix_x4(w, stage + h * kChunkBytes + k0 + ((c ^ xk) << 4));
-          mma_codes(ca, w[0], w[1], qf[c][0], qf[c][1]);
-          mma_codes(cb, w[2], w[3], qf[c + 1][0], qf[c + 1][1]);
+          widen(a, w[0], w[1]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) mma_f16(ca[n], a, qf[n][c][0], qf[n][c][1]);
+          widen(a, w[2], w[3]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) mma_f16(cb[n], a, qf[n][c + 1][0], qf[n][c + 1][1]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[h][i] = (ca[i] + cb[i]) * (qs[i & 1] * kv[h][i >> 1]);
-        if (ragged) {
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[n][h][i] = (ca[n][i] + cb[n][i]) * (qs[n][i & 1] * (i < 2 ? ka : kb));
+      }
+      if (edge) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
           const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
-          if (a < vlo || a >= vhi) { sc[h][0] = sc[h][1] = -INFINITY; ve[h][0] = 0.f; }
-          if (b < vlo || b >= vhi) { sc[h][2] = sc[h][3] = -INFINITY; ve[h][1] = 0.f; }
+          if (a < vlo || a >= vhi) ve[h][0] = 0.f;
+          if (b < vlo || b >= vhi) ve[h][1] = 0.f;
         }
       }
-      // ---- p = 2^(s - m), w = p * 2^(ev - r) with the offsets in use; they move only when a w leaves fp16 ----
-      float p[2][4], w[2][4], wtop, ptop;
-      auto weigh = [&]() {
-        wtop = ptop = 0.f;
+      uint32_t pf[NQ][2][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-#pragma unroll
-            for (int j = i; j < i + 2; ++j) {
-              p[h][j] = fast_exp2(sc[h][j] - m[j & 1]);
-              w[h][j] = p[h][j] * (ve[h][j >> 1] * rs[j & 1]);
-            }
-            wtop = tc5::fmax3(wtop, w[h][i], w[h][i + 1]);
-            ptop = tc5::fmax3(ptop, p[h][i], p[h][i + 1]);
-          }
-      };
-      weigh();
-      if (__any_sync(0xffffffffu, wtop > kMostW || ptop > kMostP)) {
-        // (rare: the first tokens of an item, and where a score or a V row outgrows all before it by 2^8)
-        float mx[2], ne[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) mx[i] = fmaxf(fmaxf(sc[0][i], sc[0][2 + i]), fmaxf(sc[1][i], sc[1][2 + i]));
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+      for (int n = 0; n < NQ; ++n) {
+        // keys that this query sees; with several queries each has its own edge
+        int nlo = vlo, nhi = vhi;
+        if (NQ * QG > 1) {
+          const int last = si.top - si.n_q + qg * NQ + n;            // the query's own position
+          const int first = P.window_left < 0 || last <= P.window_left ? 0 : last - P.window_left;
+          nlo = first > vlo ? first : vlo;
+          nhi = last + 1 < vhi ? last + 1 : vhi;
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float mn = fmaxf(m[i], mx[i]);
-          ne[i] = fast_exp2(m[i] - mn);
-          l[i] *= ne[i];
-          m[i] = mn;
-          mx[i] = 0.f;                        // from here on: the largest p * 2^ev
+        if (nlo > tb || nhi < tb + 32) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            mx[i] = fmaxf(mx[i], fast_exp2(sc[h][i] - mn) * ve[h][0]);
-            mx[i] = fmaxf(mx[i], fast_exp2(sc[h][2 + i] - mn) * ve[h][1]);
+            const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
+            if (a < nlo || a >= nhi) sc[n][h][0] = sc[n][h][1] = -INFINITY;
+            if (b < nlo || b >= nhi) sc[n][h][2] = sc[n][h][3] = -INFINITY;
           }
         }
+        // ---- p = 2^(s - m), w = p * 2^(ev - r) with the offsets in use; they move only when a w leaves fp16 ----
+        float p[2][4], w[2][4], wtop, ptop;
+        auto weigh = [&]() {
+          wtop = ptop = 0.f;
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
-        }
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          // 2^-r: the power of two that takes the largest w so far to [2^6, 2^7) (those before had one of 2^6 at least)
-          const float had = ne[i] * 64.f / rs[i];
-          int e = (int)(__float_as_uint(fmaxf(mx[i], had)) >> 23) - 127;
-          e = e < -64 ? -64 : (e > 63 ? 63 : e);
-          const float rn = q8::pow2i(6 - e), al = ne[i] * (rn / rs[i]);
-          rs[i] = rn;
+            for (int i = 0; i < 4; i += 2) {
 #pragma unroll
-          for (int mt = 0; mt < 8; ++mt) { acc[mt][i] *= al; acc[mt][2 + i] *= al; }
-        }
+              for (int j = i; j < i + 2; ++j) {
+                p[h][j] = fast_exp2(sc[n][h][j] - m[n][j & 1]);
+                w[h][j] = p[h][j] * (ve[h][j >> 1] * rs[n][j & 1]);
+              }
+              wtop = tc5::fmax3(wtop, w[h][i], w[h][i + 1]);
+              ptop = tc5::fmax3(ptop, p[h][i], p[h][i + 1]);
+            }
+        };
         weigh();
+        if (__any_sync(0xffffffffu, wtop > kMostW || ptop > kMostP)) {
+          // (rare: the first tokens of an item, and where a score or a V row outgrows all before it by 2^8)
+          float mx[2], ne[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            mx[i] = fmaxf(fmaxf(sc[n][0][i], sc[n][0][2 + i]), fmaxf(sc[n][1][i], sc[n][1][2 + i]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+            mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float mn = fmaxf(m[n][i], mx[i]);
+            ne[i] = fast_exp2(m[n][i] - mn);
+            l[n][i] *= ne[i];
+            m[n][i] = mn;
+            mx[i] = 0.f;                        // from here on: the largest p * 2^ev
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              mx[i] = fmaxf(mx[i], fast_exp2(sc[n][h][i] - mn) * ve[h][0]);
+              mx[i] = fmaxf(mx[i], fast_exp2(sc[n][h][2 + i] - mn) * ve[h][1]);
+            }
+          }
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) {
+            mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
+            mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            // 2^-r: the power of two that takes the largest w so far to [2^6, 2^7) (those before had one of 2^6 at least)
+            const float had = ne[i] * 64.f / rs[n][i];
+            int e = (int)(__float_as_uint(fmaxf(mx[i], had)) >> 23) - 127;
+            e = e < -64 ? -64 : (e > 63 ? 63 : e);
+            const float rn = q8::pow2i(6 - e), al = ne[i] * (rn / rs[n][i]);
+            rs[n][i] = rn;
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) { acc[n][mt][i] *= al; acc[n][mt][2 + i] *= al; }
+          }
+          weigh();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          l[n][0] += p[h][0] + p[h][2];
+          l[n][1] += p[h][1] + p[h][3];
+          pf[n][h][0] = movmatrix_trans(pack_f16x2(w[h][0], w[h][1]));
+          pf[n][h][1] = movmatrix_trans(pack_f16x2(w[h][2], w[h][3]));
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        l[0] += p[h][0] + p[h][2];
-        l[1] += p[h][1] + p[h][3];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t p0 = movmatrix_trans(pack_f16x2(w[h][0], w[h][1])), p1 = movmatrix_trans(pack_f16x2(w[h][2], w[h][3]));
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
-          uint32_t v[4];
+          uint32_t v[4], a[4];
           ldmatrix_b8_trans(v, stage + h * kChunkBytes + v0 + ((c ^ xv) << 4));
-          mma_codes(acc[c], v[0], v[1], p0, p1);
-          mma_codes(acc[c + 1], v[2], v[3], p0, p1);
+          widen(a, v[0], v[1]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) mma_f16(acc[n][c], a, pf[n][h][0], pf[n][h][1]);
+          widen(a, v[2], v[3]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) mma_f16(acc[n][c + 1], a, pf[n][h][0], pf[n][h][1]);
         }
       }
-      if (ragged) fence_proxy_async_smem();   // my zero fill precedes the next copy into these rows
+      if (edge) fence_proxy_async_smem();   // my zero fill precedes the next copy into these rows
     }
     __syncwarp();
     // the last stage of an item becomes the scratch of its output before it goes back to the producer
     if (lane == 0 && !(si.flags & kLast)) mbar_arrive(bar_empty + 8 * s);
     if (!(si.flags & kLast)) continue;
 
-    // ================= end of an item: its output row, or its partial =================
-    // (where nothing was visible m is kNegBig, l and O are 0)
-    float fix[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], off);
-      fix[i] = 1.f / rs[i];
-    }
-    const int64_t prow = (int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * P.H;
-    // [head][dim] floats of every warp in shared memory; warps that share a kv head (each took other tokens) are added up here
+    // ================= end of an item: its output rows, or its partials =================
+    // [head][dim] floats of every warp in shared memory, four-float columns XOR-ed by the head (no bank is met twice);
+    // warps that share a kv head (each took other tokens) are added up from there
     uint8_t* mbuf = smem + s * kStageBytes;
     float* wo = reinterpret_cast<float*>(mbuf + warp * kMergeWarpBytes);
-    float* wml = wo + kMaxG * kHeadStride;
-    consumer_bar();                         // every warp is done reading this stage
+    float* wml = reinterpret_cast<float*>(smem + C::kMlOff) + warp * 16;
 #pragma unroll
-    for (int mt = 0; mt < 8; ++mt)
+    for (int n = 0; n < NQ; ++n) {
+      // (where nothing was visible m is kNegBig, l and O are 0)
+      float fix[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        wo[(2 * t + i) * kHeadStride + 16 * mt + g] = acc[mt][i] * fix[i];
-        wo[(2 * t + i) * kHeadStride + 16 * mt + g + 8] = acc[mt][2 + i] * fix[i];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], off);
+        fix[i] = 1.f / rs[n][i];
       }
-    if (g == 0) {
-      wml[2 * t] = m[0]; wml[2 * t + 1] = m[1];
-      wml[8 + 2 * t] = l[0]; wml[8 + 2 * t + 1] = l[1];
-    }
-    if constexpr (kSub > 1) consumer_bar(); else __syncwarp();
-    // heads go round the warps (one warp to a kv head: its own heads), a lane takes four dims
-    const int h_lo = kSub > 1 ? warp : hk * G, h_hi = kSub > 1 ? P.H : hk * G + G, h_step = kSub > 1 ? kConsumerWarps : 1;
+      consumer_bar<C::kConsumers>();          // every warp is done reading this stage, or the results of the query before
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int hrow = 2 * t + i, x = (hrow & 7) << 2;
+          wo[hrow * kD + ((16 * mt + g) ^ x)] = acc[n][mt][i] * fix[i];
+          wo[hrow * kD + ((16 * mt + g + 8) ^ x)] = acc[n][mt][2 + i] * fix[i];
+        }
+      if (g == 0) {
+        wml[2 * t] = m[n][0]; wml[2 * t + 1] = m[n][1];
+        wml[8 + 2 * t] = l[n][0]; wml[8 + 2 * t + 1] = l[n][1];
+      }
+      if constexpr (kSub > 1) consumer_bar<C::kConsumers>(); else __syncwarp();
+      const int qi = qg * NQ + n;
+      if (qi < si.n_q) {
+        const int64_t orow = (int64_t)si.row + qi;
+        const int64_t prow = ((int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * kCap + qi) * P.H;
+        // heads go round the group's warps (one warp to a kv head: its own heads), a lane takes four dims
+        const int h_lo = kSub > 1 ? w4 : hk * G, h_hi = kSub > 1 ? P.H : hk * G + G, h_step = kSub > 1 ? 4 : 1;
 #pragma unroll 2
-    for (int h = h_lo; h < h_hi; h += h_step) {
-      const int kh = h / G, row = h - kh * G;
-      float M = -INFINITY;
+        for (int h = h_lo; h < h_hi; h += h_step) {
+          const int kh = h / G, row = h - kh * G;
+          float M = -INFINITY;
 #pragma unroll
-      for (int w2 = 0; w2 < kSub; ++w2)
-        M = fmaxf(M, reinterpret_cast<const float*>(mbuf + (kh + KVH * w2) * kMergeWarpBytes)[kMaxG * kHeadStride + row]);
-      const float Ms = fmaxf(M, kNegBig);
-      float L = 0.f;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int w2 = 0; w2 < kSub; ++w2)
+            M = fmaxf(M, reinterpret_cast<const float*>(smem + C::kMlOff)[(qg * 4 + kh + KVH * w2) * 16 + row]);
+          const float Ms = fmaxf(M, kNegBig);
+          float L = 0.f;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w2 = 0; w2 < kSub; ++w2) {
-        const float* po = reinterpret_cast<const float*>(mbuf + (kh + KVH * w2) * kMergeWarpBytes);
-        const float wgt = kSub > 1 ? fast_exp2(po[kMaxG * kHeadStride + row] - Ms) : 1.f;
-        const float4 o = *reinterpret_cast<const float4*>(po + row * kHeadStride + 4 * lane);
-        L += po[kMaxG * kHeadStride + 8 + row] * wgt;
-        O.x += o.x * wgt; O.y += o.y * wgt; O.z += o.z * wgt; O.w += o.w * wgt;
-      }
-      if (si.part < 0) {
-        const float f = inverse(L);
-        store4(out + (int64_t)si.b * P.out_stride + (int64_t)h * kD + 4 * lane, make_float4(O.x * f, O.y * f, O.z * f, O.w * f));
-        if (P.lse_out && lane == 0) P.lse_out[(int64_t)si.b * P.H + h] = row_lse(M, L);
-      } else {
-        *reinterpret_cast<float4*>(P.ws_o + (prow + h) * kD + 4 * lane) = O;
-        if (lane == 0) P.ws_ml[prow + h] = make_float2(M, L);
+          for (int w2 = 0; w2 < kSub; ++w2) {
+            const int src = qg * 4 + kh + KVH * w2;
+            const float* po = reinterpret_cast<const float*>(mbuf + src * kMergeWarpBytes);
+            const float* ml = reinterpret_cast<const float*>(smem + C::kMlOff) + src * 16;
+            const float wgt = kSub > 1 ? fast_exp2(ml[row] - Ms) : 1.f;
+            const float4 o = *reinterpret_cast<const float4*>(po + row * kD + ((4 * lane) ^ ((row & 7) << 2)));
+            L += ml[8 + row] * wgt;
+            O.x += o.x * wgt; O.y += o.y * wgt; O.z += o.z * wgt; O.w += o.w * wgt;
+          }
+          if (si.part < 0) {
+            const float f = inverse(L);
+            store4(out + orow * P.out_stride + (int64_t)h * kD + 4 * lane, make_float4(O.x * f, O.y * f, O.z * f, O.w * f));
+            if (P.lse_out && lane == 0) P.lse_out[orow * P.H + h] = row_lse(M, L);
+          } else {
+            *reinterpret_cast<float4*>(P.ws_o + (prow + h) * kD + 4 * lane) = O;
+            if (lane == 0) P.ws_ml[prow + h] = make_float2(M, L);
+          }
+        }
       }
     }
     fence_proxy_async_smem();               // these accesses precede the copies that refill the stage
-    if constexpr (kSub > 1) consumer_bar(); else __syncwarp();
+    if constexpr (kSub > 1) consumer_bar<C::kConsumers>(); else __syncwarp();
     if (lane == 0) mbar_arrive(bar_empty + 8 * s);
   }
 }
 
-// Folds the partials of the sequences that were cut. Block (x, y): entry x of `cut`, heads HPC y ...; WPH warps share a head,
-// each taking every WPH-th piece with its loads issued eight at a time.
+// Folds the partials of the items that were cut. Block (x, y): entry x of `cut`, heads HPC y ... of its cap * H (query, head) pairs;
+// WPH warps share one, each taking every WPH-th piece with its loads issued eight at a time.
 template <int WPH, int HPC, typename TO>
-__global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P) {
+__global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P, int cap) {
   __shared__ float4 part_o[WPH * HPC][32];
   __shared__ float2 part_ml[WPH * HPC];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 cut = P.cut[blockIdx.x];                    // sequence, first CTA, pieces
+  const int4 cut = P.cut[blockIdx.x];                    // first query row, first CTA, pieces, queries
   if (cut.z <= 1) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y * HPC + warp / WPH, w = warp % WPH;
-  const bool on = h < P.H;
+  const int hq = blockIdx.y * HPC + warp / WPH, w = warp % WPH;
+  const bool on = hq < cut.w * P.H;
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kU = 8;
@@ -636,7 +739,7 @@ __global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P) {
       ml[u] = make_float2(-INFINITY, 0.f);
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < cut.z) {
-        const int64_t row = (int64_t)(2 * (cut.y + i) + (i == 0 ? 1 : 0)) * P.H + h;
+        const int64_t row = (int64_t)(2 * (cut.y + i) + (i == 0 ? 1 : 0)) * cap * P.H + hq;
         ml[u] = __ldcg(P.ws_ml + row);
         o[u] = __ldcg(reinterpret_cast<const float4*>(P.ws_o + row * kD) + lane);
       }
@@ -673,52 +776,52 @@ __global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P) {
     Ot.x += o.x * wgt; Ot.y += o.y * wgt; Ot.z += o.z * wgt; Ot.w += o.w * wgt;
   }
   const float f = inverse(Lt);
-  store4(reinterpret_cast<TO*>(P.out) + (int64_t)cut.x * P.out_stride + (int64_t)h * kD + 4 * lane,
+  const int qi = hq / P.H, h = hq - qi * P.H;
+  store4(reinterpret_cast<TO*>(P.out) + (int64_t)(cut.x + qi) * P.out_stride + (int64_t)h * kD + 4 * lane,
          make_float4(Ot.x * f, Ot.y * f, Ot.z * f, Ot.w * f));
-  if (P.lse_out && lane == 0) P.lse_out[(int64_t)cut.x * P.H + h] = row_lse(Mt, Lt);
+  if (P.lse_out && lane == 0) P.lse_out[(int64_t)(cut.x + qi) * P.H + h] = row_lse(Mt, Lt);
 }
 
-static size_t cut_bytes() { return (size_t)kMaxCtas * sizeof(int4); }
+constexpr int kMaxPartials = 2 * 2 * kMaxSms;          // two per CTA, two CTAs per SM with one query group
+static size_t cut_bytes() { return (size_t)(2 * kMaxSms) * sizeof(int4); }
 
-template <int KVH, typename TO>
-static int launch(const Params& P0, int B_total, int sms, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
-  auto kern = decode_kernel<KVH, TO>;
+template <int KVH, int NQ, int QG, typename TO>
+static int launch(const char* who, const Params& P0, int64_t items, int sms, const CUtensorMap& map_k, const CUtensorMap& map_v,
+                  cudaStream_t st) {
+  using C = Cfg<QG>;
+  constexpr int kCap = NQ * QG, kUnit = 32 * 4 / KVH;
+  auto kern = stream_kernel<KVH, NQ, QG, TO>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     if (e != cudaSuccess) {
-      set_error("sbk_swa_decode_q8: cannot opt in to %d bytes of shared memory: %s", kSmemBytes, cudaGetErrorString(e));
+      set_error("%s: cannot opt in to %d bytes of shared memory: %s", who, C::kSmemBytes, cudaGetErrorString(e));
       return SBK_E_LAUNCH;
     }
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  constexpr int kUnit = 32 * kConsumerWarps / KVH;
-  const int n_ctas = 2 * sms < kMaxCtas ? 2 * sms : kMaxCtas;
-  for (int b0 = 0; b0 < B_total; b0 += kMaxSeqs) {
+  const int n_ctas = C::kCtasPerSm * (sms < kMaxSms ? sms : kMaxSms);
+  for (int64_t b0 = 0; b0 < items; b0 += kMaxSeqs) {
     Params P = P0;
-    P.B = B_total - b0 < kMaxSeqs ? B_total - b0 : kMaxSeqs;
-    P.q = P0.q + (int64_t)b0 * P0.q_stride;
-    P.block_tables = P0.block_tables + (int64_t)b0 * P0.max_blocks;
-    P.seq_lens = P0.seq_lens + b0;
-    P.out = (uint8_t*)P0.out + (int64_t)b0 * P0.out_stride * sizeof(TO);
-    if (P0.lse_out) P.lse_out = P0.lse_out + (int64_t)b0 * P0.H;
+    P.item0 = (int)b0;
+    P.B = items - b0 < kMaxSeqs ? (int)(items - b0) : kMaxSeqs;
     // no more CTAs than there can be units of work
-    const int64_t width = (int64_t)P.max_blocks * P.block_size;
-    const int64_t vis = P.window_left < 0 || width < (int64_t)P.window_left + 1 ? width : (int64_t)P.window_left + 1;
+    const int64_t width = (int64_t)P.max_blocks * P.block_size, seen = (int64_t)P.window_left + kCap;
+    const int64_t vis = P.window_left < 0 || width < seen ? width : seen;
     const int64_t most = (int64_t)P.B * (vis / kUnit + 2 + kItemCost);
     int grid = (int)(most < n_ctas ? most : n_ctas);
-    // a batch between one and two sequences per SM: one CTA each, so that every SM has work either way of cutting
+    // a batch between one and two items per SM: one CTA each, so that every SM has work either way of cutting
     if (2 * P.B >= n_ctas && P.B < n_ctas) grid = P.B;
-    P.cut_by_seq = P.B < grid;
-    kern<<<grid, kThreads, kSmemBytes, st>>>(P, map_k, map_v);
-    int rc = check_launch("sbk_swa_decode_q8");
+    P.cut_by_item = P.B < grid;
+    kern<<<grid, C::kThreads, C::kSmemBytes, st>>>(P, map_k, map_v);
+    const int rc = check_launch(who);
     if (rc != SBK_OK) return rc;
-    // Few sequences are cut into many pieces: sixteen warps to a head. Else four heads to a block of eight warps.
+    // Few items are cut into many pieces: sixteen warps to a head. Else four heads to a block of eight warps.
     const bool few = P.B <= 32;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(P.cut_by_seq ? P.B : grid, few ? P.H : (P.H + 3) / 4);
+    cfg.gridDim = dim3(P.cut_by_item ? P.B : grid, few ? P.H * kCap : (P.H * kCap + 3) / 4);
     cfg.blockDim = dim3(few ? 512 : 256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -726,22 +829,68 @@ static int launch(const Params& P0, int B_total, int sms, const CUtensorMap& map
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, fold_kernel<16, 1, TO>, P) : cudaLaunchKernelEx(&cfg, fold_kernel<2, 4, TO>, P);
+    const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, fold_kernel<16, 1, TO>, P, kCap) : cudaLaunchKernelEx(&cfg, fold_kernel<2, 4, TO>, P, kCap);
     if (e != cudaSuccess) {
-      set_error("sbk_swa_decode_q8: launch of the folding kernel failed: %s", cudaGetErrorString(e));
+      set_error("%s: launch of the folding kernel failed: %s", who, cudaGetErrorString(e));
       return SBK_E_LAUNCH;
     }
   }
   return SBK_OK;
 }
 
+// rows of partials per head: runs have half the CTAs (two query groups each) and four queries to an item
+static size_t partial_rows(bool runs) { return (size_t)kMaxPartials * (runs ? 2 : 1); }
+size_t workspace_bytes(int H, bool runs) { return cut_bytes() + partial_rows(runs) * H * (kD + 2) * sizeof(float); }
+
+int stream_cache(const char* who, const Call& c, cudaStream_t st) {
+  const bool runs = c.seq_lens == nullptr;
+  Params P = {};
+  P.q = (const __nv_bfloat16*)c.q; P.q_stride = c.q_stride;
+  P.k_scale = (const uint8_t*)c.k_scale; P.v_scale = (const uint8_t*)c.v_scale; P.scale_block_stride = c.scale_block_stride;
+  P.block_tables = c.block_tables; P.max_blocks = c.max_blocks; P.seq_lens = c.seq_lens;
+  P.query_start_loc = c.query_start_loc; P.context_lens = c.context_lens; P.max_query_len = c.max_query_len;
+  P.per_seq = runs ? (c.max_query_len + 3) / 4 : 1;
+  P.H = c.H; P.num_blocks = c.num_blocks; P.block_size = c.block_size; P.window_left = c.window_left;
+  P.scale_log2 = c.scale * kLog2e; P.out = c.out; P.out_stride = c.out_stride; P.lse_out = c.lse_out; P.status = c.status;
+  P.cut = (int4*)c.workspace;
+  P.ws_o = (float*)((uint8_t*)c.workspace + cut_bytes());
+  P.ws_ml = (float2*)(P.ws_o + partial_rows(runs) * c.H * kD);
+  static int sm_count[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int sms = dev >= 0 && dev < 64 ? sm_count[dev] : 0;
+  if (sms == 0) {
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (sms <= 0) sms = 148;
+    if (dev >= 0 && dev < 64) sm_count[dev] = sms;
+  }
+  MapKey keys[2] = {MapKey{c.k_cache, c.kvh, c.num_blocks, c.block_size, c.cache_block_stride, c.kvh},
+                    MapKey{c.v_cache, c.kvh, c.num_blocks, c.block_size, c.cache_block_stride, c.kvh}};
+  for (MapKey& k : keys) { k.tok_stride = (int64_t)c.kvh * kD; k.rows = c.kvh; }
+  CUtensorMap maps[2];
+  if (!get_maps(maps, keys, 2, &P.tile_copy)) {
+    set_error("%s: cuTensorMapEncodeTiled rejected the cache geometry (blocks=%lld block=%d kvh=%d)", who,
+              (long long)c.num_blocks, c.block_size, c.kvh);
+    return SBK_E_ARG;
+  }
+  const int64_t items = (int64_t)c.n_seqs * P.per_seq;
+#define SBK_STREAM(NQ, QG, TO)                                                            \
+  switch (c.kvh) {                                                                        \
+    case 1: return launch<1, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);       \
+    case 2: return launch<2, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);       \
+    default: return launch<4, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);      \
+  }
+  if (runs) { SBK_STREAM(2, 2, __nv_bfloat16) }
+  if (c.out_dtype == SBK_BF16) { SBK_STREAM(1, 1, __nv_bfloat16) } else { SBK_STREAM(1, 1, float) }
+#undef SBK_STREAM
+}
+
 }  // namespace decode_q8
 }  // namespace sbk
 
 extern "C" size_t sbk_swa_decode_q8_workspace_bytes(int B, int H, int D) {
-  using namespace sbk::decode_q8;
   if (B <= 0 || H <= 0 || D <= 0) return 0;
-  return cut_bytes() + (size_t)kMaxCtas * 2 * H * ((size_t)D + 2) * sizeof(float);
+  return sbk::decode_q8::workspace_bytes(H, false);
 }
 
 extern "C" int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void* k_cache, const void* v_cache,
@@ -792,40 +941,13 @@ extern "C" int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void
     set_error("sbk_swa_decode_q8: workspace must be 16-byte aligned");
     return SBK_E_ALIGN;
   }
-  Params P = {};
-  P.q = (const __nv_bfloat16*)q; P.q_stride = q_seq_stride;
-  P.k_scale = (const uint8_t*)k_scale; P.v_scale = (const uint8_t*)v_scale; P.scale_block_stride = scale_block_stride_bytes;
-  P.block_tables = block_tables; P.max_blocks = max_blocks; P.seq_lens = seq_lens;
-  P.H = H; P.num_blocks = num_blocks; P.block_size = block_size; P.window_left = window_left;
-  P.scale_log2 = scale * kLog2e; P.out = out; P.out_stride = out_seq_stride; P.lse_out = lse_out; P.status = status;
-  P.cut = (int4*)workspace;
-  P.ws_o = (float*)((uint8_t*)workspace + cut_bytes());
-  P.ws_ml = (float2*)(P.ws_o + (size_t)kMaxCtas * 2 * H * D);
-  static int sm_count[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  int sms = dev >= 0 && dev < 64 ? sm_count[dev] : 0;
-  if (sms == 0) {
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (sms <= 0) sms = 148;
-    if (dev >= 0 && dev < 64) sm_count[dev] = sms;
-  }
-  MapKey keys[2] = {MapKey{k_cache, kvh, num_blocks, block_size, cache_block_stride_bytes, kvh},
-                    MapKey{v_cache, kvh, num_blocks, block_size, cache_block_stride_bytes, kvh}};
-  for (MapKey& k : keys) { k.tok_stride = (int64_t)kvh * kD; k.rows = kvh; }
-  CUtensorMap maps[2];
-  if (!get_maps(maps, keys, 2, &P.tile_copy)) {
-    set_error("sbk_swa_decode_q8: cuTensorMapEncodeTiled rejected the cache geometry (blocks=%lld block=%d kvh=%d)",
-              (long long)num_blocks, block_size, kvh);
-    return SBK_E_ARG;
-  }
-  cudaStream_t st = (cudaStream_t)stream;
-#define SBK_DECODE_Q8(TO)                                                 \
-  switch (kvh) {                                                          \
-    case 1: return launch<1, TO>(P, B, sms, maps[0], maps[1], st);        \
-    case 2: return launch<2, TO>(P, B, sms, maps[0], maps[1], st);        \
-    default: return launch<4, TO>(P, B, sms, maps[0], maps[1], st);       \
-  }
-  if (out_dtype == SBK_BF16) { SBK_DECODE_Q8(__nv_bfloat16) } else { SBK_DECODE_Q8(float) }
-#undef SBK_DECODE_Q8
+  Call c = {};
+  c.q = q; c.q_stride = q_seq_stride;
+  c.k_cache = k_cache; c.v_cache = v_cache; c.k_scale = k_scale; c.v_scale = v_scale;
+  c.cache_block_stride = cache_block_stride_bytes; c.scale_block_stride = scale_block_stride_bytes;
+  c.block_tables = block_tables; c.max_blocks = max_blocks; c.seq_lens = seq_lens; c.max_query_len = 1;
+  c.n_seqs = B; c.H = H; c.kvh = kvh; c.num_blocks = num_blocks; c.block_size = block_size; c.window_left = window_left;
+  c.scale = scale; c.out = out; c.out_dtype = out_dtype; c.out_stride = out_seq_stride; c.lse_out = lse_out;
+  c.workspace = workspace; c.status = status;
+  return stream_cache("sbk_swa_decode_q8", c, (cudaStream_t)stream);
 }

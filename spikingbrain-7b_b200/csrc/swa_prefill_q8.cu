@@ -22,6 +22,7 @@
 #include "kv_q8.cuh"
 #include "sbk_tcgen05.cuh"
 #include "sbk_tma.cuh"
+#include "swa_decode_q8.cuh"
 
 namespace sbk {
 namespace prefill_q8 {
@@ -438,6 +439,11 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   if (warp == kSoftmaxWarps + 2) tmem_dealloc(tmem, kTmemCols);
 }
 
+// Runs of at most kFew queries go through the kernel of the single tokens, which reads the cache once for four queries and
+// expands nothing.
+constexpr int kFew = 16;
+static bool few_queries(int max_query_len, int kvh) { return max_query_len <= kFew && (kvh == 1 || kvh == 2 || kvh == 4); }
+
 // dense rows of a sequence, and sequences that share one scratch
 struct Layout { int64_t rows_per_seq; int group; };
 static Layout layout_of(int n_seqs, int max_query_len, int max_blocks, int kvh, int block_size, int window_left) {
@@ -460,6 +466,7 @@ extern "C" size_t sbk_swa_prefill_q8_workspace_bytes(int n_seqs, int max_query_l
                                                      int window_left) {
   using namespace sbk::prefill_q8;
   if (n_seqs <= 0 || max_query_len <= 0 || max_blocks <= 0 || kvh <= 0 || D <= 0 || block_size <= 0) return 0;
+  if (few_queries(max_query_len, kvh)) return sbk::decode_q8::workspace_bytes(8 * kvh, true);   // H is 8 * kvh at the most
   const Layout y = layout_of(n_seqs, max_query_len, max_blocks, kvh, block_size, window_left);
   return (size_t)(y.rows_per_seq * y.group) * kvh * D * 4;
 }
@@ -500,6 +507,27 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     set_error("sbk_swa_prefill_q8: a block stride is smaller than the block it spans");
     return SBK_E_ARG;
   }
+  const size_t need = sbk_swa_prefill_q8_workspace_bytes(n_seqs, max_query_len, max_blocks, kvh, D, block_size, window_left);
+  if (!workspace || workspace_bytes < need) {
+    set_error("sbk_swa_prefill_q8: workspace of %zu bytes given, %zu needed", workspace ? workspace_bytes : 0, need);
+    return SBK_E_WORKSPACE;
+  }
+  if (!aligned16(workspace)) {
+    set_error("sbk_swa_prefill_q8: workspace must be 16-byte aligned");
+    return SBK_E_ALIGN;
+  }
+  if (few_queries(max_query_len, kvh)) {
+    decode_q8::Call c = {};
+    c.q = q; c.q_stride = q_tok_stride;
+    c.k_cache = k_cache; c.v_cache = v_cache; c.k_scale = k_scale; c.v_scale = v_scale;
+    c.cache_block_stride = cache_block_stride_bytes; c.scale_block_stride = scale_block_stride_bytes;
+    c.block_tables = block_tables; c.max_blocks = max_blocks;
+    c.query_start_loc = query_start_loc; c.context_lens = context_lens; c.max_query_len = max_query_len;
+    c.n_seqs = n_seqs; c.H = H; c.kvh = kvh; c.num_blocks = num_blocks; c.block_size = block_size; c.window_left = window_left;
+    c.scale = scale; c.out = out; c.out_dtype = SBK_BF16; c.out_stride = out_tok_stride;
+    c.workspace = workspace; c.status = status;
+    return decode_q8::stream_cache("sbk_swa_prefill_q8", c, (cudaStream_t)stream);
+  }
   const Layout y = layout_of(n_seqs, max_query_len, max_blocks, kvh, block_size, window_left);
   const int64_t rows = y.rows_per_seq * y.group;
   const int bq = 128 / (H / kvh);
@@ -509,14 +537,6 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     return SBK_E_ARG;
   }
   const size_t half = (size_t)rows * kvh * D * 2;
-  if (!workspace || workspace_bytes < 2 * half) {
-    set_error("sbk_swa_prefill_q8: workspace of %zu bytes given, %zu needed", workspace ? workspace_bytes : 0, 2 * half);
-    return SBK_E_WORKSPACE;
-  }
-  if (!aligned16(workspace)) {
-    set_error("sbk_swa_prefill_q8: workspace must be 16-byte aligned");
-    return SBK_E_ALIGN;
-  }
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     if (!encode_rows_map(&maps[i], (uint8_t*)workspace + i * half, rows, kvh)) {
