@@ -8,6 +8,7 @@ to PyTorch ops: without a CUDA device and libsbk.so these functions raise.
 from typing import Optional, Sequence, Tuple
 
 import ctypes
+import functools
 
 import torch
 
@@ -669,6 +670,22 @@ def _q8_geometry(k_cache, v_cache, k_scale, v_scale) -> Tuple[int, int, int, int
     return nb, bs, kvh, d, cs, k_scale.stride(0)
 
 
+_I32, _I64 = torch.int32, torch.int64
+
+
+def _rows_i32(block_tables: torch.Tensor, B: int) -> int:
+    """Checks block_tables [B, max_blocks] -> max_blocks."""
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] != B or block_tables.dtype is not _I32 or not block_tables.is_contiguous():
+        raise ValueError(f"block_tables must be contiguous int32 [{B}, max_blocks]")
+    return shape[1]
+
+
+def _vec(t: torch.Tensor, dtype: torch.dtype, n: int, name: str) -> None:
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor with {n} entries")
+
+
 def _heads_contiguous(t: torch.Tensor) -> bool:
     """[n, heads, D] with the heads of a row one behind the other (strides of size-1 dimensions carry no meaning)."""
     return not t.shape[0] or (t.stride(2) == 1 and (t.shape[1] < 2 or t.stride(1) == t.shape[2]))
@@ -698,33 +715,34 @@ def _call_on(dev: int, name: str, *args) -> None:
 
 def _q8_append_args(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc,
                     retired_out):
+    """Checks -> (the C arguments from num_blocks to max_retired, T, kvh, D, bytes between tokens)."""
     nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
-    T = key.shape[0]
-    if key.shape != (T, kvh, d) or value.shape != key.shape:
+    shape = key.shape
+    T = shape[0]
+    if shape != (T, kvh, d) or value.shape != shape:
         raise ValueError(f"key/value must be [T, {kvh}, {d}], got {tuple(key.shape)} / {tuple(value.shape)}")
-    if key.dtype not in _DTYPE_CODE or value.dtype != key.dtype:
+    if key.dtype not in _DTYPE_CODE or value.dtype is not key.dtype:
         raise ValueError("key and value must share one dtype (bf16 or fp32)")
     if not (_heads_contiguous(key) and _heads_contiguous(value)):
         raise ValueError("key/value rows must be contiguous")
     if T > 1 and value.stride(0) != key.stride(0):
         raise ValueError("key and value must share one token stride")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T or not slot_mapping.is_contiguous():
-        raise ValueError("slot_mapping must be a contiguous int64 tensor with one entry per token")
-    B = max_blocks = max_ret = 0
-    if block_tables is not None:
-        if seq_lens is None:
-            raise ValueError("retirement needs seq_lens")
-        B, max_blocks = block_tables.shape
-        _i32(block_tables, "block_tables")
-        _i32(seq_lens, "seq_lens", B)
-        _i32(query_start_loc, "query_start_loc", B + 1)
-        if retired_out is not None:
-            if retired_out.dtype != torch.int32 or not retired_out.is_contiguous() or retired_out.shape[0] != B:
-                raise ValueError("retired_out must be contiguous int32 [B, max_retired]")
-            max_ret = retired_out.shape[1]
-    es = key.element_size()
-    tok_stride = (key.stride(0) if T > 1 else kvh * d) * es
-    return nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, es, tok_stride
+    _vec(slot_mapping, _I64, T, "slot_mapping")
+    tok_stride = (key.stride(0) if T > 1 else kvh * d) * key.element_size()
+    if block_tables is None:
+        return (nb, bs, cs, ss, None, 0, None, None, 0), (None, 0), T, kvh, d, tok_stride
+    if seq_lens is None:
+        raise ValueError("retirement needs seq_lens")
+    B = block_tables.shape[0]
+    max_blocks = _rows_i32(block_tables, B)
+    _vec(seq_lens, _I32, B, "seq_lens")
+    if query_start_loc is not None:
+        _vec(query_start_loc, _I32, B + 1, "query_start_loc")
+    max_ret = 0
+    if retired_out is not None:
+        max_ret = _rows_i32(retired_out, B)
+    return ((nb, bs, cs, ss, block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), _ptr(query_start_loc), B),
+            (_ptr(retired_out), max_ret), T, kvh, d, tok_stride)
 
 
 def kv_append_q8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -736,11 +754,11 @@ def kv_append_q8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, 
     they are written. A slot may be named once per call. The remaining arguments are those of kv_append."""
     dev = _one_device(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens,
                       query_start_loc, retired_out, status)
-    nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, _, tok_stride = _q8_append_args(
+    cache, retire, T, kvh, d, tok_stride = _q8_append_args(
         key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc, retired_out)
-    _call_on(dev, "sbk_kv_append_q8", _ptr(key), _ptr(value), _DTYPE_CODE[key.dtype], _ptr(k_cache), _ptr(v_cache),
-             _ptr(k_scale), _ptr(v_scale), _ptr(slot_mapping), T, kvh, d, tok_stride, nb, bs, cs, ss, _ptr(block_tables),
-             max_blocks, _ptr(seq_lens), _ptr(query_start_loc), B, window_left, _ptr(retired_out), max_ret, _ptr(status))
+    _call_on(dev, "sbk_kv_append_q8", key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], k_cache.data_ptr(),
+             v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slot_mapping.data_ptr(), T, kvh, d, tok_stride, *cache,
+             window_left, *retire, _ptr(status))
 
 
 def rope_kv_append_q8(query: Optional[torch.Tensor], key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -753,26 +771,25 @@ def rope_kv_append_q8(query: Optional[torch.Tensor], key: torch.Tensor, value: t
     fp32: K is quantised from the fp32 result; ``query`` (and ``key`` with ``key_in_place``) is rounded once to its dtype."""
     dev = _one_device(key, query, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, positions, cos_sin_cache,
                       block_tables, seq_lens, query_start_loc, retired_out, status)
-    nb, bs, kvh, d, cs, ss, T, B, max_blocks, max_ret, es, tok_stride = _q8_append_args(
+    cache, retire, T, kvh, d, tok_stride = _q8_append_args(
         key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, seq_lens, query_start_loc, retired_out)
-    if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype != key.dtype or not cos_sin_cache.is_contiguous():
+    dtype = key.dtype
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.dtype is not dtype or not cos_sin_cache.is_contiguous():
         raise ValueError("cos_sin_cache must be contiguous [max_position, rot_dim] in the dtype of key")
     max_pos, rot_dim = cos_sin_cache.shape
-    if positions.dtype != torch.int64 or positions.numel() != T or not positions.is_contiguous():
-        raise ValueError("positions must be a contiguous int64 tensor with one entry per token")
+    _vec(positions, _I64, T, "positions")
     H = q_stride = 0
     if query is not None:
-        if query.dim() != 3 or query.shape[0] != T or query.shape[2] != d or query.dtype != key.dtype:
-            raise ValueError(f"query must be [T, H, {d}] in the dtype of key")
         H = query.shape[1]
+        if query.shape != (T, H, d) or query.dtype is not dtype:
+            raise ValueError(f"query must be [T, H, {d}] in the dtype of key")
         if not _heads_contiguous(query):
             raise ValueError("query rows must be contiguous")
-        q_stride = (query.stride(0) if T > 1 else H * d) * es
-    _call_on(dev, "sbk_rope_kv_append_q8", _ptr(query), H, q_stride, _ptr(key), _ptr(value), int(key_in_place),
-             _DTYPE_CODE[key.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(slot_mapping),
-             _ptr(positions), _ptr(cos_sin_cache), rot_dim, max_pos, T, kvh, d, tok_stride, nb, bs, cs, ss,
-             _ptr(block_tables), max_blocks, _ptr(seq_lens), _ptr(query_start_loc), B, window_left, _ptr(retired_out),
-             max_ret, _ptr(status))
+        q_stride = (query.stride(0) if T > 1 else H * d) * query.element_size()
+    _call_on(dev, "sbk_rope_kv_append_q8", _ptr(query), H, q_stride, key.data_ptr(), value.data_ptr(), int(key_in_place),
+             _DTYPE_CODE[dtype], k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+             slot_mapping.data_ptr(), positions.data_ptr(), cos_sin_cache.data_ptr(), rot_dim, max_pos, T, kvh, d, tok_stride,
+             *cache, window_left, *retire, _ptr(status))
 
 
 def kv_gather_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -784,20 +801,26 @@ def kv_gather_q8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Te
     nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
     if dtype not in _DTYPE_CODE:
         raise ValueError("dtype must be bf16 or fp32")
-    B, max_blocks = block_tables.shape
-    _i32(block_tables, "block_tables")
-    _i32(seq_lens, "seq_lens", B)
-    k_out, v_out = torch.empty((2, B, kvh, n_out, d), dtype=dtype, device=k_cache.device).unbind()
-    _call_on(dev, "sbk_kv_gather_q8", _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(block_tables),
-             max_blocks, _ptr(seq_lens), B, kvh, d, nb, bs, cs, ss, window_left, _ptr(k_out), _ptr(v_out),
-             _DTYPE_CODE[dtype], n_out, _ptr(status))
+    B = block_tables.shape[0]
+    max_blocks = _rows_i32(block_tables, B)
+    _vec(seq_lens, _I32, B, "seq_lens")
+    k_out = k_cache.new_empty((B, kvh, n_out, d), dtype=dtype)
+    v_out = torch.empty_like(k_out)
+    _call_on(dev, "sbk_kv_gather_q8", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+             block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), B, kvh, d, nb, bs, cs, ss, window_left,
+             k_out.data_ptr(), v_out.data_ptr(), _DTYPE_CODE[dtype], n_out, _ptr(status))
     return k_out, v_out
+
+
+@functools.lru_cache(maxsize=None)
+def _decode_q8_workspace_bytes(B: int, H: int, D: int) -> int:
+    return _abi.lib.sbk_swa_decode_q8_workspace_bytes(B, H, D)
 
 
 def swa_decode_q8_workspace(B: int, H: int, D: int, device) -> Optional[torch.Tensor]:
     """Scratch for swa_decode_q8 (None when it needs none). Its contents need no initialisation and mean nothing between
     calls; calls that can overlap on the GPU (other streams) need one each."""
-    n = _abi.lib.sbk_swa_decode_q8_workspace_bytes(B, H, D)
+    n = _decode_q8_workspace_bytes(B, H, D)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -810,30 +833,40 @@ def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     log-sum-exp of the scaled scores. ``workspace`` (swa_decode_q8_workspace): kept by callers that must not allocate."""
     dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, out, lse, workspace, status)
     nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
-    if q.dim() != 3 or q.shape[2] != d or q.dtype != torch.bfloat16:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or q.dtype is not torch.bfloat16:
         raise ValueError(f"q must be bf16 [B, H, {d}]")
-    B, H, _ = q.shape
-    if not _heads_contiguous(q):
+    B, H, _ = shape
+    row = H * d
+    if q.is_contiguous():
+        q_stride = row
+    elif _heads_contiguous(q):
+        q_stride = q.stride(0) if B > 1 else row
+    else:
         raise ValueError("the heads of q must be contiguous")
-    if block_tables.dim() != 2 or block_tables.shape[0] != B:
-        raise ValueError("block_tables needs one row per query")
-    _i32(block_tables, "block_tables")
-    _i32(seq_lens, "seq_lens", B)
+    max_blocks = _rows_i32(block_tables, B)
+    _vec(seq_lens, _I32, B, "seq_lens")
+    out_stride = row
     if out is None:
-        out = torch.empty((B, H, d), dtype=out_dtype or torch.bfloat16, device=q.device)
-    elif out.shape != (B, H, d) or not _heads_contiguous(out):
+        out = q.new_empty(shape, dtype=out_dtype)
+    elif out.shape != shape or not _heads_contiguous(out):
         raise ValueError("out must be [B, H, D] with contiguous heads")
-    if out.dtype not in _DTYPE_CODE:
+    elif B > 1:
+        out_stride = out.stride(0)
+    code = _DTYPE_CODE.get(out.dtype)
+    if code is None:
         raise ValueError("out must be bf16 or fp32")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (B, H) or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous fp32 [B, H]")
     if workspace is None:
-        workspace = swa_decode_q8_workspace(B, H, d, q.device)
-    _call_on(dev, "sbk_swa_decode_q8", _ptr(q), q.stride(0) if B > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-             _ptr(v_scale), _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), B, H, kvh, d, nb, bs, cs, ss,
-             window_left, d ** -0.5 if scale is None else float(scale), _ptr(out), _DTYPE_CODE[out.dtype],
-             out.stride(0) if B > 1 else H * d, _ptr(lse), _ptr(workspace),
-             workspace.numel() * workspace.element_size() if workspace is not None else 0, _ptr(status))
+        n = _decode_q8_workspace_bytes(B, H, d)
+        workspace = q.new_empty((n,), dtype=torch.uint8)
+    else:
+        n = workspace.numel() * workspace.element_size()
+    _call_on(dev, "sbk_swa_decode_q8", q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+             v_scale.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), B, H, kvh, d, nb, bs, cs, ss,
+             window_left, d ** -0.5 if scale is None else float(scale), out.data_ptr(), code, out_stride, _ptr(lse),
+             workspace.data_ptr(), n, _ptr(status))
     return out
 
 
@@ -860,22 +893,20 @@ def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     T, H, _ = q.shape
     if not _heads_contiguous(q):
         raise ValueError("the heads of q must be contiguous")
-    if block_tables.dim() != 2:
-        raise ValueError("block_tables needs one row per sequence")
     n_seqs = block_tables.shape[0]
-    _i32(block_tables, "block_tables")
-    _i32(query_start_loc, "query_start_loc", n_seqs + 1)
-    _i32(context_lens, "context_lens", n_seqs)
+    max_blocks = _rows_i32(block_tables, n_seqs)
+    _vec(query_start_loc, _I32, n_seqs + 1, "query_start_loc")
+    _vec(context_lens, _I32, n_seqs, "context_lens")
     if out is None:
-        out = torch.empty((T, H, d), dtype=torch.bfloat16, device=q.device)
+        out = q.new_empty((T, H, d))
     elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not _heads_contiguous(out):
         raise ValueError("out must be bf16 [T, H, D] with contiguous heads")
     max_query_len = int(max_query_len)
     if workspace is None and n_seqs:
-        workspace = swa_prefill_q8_workspace(n_seqs, max_query_len, block_tables.shape[1], kvh, d, q.device, block_size=bs,
+        workspace = swa_prefill_q8_workspace(n_seqs, max_query_len, max_blocks, kvh, d, q.device, block_size=bs,
                                              window_left=window_left)
     _call_on(dev, "sbk_swa_prefill_q8", _ptr(q), q.stride(0) if T > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-             _ptr(v_scale), _ptr(block_tables), block_tables.shape[1], _ptr(query_start_loc), _ptr(context_lens), n_seqs,
+             _ptr(v_scale), _ptr(block_tables), max_blocks, _ptr(query_start_loc), _ptr(context_lens), n_seqs,
              max_query_len, H, kvh, d, nb, bs, cs, ss, window_left, d ** -0.5 if scale is None else float(scale),
              _ptr(out), out.stride(0) if T > 1 else H * d, _ptr(workspace),
              workspace.numel() * workspace.element_size() if workspace is not None else 0, _ptr(status))
