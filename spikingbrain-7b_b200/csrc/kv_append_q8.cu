@@ -1,9 +1,8 @@
 // Writing the 8-bit K/V cache and reading it back: the quantising append (with the rotary embedding folded in on request)
 // and the gather of a window as dense tensors. Formats and rounding: kv_q8.cuh.
 //
-// A row is the unit of work throughout: D values of one token and head, held by D / 8 neighbouring lanes, eight each, so
-// that its largest magnitude takes log2(D / 8) shuffles, its codes leave as one 8-byte store per lane (a 128-byte row
-// at D = 128), and no row knows of another.
+// A row is the unit of work throughout: D values of one token and head, held by neighbouring lanes, so that its largest
+// magnitude takes a few shuffles and no row knows of another.
 //   rotation (NeoX form, the halves of the first rot_dim values turn together), in fp32 with every product and sum
 //   rounded once to fp32 and no rounding to the input type before the quantisation:
 //     x'[i] = x[i] cos[i] - x[i+h] sin[i],   x'[i+h] = x[i+h] cos[i] + x[i] sin[i],   h = rot_dim / 2
@@ -50,94 +49,111 @@ struct AppendParams {
   const int64_t* slot_mapping; int64_t num_slots; int block_size;
   const int64_t* positions; const uint8_t* cos_sin; int64_t max_position; int rot_dim;
   int T, kvh;
-  int64_t n_rows;                                             // T * (2 kvh + H)
+  uint32_t n_rows;                                            // T * (2 kvh + H)
   int32_t* block_tables; int max_blocks; const int32_t* seq_lens; const int32_t* query_start_loc;
   int B, window_left; int32_t* retired_out; int max_retired; int32_t* status;
 };
 
 constexpr int kAppendThreads = 256;
 
-// LPR lanes per row (D = 8 LPR). Rows of a token: kvh of K, kvh of V, H of the query. CTAs past the last row retire blocks.
-template <typename T, int LPR, bool ROPE>
+// V = D / 8 vectors per row, V / 2 lanes, two vectors each: a rotated pair (j, j + half) lies in one lane, so the rotation needs
+// no exchange and its cosines are read once for both. Rows of a token: kvh of K, kvh of V, H of the query. CTAs past the
+// last row retire blocks.
+template <typename T, int V, bool ROPE>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_q8_kernel(const AppendParams p, int row_ctas) {
-  constexpr int D = 8 * LPR, kRows = kAppendThreads / LPR;
+  constexpr int D = 8 * V, LPR = V / 2, kRows = kAppendThreads / LPR, ES = (int)sizeof(T);
   if ((int)blockIdx.x >= row_ctas) {
     retire_rows(((int)blockIdx.x - row_ctas) * kAppendThreads + threadIdx.x, p.block_tables, p.max_blocks, p.seq_lens,
                 p.query_start_loc, p.B, p.window_left, p.block_size, p.retired_out, p.max_retired, p.status);
     return;
   }
   const int l = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LPR;
-  const int per_tok = 2 * p.kvh + (ROPE ? p.H : 0);
+  const uint32_t row = blockIdx.x * kRows + threadIdx.x / LPR, per_tok = 2 * p.kvh + (ROPE ? p.H : 0);
   const bool live = row < p.n_rows;
   const int t = live ? (int)(row / per_tok) : 0;
-  const int r = live ? (int)(row - (int64_t)t * per_tok) : 0;
-  const bool is_k = r < p.kvh, is_v = !is_k && r < 2 * p.kvh;
-  // where the row comes from and whether (and where) it goes into the cache
-  int64_t slot = live && (is_k || is_v) ? p.slot_mapping[t] : -1;
-  int64_t pos = 0;
+  const int r = live ? (int)(row - (uint32_t)t * per_tok) : 0;
+  const bool is_k = r < p.kvh, is_v = !is_k && r < 2 * p.kvh, is_q = ROPE && !is_k && !is_v;
+  const int head = is_k ? r : (is_v ? r - p.kvh : r - 2 * p.kvh);
+  uint8_t* src = is_k ? p.key : (is_v ? const_cast<uint8_t*>(p.value) : p.query);
+  src += (int64_t)t * (is_q ? p.q_token_stride : p.kv_token_stride) + (int64_t)head * D * ES;
+  // this lane's vectors: the halves of a rotated pair, or two neighbours beyond the rotated part
+  const int hv = ROPE ? p.rot_dim >> 4 : 0;
+  const bool inside = l < hv;
+  const int va = inside ? l : 2 * l, vb = inside ? l + hv : va + 1;
+  float a[8], b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+  if (live) {                                    // (on their way while the slot and the position are read)
+    Vec8<T>::load(src + 8 * va * ES, a);
+    Vec8<T>::load(src + 8 * vb * ES, b);
+  }
+  // whether (and where) the row goes into the cache
+  int64_t slot = live && !is_q ? p.slot_mapping[t] : -1;
   bool skip = !live;
+  int64_t pos = 0;
   if (ROPE && live) {
     pos = p.positions[t];
     if (pos < 0 || pos >= p.max_position) {      // nothing of this token is written
       if (r == 0 && l == 0) raise_status(p.status, SBK_ST_BAD_POSITION);
       skip = true;
-      pos = 0;
     }
   }
   if (!skip && slot >= p.num_slots) {
     if (r == 0 && l == 0) raise_status(p.status, SBK_ST_BAD_SLOT);
     slot = -1;
   }
-  const int head = is_k ? r : (is_v ? r - p.kvh : r - 2 * p.kvh);
-  uint8_t* src = is_k ? p.key : (is_v ? const_cast<uint8_t*>(p.value) : p.query);
-  src += (int64_t)t * (is_k || is_v ? p.kv_token_stride : p.q_token_stride) + ((int64_t)head * D + 8 * l) * (int)sizeof(T);
   const bool turn = ROPE && !is_v;
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
-  if (!skip && (turn || slot >= 0)) Vec8<T>::load(src, x);
-  if (ROPE) {
-    const int hl = p.rot_dim >> 4;               // lanes of half the rotated values
-    const bool first = l < hl, inside = l < 2 * hl;
-    float c[8], s[8];
-    if (!skip && turn && inside) {
-      const uint8_t* tab = p.cos_sin + (pos * p.rot_dim + 8 * (first ? l : l - hl)) * (int)sizeof(T);
+  const bool work = !skip && (turn || slot >= 0);
+  if (work && turn) {
+    if (inside) {
+      float c[8], s[8];
+      const uint8_t* tab = p.cos_sin + (pos * p.rot_dim + 8 * l) * ES;
       Vec8<T>::load(tab, c);
-      Vec8<T>::load(tab + (p.rot_dim >> 1) * (int)sizeof(T), s);
-    } else {
+      Vec8<T>::load(tab + (p.rot_dim >> 1) * ES, s);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { c[i] = 1.f; s[i] = 0.f; }
-    }
-    const int other = (threadIdx.x & 31) + (first ? hl : (inside ? -hl : 0));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __shfl_sync(0xffffffffu, x[i], other);
-      if (turn && inside) {
-        const float a = __fmul_rn(x[i], c[i]), b = __fmul_rn(y, s[i]);
-        x[i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
+      for (int i = 0; i < 8; ++i) {
+        const float x = a[i], y = b[i];
+        a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+        b[i] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
       }
     }
-    if (!skip && turn && (!is_k || p.key_in_place)) Vec8<T>::store(src, x);
+    if (is_q || p.key_in_place) {
+      Vec8<T>::store(src + 8 * va * ES, a);
+      Vec8<T>::store(src + 8 * vb * ES, b);
+    }
   }
+  if (__all_sync(0xffffffffu, slot < 0 || skip)) return;       // a warp of query rows ends here
   // ---- the row's exponent: largest finite magnitude over its lanes ----
   float top = 0.f;
+  bool odd = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite(x[i]) ? fabsf(x[i]) : 0.f);
+  for (int i = 0; i < 8; ++i) {
+    odd |= !finite(a[i]) || !finite(b[i]);
+    top = fmaxf(top, fmaxf(finite(a[i]) ? fabsf(a[i]) : 0.f, finite(b[i]) ? fabsf(b[i]) : 0.f));
+  }
 #pragma unroll
   for (int off = 1; off < LPR; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   if (skip || slot < 0) return;
   const int e = row_exponent(top);
   const float inv = pow2i(-e);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = finite(x[i]) ? x[i] * inv : __uint_as_float(0x7fffffffu);
-  uint2 codes;
-  codes.x = pack_e4m3x2(x[0], x[1]) | (pack_e4m3x2(x[2], x[3]) << 16);
-  codes.y = pack_e4m3x2(x[4], x[5]) | (pack_e4m3x2(x[6], x[7]) << 16);
-  const int64_t blk = slot / p.block_size;
+  for (int i = 0; i < 8; ++i) { a[i] *= inv; b[i] *= inv; }
+  if (odd) {                                                    // infinities become NaN like NaN itself
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a[i] = finite(a[i]) ? a[i] : __uint_as_float(0x7fffffffu);
+      b[i] = finite(b[i]) ? b[i] : __uint_as_float(0x7fffffffu);
+    }
+  }
+  auto codes = [](const float (&x)[8]) {
+    return make_uint2(pack_e4m3x2(x[0], x[1]) | (pack_e4m3x2(x[2], x[3]) << 16),
+                      pack_e4m3x2(x[4], x[5]) | (pack_e4m3x2(x[6], x[7]) << 16));
+  };
+  const int64_t blk = slot <= 0x7fffffff ? (int64_t)((uint32_t)slot / (uint32_t)p.block_size) : slot / p.block_size;
   const int off = (int)(slot - blk * p.block_size);
-  uint8_t* dst = (is_k ? p.k_cache : p.v_cache) + blk * p.cache_block_stride + ((int64_t)off * p.kvh + head) * D + 8 * l;
-  *reinterpret_cast<uint2*>(dst) = codes;
+  uint8_t* dst = (is_k ? p.k_cache : p.v_cache) + blk * p.cache_block_stride + ((int64_t)off * p.kvh + head) * D;
+  *reinterpret_cast<uint2*>(dst + 8 * va) = codes(a);
+  *reinterpret_cast<uint2*>(dst + 8 * vb) = codes(b);
   if (l == 0) ((is_k ? p.k_scale : p.v_scale) + blk * p.scale_block_stride)[(int64_t)head * p.block_size + off] = (uint8_t)(e + 127);
 }
 
@@ -266,20 +282,21 @@ static int append(const char* who, AppendParams& p, int dtype, int D, int64_t nu
     set_error("%s: retirement needs seq_lens, max_blocks > 0 and max_retired > 0", who);
     return SBK_E_ARG;
   }
-  p.n_rows = (int64_t)p.T * (2 * p.kvh + (rope ? p.H : 0));
-  const int per_cta = kAppendThreads / (D / 8 > 0 ? D / 8 : 1);
-  const int64_t row_ctas = p.T > 0 ? (p.n_rows + per_cta - 1) / per_cta : 0;
-  const int64_t grid = row_ctas + (retire ? (p.B + kAppendThreads - 1) / kAppendThreads : 0);
-  if (grid > 2147483647LL) {
-    set_error("%s: grid too large", who);
+  const int64_t n_rows = p.T > 0 ? (int64_t)p.T * (2 * p.kvh + (rope ? p.H : 0)) : 0;
+  if (n_rows > 2147483647LL) {
+    set_error("%s: %lld rows in one call, at most 2^31 - 1", who, (long long)n_rows);
     return SBK_E_ARG;
   }
+  p.n_rows = (uint32_t)n_rows;
+  const int per_cta = p.T > 0 ? kAppendThreads / (D / 16) : 1;
+  const int64_t row_ctas = (n_rows + per_cta - 1) / per_cta;
+  const int64_t grid = row_ctas + (retire ? (p.B + kAppendThreads - 1) / kAppendThreads : 0);
   if (!retire) p.block_tables = nullptr;
   if (grid == 0) return SBK_OK;
-#define SBK_LAUNCH_APPEND(TT, LPR)                                                                             \
+#define SBK_LAUNCH_APPEND(TT, V)                                                                               \
   do {                                                                                                         \
-    if (rope) kv_append_q8_kernel<TT, LPR, true><<<(unsigned)grid, kAppendThreads, 0, st>>>(p, (int)row_ctas);  \
-    else kv_append_q8_kernel<TT, LPR, false><<<(unsigned)grid, kAppendThreads, 0, st>>>(p, (int)row_ctas);      \
+    if (rope) kv_append_q8_kernel<TT, V, true><<<(unsigned)grid, kAppendThreads, 0, st>>>(p, (int)row_ctas);  \
+    else kv_append_q8_kernel<TT, V, false><<<(unsigned)grid, kAppendThreads, 0, st>>>(p, (int)row_ctas);      \
   } while (0)
 #define SBK_APPEND_D(TT)                              \
   switch (D) {                                        \
