@@ -18,8 +18,11 @@ What runs where
                          softmax (reference: second flash-attn pass + LSE merge,
                          fa_kernel_metatoken.py:124-194); the meta tokens' own queries (query2) run
                          non-causally over key2/value2 through sbk_swa_prefill_dense (:262-280)
-  fp8 KV, ALiBi, soft-cap, encoder and cross attention, head sizes the kernels are not built for
-                      -> NotImplementedError, never a fallback.
+  8-bit cache (kv_cache_dtype "fp8_e4m3", an exponent byte per token and head in `kv_scales`)
+                      -> sbk_kv_append_q8 / sbk_rope_kv_append_q8, sbk_swa_decode_q8, sbk_swa_prefill_q8; a prompt run
+                         without block tables attends over key/value as passed. No meta tokens.
+  other fp8 forms (one scale per tensor), ALiBi, soft-cap, encoder and cross attention, head sizes the kernels are not
+  built for             -> NotImplementedError, never a fallback.
 """
 from collections import defaultdict
 from dataclasses import dataclass
@@ -126,6 +129,15 @@ class MetaAttentionBackend:
         return (2, num_blocks, block_size, num_kv_heads, head_size)
 
     @staticmethod
+    def get_kv_scale_shape(num_blocks: int, block_size: int, num_kv_heads: int) -> Tuple[int, ...]:
+        """Exponent bytes (uint8) that go with an 8-bit cache (kv_cache_dtype "fp8_e4m3"), which itself has the shape of
+        get_kv_cache_shape in float8_e4m3fn or uint8. swap_blocks and copy_blocks move them like a cache."""
+        if block_size % 16 != 0 or block_size < 16:
+            raise ValueError(
+                f"Invalid block size {block_size}. Must be a multiple of 16 and at least 16.")
+        return (2, num_blocks, num_kv_heads, block_size)
+
+    @staticmethod
     def swap_blocks(src_kv_cache: torch.Tensor, dst_kv_cache: torch.Tensor,
                     scr_to_dst: torch.Tensor) -> None:
         """Copy whole blocks between two caches (preemption); `scr_to_dst` is [n, 2] int64."""
@@ -139,6 +151,8 @@ class MetaAttentionBackend:
         src = src_to_dists[:, 0].long()
         dst = src_to_dists[:, 1].long()
         for kv in kv_caches:
+            if kv.element_size() == 1:
+                kv = kv.view(torch.uint8)
             kv[:, dst.to(kv.device)] = kv[:, src.to(kv.device)]
 
 
@@ -408,10 +422,10 @@ class MetaAttentionImpl:
             raise NotImplementedError("ALiBi is not part of the sliding-window decode kernel")
         if logits_soft_cap:
             raise NotImplementedError("logits soft-capping is not part of the sliding-window decode kernel")
-        if kv_cache_dtype != "auto":
+        if kv_cache_dtype not in ("auto", "fp8_e4m3"):
             raise NotImplementedError(
                 f"MetaAttention does not support {kv_cache_dtype} kv-cache on this device "
-                "(the paged cache holds bf16)")
+                "(the paged cache holds bf16, or e4m3 codes with an exponent per token and head: \"fp8_e4m3\")")
         if attn_type != AttentionType.DECODER:
             raise NotImplementedError("only decoder self-attention is implemented")
         self.num_heads = num_heads
@@ -456,9 +470,14 @@ class MetaAttentionImpl:
                 value2: Optional[torch.Tensor], kv_cache: torch.Tensor,
                 attn_metadata: MetaAttentionMetadata, output: Optional[torch.Tensor] = None,
                 output_scale: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
-                cos_sin_cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+                cos_sin_cache: Optional[torch.Tensor] = None,
+                kv_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
         """query [T, H, D]; key, value [T, KVH, D]; kv_cache [2, NB, BS, KVH, D] (numel 0 on the
         memory-profiling run); writes into `output` ([T, H, D] or [T, H*D]) and returns it.
+
+        With kv_cache_dtype "fp8_e4m3" the cache holds float8_e4m3fn (or uint8) codes and ``kv_scales``
+        [2, NB, KVH, BS] uint8 (MetaAttentionBackend.get_kv_scale_shape) their exponents; the engine allocates both
+        and moves them together.
 
         With ``positions`` [T] int64 and ``cos_sin_cache`` (ops.build_cos_sin_cache) the rotary
         embedding the reference applies just before this call
@@ -473,6 +492,14 @@ class MetaAttentionImpl:
                 "key/v_scale is only supported with an fp8 cache, which this path does not have")
         if (key2 is None) != (value2 is None):
             raise ValueError("key2 and value2 come together")
+        q8 = self.kv_cache_dtype == "fp8_e4m3"
+        if q8 and (key2 is not None or query2 is not None):
+            raise NotImplementedError("meta tokens with an 8-bit cache are not supported")
+        if q8 and kv_cache.numel() > 0 and kv_scales is None:
+            raise ValueError("an 8-bit cache needs kv_scales")
+        if not q8 and kv_scales is not None:
+            raise ValueError("kv_scales go with kv_cache_dtype \"fp8_e4m3\"")
+        cache = (kv_cache[0], kv_cache[1], kv_scales[0], kv_scales[1]) if q8 and kv_cache.numel() > 0 else None
         if key2 is not None:
             assert self.num_meta_tokens == key2.shape[0], "num_meta_tokens differs from key2"
             key2 = key2.view(-1, self.num_kv_heads, self.head_size).contiguous()
@@ -507,7 +534,14 @@ class MetaAttentionImpl:
         if (positions is None) != (cos_sin_cache is None):
             raise ValueError("positions and cos_sin_cache come together")
         if kv_cache.numel() > 0 and key is not None and value is not None:
-            if positions is not None:
+            if q8 and positions is not None:
+                ops.rope_kv_append_q8(query, key.view(-1, self.num_kv_heads, D), value.view(-1, self.num_kv_heads, D), *cache,
+                                      attn_metadata.slot_mapping.flatten(), positions.flatten(), cos_sin_cache,
+                                      key_in_place=True, status=self._status)
+            elif q8:
+                ops.kv_append_q8(key.view(-1, self.num_kv_heads, D), value.view(-1, self.num_kv_heads, D), *cache,
+                                 attn_metadata.slot_mapping.flatten(), status=self._status)
+            elif positions is not None:
                 ops.rope_kv_append(query, key.view(-1, self.num_kv_heads, D),
                                    value.view(-1, self.num_kv_heads, D), kv_cache[0], kv_cache[1],
                                    attn_metadata.slot_mapping.flatten(), positions.flatten(),
@@ -551,11 +585,10 @@ class MetaAttentionImpl:
         if prefill_meta:
             # windowed attention of the prompt tokens over the paged cache (their own K/V included:
             # the append above has run), 16 queries and one kv group per CTA
-            ops.swa_prefill(pq, kv_cache[0], kv_cache[1], prefill_meta.block_tables.contiguous(),
-                            prefill_meta.query_start_loc.to(torch.int32).contiguous(),
-                            prefill_meta.context_lens_tensor.to(torch.int32).contiguous(),
-                            prefill_meta.max_query_len, window_left=window_left, scale=self.scale, out=tmp,
-                            key2=key2, value2=value2, status=self._status)
+            self._runs(pq, kv_cache, cache, prefill_meta.block_tables.contiguous(),
+                       prefill_meta.query_start_loc.to(torch.int32).contiguous(),
+                       prefill_meta.context_lens_tensor.to(torch.int32).contiguous(),
+                       prefill_meta.max_query_len, window_left, tmp, key2, value2)
             if tmp is not po:
                 po.copy_(tmp)
 
@@ -571,19 +604,45 @@ class MetaAttentionImpl:
                 dtmp = do if do.stride()[1:] == (D, 1) else torch.empty_like(do, memory_format=torch.contiguous_format)
                 dqsl = decode_meta.query_start_loc.to(torch.int32).contiguous()
                 ctx = (decode_meta.seq_lens_tensor.to(torch.int32) - (dqsl[1:] - dqsl[:-1])).contiguous()
-                ops.swa_prefill(dq, kv_cache[0], kv_cache[1], decode_meta.block_tables.contiguous(), dqsl, ctx,
-                                decode_meta.max_decode_query_len, window_left=window_left, scale=self.scale,
-                                out=dtmp, key2=key2, value2=value2, status=self._status)
+                self._runs(dq, kv_cache, cache, decode_meta.block_tables.contiguous(), dqsl, ctx,
+                           decode_meta.max_decode_query_len, window_left, dtmp, key2, value2)
                 if dtmp is not do:
                     do.copy_(dtmp)
                 return output
             self._decode(decode_query, kv_cache, decode_meta.block_tables, decode_meta.seq_lens_tensor,
-                         window_left, out3[num_prefill_tokens:], key2, value2)
+                         window_left, out3[num_prefill_tokens:], key2, value2, cache)
         return output
 
-    def _decode(self, q, kv_cache, block_tables, seq_lens, window_left, out, key2=None, value2=None) -> None:
+    def _runs(self, q, kv_cache, cache8, block_tables, query_start_loc, context_lens, max_query_len, window_left, out,
+              key2, value2) -> None:
+        """Runs of query tokens over the paged cache, bf16 or (cache8) 8-bit."""
+        if cache8 is not None:
+            if q.data_ptr() % 16 or (q.shape[0] > 1 and q.stride(0) % 8):
+                q = q.clone(memory_format=torch.contiguous_format)
+            dst = out if out.data_ptr() % 16 == 0 and (out.shape[0] < 2 or out.stride(0) % 8 == 0) else torch.empty(
+                out.shape, dtype=out.dtype, device=out.device)
+            ops.swa_prefill_q8(q, *cache8, block_tables, query_start_loc, context_lens, max_query_len,
+                               window_left=window_left, scale=self.scale, out=dst, status=self._status)
+            if dst is not out:
+                out.copy_(dst)
+            return
+        ops.swa_prefill(q, kv_cache[0], kv_cache[1], block_tables, query_start_loc, context_lens, max_query_len,
+                        window_left=window_left, scale=self.scale, out=out, key2=key2, value2=value2, status=self._status)
+
+    def _decode(self, q, kv_cache, block_tables, seq_lens, window_left, out, key2=None, value2=None, cache8=None) -> None:
         B = q.shape[0]
         if B == 0:
+            return
+        if cache8 is not None:
+            D = self.head_size
+            if q.stride()[1:] != (D, 1):
+                q = q.contiguous()
+            tmp = out if out.stride()[1:] == (D, 1) else torch.empty_like(out, memory_format=torch.contiguous_format)
+            # (the workspace holds nothing between calls: the allocator hands it out, from a graph's own pool under capture)
+            ops.swa_decode_q8(q, *cache8, block_tables.contiguous(), seq_lens.contiguous(), window_left=window_left,
+                              scale=self.scale, out=tmp, status=self._status)
+            if tmp is not out:
+                out.copy_(tmp)
             return
         bs = kv_cache.shape[2]
         width = block_tables.shape[1] * bs

@@ -20,6 +20,10 @@ Behaviour at the edges of the reference class (hf_7B_model/cache.py:96-107):
     NotImplementedError: the reference silently stops trimming from then on and grows
     without bound, which no caller wants from a paged pool.
 Tensors must live on a CUDA device: there is no CPU path.
+
+``Cache(kv_dtype="fp8_e4m3")`` holds the window in 8 bits (e4m3 codes, an exponent per token and head): half the memory,
+and decode reads half the bytes. `attn_state` then returns the values the codes stand for, in the dtype of the K/V given;
+head sizes 64, 128 and 256 (swa_decode: 128).
 """
 from typing import Any, Dict, List, Optional, Tuple
 
@@ -36,7 +40,8 @@ class _PagedWindow:
     one planner launch and one append launch, with nothing copied from the host."""
 
     def __init__(self, B: int, kvh: int, D: int, dtype: torch.dtype, device, window: Optional[int],
-                 block_size: int, capacity_tokens: int):
+                 block_size: int, capacity_tokens: int, q8: bool = False):
+        self.q8 = q8       # codes in `kv`, their exponents in `scales`
         self.B, self.kvh, self.D, self.dtype, self.device = B, kvh, D, dtype, device
         self.window = window
         self.bs = block_size
@@ -54,7 +59,10 @@ class _PagedWindow:
         nb = self.B * per_row
         self.plan = DeviceStepPlanner(nb, self.bs, -1 if self.window is None else self.window - 1,
                                       self.B, self.max_blocks, self.device, max_tokens=self.B)
-        self.kv = torch.zeros(2, nb, self.bs, self.kvh, self.D, dtype=self.dtype, device=self.device)
+        if self.q8:
+            self.kv, self.scales = ops.kv_cache_q8(nb, self.bs, self.kvh, self.D, device=self.device)
+        else:
+            self.kv = torch.zeros(2, nb, self.bs, self.kvh, self.D, dtype=self.dtype, device=self.device)
         self.table_d, self.lens_d, self.status = self.plan.block_tables, self.plan.seq_lens, self.plan.status
         self._n_new = torch.zeros(self.B, dtype=torch.int32, device=self.device)
         self.L = 0
@@ -127,7 +135,10 @@ class _PagedWindow:
         tm = lambda t: t.transpose(1, 2).reshape(self.B * t.shape[-2], t.shape[1], self.D).contiguous()
         kt, vt = tm(k), tm(v)
         if rope is None:
-            ops.kv_append(kt, vt, self.kv[0], self.kv[1], slots, status=self.status)
+            if self.q8:
+                ops.kv_append_q8(kt, vt, *self._cache8(), slots, status=self.status)
+            else:
+                ops.kv_append(kt, vt, self.kv[0], self.kv[1], slots, status=self.status)
             return None
         q, position_ids, table = rope
         if n_in != n:  # prompt longer than the window: every token is rotated, the last W are cached
@@ -135,12 +146,20 @@ class _PagedWindow:
             full[:, n_in - n:] = slots.view(self.B, n)
             slots = full.view(-1)
         qt = tm(q) if q is not None else None
-        ops.rope_kv_append(qt, kt, vt, self.kv[0], self.kv[1], slots,
-                           position_ids.to(torch.int64).expand(self.B, n_in).reshape(-1).contiguous(), table,
-                           status=self.status)
+        pos = position_ids.to(torch.int64).expand(self.B, n_in).reshape(-1).contiguous()
+        if self.q8:
+            ops.rope_kv_append_q8(qt, kt, vt, *self._cache8(), slots, pos, table, status=self.status)
+        else:
+            ops.rope_kv_append(qt, kt, vt, self.kv[0], self.kv[1], slots, pos, table, status=self.status)
         return None if qt is None else qt.view(self.B, n_in, q.shape[1], self.D).transpose(1, 2)
 
+    def _cache8(self):
+        return self.kv[0], self.kv[1], self.scales[0], self.scales[1]
+
     def gather(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        if self.q8:
+            return ops.kv_gather_q8(*self._cache8(), self.table_d, self.lens_d, self.n_cached,
+                                    window_left=self.n_cached - 1, dtype=self.dtype, status=self.status)
         return ops.kv_gather(self.kv[0], self.kv[1], self.table_d, self.lens_d, self.n_cached,
                              window_left=self.n_cached - 1, status=self.status)
 
@@ -148,6 +167,11 @@ class _PagedWindow:
         # one zero-initialised workspace per head count, sized for the fixed batch and the widest
         # window the table can hold: no allocation and no memset per step
         H = q.shape[1]
+        if self.q8:
+            if H not in self._scratch:
+                self._scratch[H] = ops.swa_decode_q8_workspace(self.B, H, self.D, self.device)
+            return ops.swa_decode_q8(q, *self._cache8(), self.table_d, self.lens_d, window_left=self.n_cached - 1, scale=scale,
+                                     out=out, workspace=self._scratch[H], status=self.status)
         if H not in self._scratch:
             vis = self.max_blocks * self.bs if self.window is None else min(self.max_blocks * self.bs, self.window)
             split = ops.swa_auto_split(self.B, vis, self.device)
@@ -183,12 +207,16 @@ class _LayerState(dict):
 class Cache(transformers.cache_utils.Cache):
     """Drop-in for hf_7B_model/cache.py:11 `Cache` (same public surface and values)."""
 
-    def __init__(self, seen_tokens: int = 0, *, block_size: int = 16, unbounded_capacity: int = 4096):
+    def __init__(self, seen_tokens: int = 0, *, block_size: int = 16, unbounded_capacity: int = 4096,
+                 kv_dtype: Optional[str] = None):
+        if kv_dtype not in (None, "auto", "fp8_e4m3"):
+            raise NotImplementedError(f"kv_dtype {kv_dtype}: the window is held in the dtype given, or as \"fp8_e4m3\"")
         # like the reference, the transformers base initialiser is not chained
         self.states: List[_LayerState] = []
         self._seen_tokens = seen_tokens
         self._block_size = block_size
         self._unbounded_capacity = unbounded_capacity
+        self._q8 = kv_dtype == "fp8_e4m3"
 
     def __getitem__(self, layer_idx: int) -> Dict[str, Any]:
         if layer_idx < len(self):
@@ -208,7 +236,7 @@ class Cache(transformers.cache_utils.Cache):
             raise RuntimeError("this Cache keeps K/V in paged CUDA memory; CPU tensors are not supported")
         B, kvh, n, D = k.shape
         cap = 3 * window + 2 * self._block_size if window is not None else max(self._unbounded_capacity, 2 * n)
-        return _PagedWindow(B, kvh, D, k.dtype, k.device, window, self._block_size, cap)
+        return _PagedWindow(B, kvh, D, k.dtype, k.device, window, self._block_size, cap, self._q8)
 
     def update(self, recurrent_state: torch.Tensor = None,
                attn_state: Tuple[torch.Tensor, torch.Tensor] = None,
@@ -261,8 +289,8 @@ class Cache(transformers.cache_utils.Cache):
 
     @classmethod
     def from_legacy_cache(cls, past_key_values: Optional[Tuple[Dict[str, Any], ...]] = None,
-                          seen_tokens: int = 0) -> "Cache":
-        cache = cls(seen_tokens)
+                          seen_tokens: int = 0, *, kv_dtype: Optional[str] = None) -> "Cache":
+        cache = cls(seen_tokens, kv_dtype=kv_dtype)
         if past_key_values is not None:
             for d in past_key_values:
                 cache.states.append(_LayerState(recurrent_state=d.get("recurrent_state"),

@@ -634,3 +634,162 @@ def test_a_sequence_written_in_pieces_equals_the_whole_and_decodes_like_its_valu
     plain = torch.softmax(torch.einsum("bhgd,bhnd->bhgn", q[:, n - 1].double().view(B, kvh, 7, D), kd.double()) * D ** -0.5, -1)
     assert ((torch.einsum("bhgn,bhnd->bhgd", plain, vd.double()).reshape(B, H, D) - want).abs() <= err + 1e-12).all()
     assert st.item() == 0
+
+
+# ------------------------------------------------------------------------------------- the framework's surfaces
+def _impl(dtype="fp8_e4m3", window=64, H=28, kvh=4):
+    from spikingbrain_7b_b200.backend import MetaAttentionImpl
+    return MetaAttentionImpl(H, 128, 128 ** -0.5, kvh, None, window, dtype)
+
+
+def _meta(ctx, new, n_prefill, table, slots, dev):
+    from spikingbrain_7b_b200.backend import MetaAttentionMetadata
+    lens = [a + b for a, b in zip(ctx, new)]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    start = [sum(new[:i]) for i in range(len(new) + 1)]
+    return MetaAttentionMetadata(
+        num_prefills=n_prefill, num_prefill_tokens=sum(new[:n_prefill]), num_decode_tokens=sum(new[n_prefill:]),
+        slot_mapping=slots, seq_lens=lens, seq_lens_tensor=i32(lens), max_prefill_seq_len=max(lens[:n_prefill], default=0),
+        max_decode_seq_len=max(lens[n_prefill:], default=0), context_lens_tensor=i32(ctx), block_tables=table,
+        use_cuda_graph=False, max_query_len=max(new), max_decode_query_len=max(new[n_prefill:], default=1),
+        query_start_loc=i32(start), seq_start_loc=i32([sum(lens[:i]) for i in range(len(lens) + 1)]))
+
+
+def test_backend_takes_the_8_bit_cache_and_refuses_what_it_does_not_have(sb):
+    from spikingbrain_7b_b200.backend import MetaAttentionBackend, MetaAttentionImpl
+    assert MetaAttentionBackend.get_kv_scale_shape(7, 32, 4) == (2, 7, 4, 32)
+    with pytest.raises(ValueError):
+        MetaAttentionBackend.get_kv_scale_shape(7, 24, 4)
+    for other in ("fp8", "fp8_e5m2", "int8"):
+        with pytest.raises(NotImplementedError):
+            MetaAttentionImpl(28, 128, 1.0, 4, None, 4097, other)
+    impl = _impl()
+    q, k = torch.zeros(1, 28, 128).bfloat16(), torch.zeros(1, 4, 128).bfloat16()
+    md = _meta([3], [1], 0, torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int64), "cpu")
+    kv, sc = torch.zeros(2, 4, 16, 4, 128, dtype=torch.uint8), torch.zeros(2, 4, 4, 16, dtype=torch.uint8)
+    with pytest.raises(ValueError):                                          # codes without exponents
+        impl.forward(None, q, k, k, None, None, None, kv, md, output=torch.empty_like(q))
+    with pytest.raises(NotImplementedError):                                 # meta tokens
+        MetaAttentionImpl(28, 128, 1.0, 4, None, 64, "fp8_e4m3", num_meta_tokens=1).forward(
+            None, q, k, k, None, k, k, kv, md, output=torch.empty_like(q), kv_scales=sc)
+    with pytest.raises(ValueError):                                          # exponents without codes
+        _impl("auto").forward(None, q, k, k, None, None, None, torch.zeros(2, 4, 16, 4, 128).bfloat16(), md,
+                              output=torch.empty_like(q), kv_scales=sc)
+    from spikingbrain_7b_b200.hf_cache import Cache
+    with pytest.raises(NotImplementedError):
+        Cache(kv_dtype="int8")
+
+
+@gpu
+@pytest.mark.parametrize("rotary", [False, True])
+def test_backend_forward_over_the_8_bit_cache(ops, rotary):
+    """Two prompt chunks and two decoding sequences in one call, then a call whose sequences verify several tokens each:
+    K/V are written in 8 bits and every output is the attention over the values the cache holds."""
+    H, kvh, D, bs, W = 28, 4, 128, 16, 65
+    ctx, new = [30, 0, 90, 7], [50, 20, 1, 1]
+    impl = _impl(window=W)
+    rows, nb = len(ctx), 60
+    table = torch.randperm(nb, generator=torch.Generator().manual_seed(80))[:rows * 12].to(torch.int32).view(rows, 12).to(DEV)
+    kv, sc = ops.kv_cache_q8(nb, bs, kvh, D, device=DEV)
+    cos_sin = ops.build_cos_sin_cache(D, 256, device=DEV)
+
+    def slots_of(ctx, new):
+        return torch.cat([table[s].long()[torch.arange(c, c + n, device=DEV) // bs] * bs
+                          + torch.arange(c, c + n, device=DEV) % bs for s, (c, n) in enumerate(zip(ctx, new))])
+    k0, v0 = (_rows((sum(ctx), kvh, D), 81 + i).bfloat16().to(DEV) for i in range(2))
+    ops.kv_append_q8(k0, v0, kv[0], kv[1], sc[0], sc[1], slots_of([0] * rows, ctx))
+    for step, (ctx, new, n_prefill) in enumerate([(ctx, new, 2), ([80, 20, 91, 8], [3, 1, 4, 2], 0)]):
+        T = sum(new)
+        q, k, v = (_rows((T, h, D), 83 + 10 * step + i).bfloat16().to(DEV) for i, h in enumerate((H, kvh, kvh)))
+        slots = slots_of(ctx, new)
+        kw = {}
+        want_kv, want_sc = kv.view(torch.uint8).clone(), sc.clone()
+        qr, kr = q.clone(), k.clone()
+        if rotary:
+            pos = torch.cat([torch.arange(c, c + n, device=DEV) for c, n in zip(ctx, new)])
+            kw = {"positions": pos, "cos_sin_cache": cos_sin}
+            ops.rope_kv_append_q8(qr, kr, v, want_kv[0], want_kv[1], want_sc[0], want_sc[1], slots, pos, cos_sin, key_in_place=True)
+        else:
+            ops.kv_append_q8(kr, v, want_kv[0], want_kv[1], want_sc[0], want_sc[1], slots)
+        out = torch.empty(T, H * D, dtype=torch.bfloat16, device=DEV)
+        impl.forward(None, q, k, v, None, None, None, kv, _meta(ctx, new, n_prefill, table, slots, DEV), output=out, kv_scales=sc, **kw)
+        assert impl.status() == 0
+        assert torch.equal(kv.view(torch.uint8), want_kv) and torch.equal(sc, want_sc)
+        assert torch.equal(q, qr) and torch.equal(k, kr)
+        _check(out.view(T, H, D), None, ref.runs(qr, kv, sc, table, ctx, new, W - 1, D ** -0.5))
+
+
+@gpu
+def test_backend_block_moves_take_codes_and_exponents(ops):
+    from spikingbrain_7b_b200.backend import MetaAttentionBackend
+    codes, scales, table = _pool([100], -1, 2, 128, 16, seed=90)
+    kv, sc = codes.to(DEV), scales.to(DEV)
+    want = (kv.view(torch.uint8).clone(), sc.clone())
+    pairs = torch.tensor([[int(table[0, 0]), 8], [int(table[0, 1]), 9]])
+    MetaAttentionBackend.copy_blocks([kv, sc], pairs)
+    other = (torch.zeros_like(kv.view(torch.uint8)).view(kv.dtype), torch.zeros_like(sc))
+    for a, b in zip((kv, sc), other):
+        MetaAttentionBackend.swap_blocks(a, b, pairs)
+    for src, dst in pairs.tolist():
+        assert torch.equal(kv.view(torch.uint8)[:, dst], want[0][:, src]) and torch.equal(sc[:, dst], want[1][:, src])
+        assert torch.equal(other[0].view(torch.uint8)[:, dst], want[0][:, src]) and torch.equal(other[1][:, dst], want[1][:, src])
+
+
+@gpu
+@pytest.mark.parametrize("window,dtype,D", [(24, torch.bfloat16, 128), (24, torch.float32, 64), (None, torch.bfloat16, 128)])
+def test_hf_cache_in_8_bits_holds_the_quantised_window(ops, window, dtype, D):
+    """The stream of the reference class with every token replaced by what the 8-bit format makes of it, also across the
+    growth of an unbounded layer; decode against attention over exactly those values."""
+    from spikingbrain_7b_b200.hf_cache import Cache
+    B, kvh, H = 2, 4, 28
+    cache = Cache(kv_dtype="fp8_e4m3", unbounded_capacity=40)
+    oracle = ref_ops.RefWindowCache()
+    for step, n in enumerate([20, 4] + [1] * 60):
+        if step == 1 and window is not None:
+            n = window - 20
+        k, v = (_rows((B, kvh, n, D), 100 + 2 * step + i).to(dtype) for i in range(2))
+        st = cache.update(attn_state=(k.to(DEV), v.to(DEV)), layer_idx=0, offset=n, cache_kwargs={"window_size": window})
+        kq, vq = (ref.values(*ref.quantise(x)).to(dtype) for x in (k, v))
+        want = oracle.update(attn_state=(kq, vq), layer_idx=0, offset=n, cache_kwargs={"window_size": window})["attn_state"]
+        for a, b in zip(st["attn_state"], want):
+            assert a.dtype == dtype and torch.equal(a.cpu(), b)
+        if D == 128 and n == 1 and step % 9 == 0:
+            q = _rows((B, H, D), 300 + step).bfloat16().to(DEV)
+            out = cache.swa_decode(q, 0)
+            for b in range(B):
+                kk, vv = (t[b].transpose(0, 1).to(DEV) for t in want)
+                seen = torch.ones(1, kk.shape[0], dtype=torch.bool, device=DEV)
+                _check(out[b:b + 1], None, ref.attend(q[b:b + 1], kk, vv, seen, D ** -0.5))
+    assert cache.status() == 0
+    legacy = cache.to_legacy_cache()
+    again = Cache.from_legacy_cache(legacy, seen_tokens=cache.get_seq_length(), kv_dtype="fp8_e4m3")
+    k, v = (_rows((B, kvh, 1, D), 400 + i).to(dtype) for i in range(2))
+    got = again.update(attn_state=(k.to(DEV), v.to(DEV)), layer_idx=0, offset=1, cache_kwargs={"window_size": window})["attn_state"]
+    kq = ref.values(*ref.quantise(k)).to(dtype)
+    old = legacy[0]["attn_state"][0].cpu()
+    keep = old if window is None else old[..., -(window - 1):, :]
+    assert torch.equal(got[0].cpu(), torch.cat([keep, kq], -2))              # quantising values again changes nothing
+
+
+@gpu
+def test_hf_cache_in_8_bits_with_rotary(ops):
+    from spikingbrain_7b_b200.hf_cache import Cache
+    B, kvh, H, D, W = 2, 4, 28, 128, 20
+    table = ops.build_cos_sin_cache(D, 512, device=DEV)
+    cache = Cache(kv_dtype="fp8_e4m3")
+    for n, p0 in ((33, 0), (1, 33), (1, 34)):                                # a prompt longer than the window, then tokens
+        q, k, v = (_rows((B, h, n, D), 500 + p0 + i).bfloat16().to(DEV) for i, h in enumerate((H, kvh, kvh)))
+        pos = torch.arange(p0, p0 + n, device=DEV).unsqueeze(0)
+        c, s = table.double()[pos[0], :64], table.double()[pos[0], 64:]
+        turn = lambda x: torch.cat([x.double()[..., :64] * c - x.double()[..., 64:] * s,
+                                    x.double()[..., 64:] * c + x.double()[..., :64] * s], -1)
+        want_q, want_k = turn(q), turn(k)
+        got = cache.update_rotary(q, k, v, pos, table, 0, window_size=W)
+        assert ((got.double() - want_q).abs() <= 2.0 ** -8 * want_q.abs() + 2.0 ** -21 * q.double().abs().amax()).all()
+        m = min(n, W)
+        newest = cache[0]["attn_state"][0][:, :, -m:].double()
+        want_k = want_k[:, :, -m:]
+        # nearest code: half a step of the value, or of the smallest codes of its row (2^-10 of a 448th of the row's largest)
+        bound = torch.maximum(want_k.abs() * 2.0 ** -4, want_k.abs().amax(-1, keepdim=True) * 2.0 ** -17) * (1 + 2.0 ** -10)
+        assert ((newest - want_k).abs() <= bound).all()
+    assert cache.status() == 0
