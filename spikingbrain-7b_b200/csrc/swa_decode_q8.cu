@@ -132,6 +132,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 template <int N>
 __device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
 
@@ -177,6 +181,8 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (threadIdx.x == 0) {
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(bar_full + 8 * s, 1 + 32);   // the stage's bytes, and each producer lane's exponents
       mbar_init(bar_empty + 8 * s, C::kWarps);
@@ -187,6 +193,8 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     fence_mbar_init();
   }
   __syncthreads();
+  // what came before on the stream is done from here on (this kernel may have been set up ahead of its end)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // ---- what every item costs, as an exclusive prefix: units of b occupy [pre[b], pre[b] + units), its charge follows ----
   {
     constexpr int kRun = (kMaxSeqs + kThreads - 1) / kThreads;
@@ -277,6 +285,12 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       const int seq = (P.item0 + b) / P.per_seq;
       const int row = first_row(b);
       const int32_t* table = P.block_tables + (int64_t)seq * P.max_blocks;
+      // the consumers ask for the query rows when the first stage is there: by then they are in this SM's cache
+      const uint8_t* q_rows = reinterpret_cast<const uint8_t*>(P.q + (int64_t)row * P.q_stride);
+      for (int i = lane; i < n_q * P.H * kD / 64; i += 32) {
+        const int qi = i / (P.H * kD / 64);
+        prefetch_l1(q_rows + (int64_t)qi * P.q_stride * 2 + (i - qi * (P.H * kD / 64)) * 128);
+      }
       int64_t pb_lane = -1;            // physical block of chunk (batch0 + lane): one table read per 32 chunks
       int batch0 = 0;
       const int n = n_units > 0 ? n_units : 1;
@@ -721,6 +735,7 @@ template <int WPH, int HPC, typename TO>
 __global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P, int cap) {
   __shared__ float4 part_o[WPH * HPC][32];
   __shared__ float2 part_ml[WPH * HPC];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the next launch waits for this one's end in the same way)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 cut = P.cut[blockIdx.x];                    // first query row, first CTA, pieces, queries
   if (cut.z <= 1) return;
@@ -815,21 +830,30 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
     // a batch between one and two items per SM: one CTA each, so that every SM has work either way of cutting
     if (2 * P.B >= n_ctas && P.B < n_ctas) grid = P.B;
     P.cut_by_item = P.B < grid;
-    kern<<<grid, C::kThreads, C::kSmemBytes, st>>>(P, map_k, map_v);
-    const int rc = check_launch(who);
-    if (rc != SBK_OK) return rc;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t main_cfg = {};
+    main_cfg.gridDim = dim3(grid);
+    main_cfg.blockDim = dim3(C::kThreads);
+    main_cfg.dynamicSmemBytes = C::kSmemBytes;
+    main_cfg.stream = st;
+    main_cfg.attrs = attr;
+    main_cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&main_cfg, kern, P, map_k, map_v);
+    if (e != cudaSuccess) {
+      set_error("%s: launch failed: %s", who, cudaGetErrorString(e));
+      return SBK_E_LAUNCH;
+    }
     // Few items are cut into many pieces: sixteen warps to a head. Else four heads to a block of eight warps.
     const bool few = P.B <= 32;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(P.cut_by_item ? P.B : grid, few ? P.H * kCap : (P.H * kCap + 3) / 4);
     cfg.blockDim = dim3(few ? 512 : 256);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, fold_kernel<16, 1, TO>, P, kCap) : cudaLaunchKernelEx(&cfg, fold_kernel<2, 4, TO>, P, kCap);
+    e = few ? cudaLaunchKernelEx(&cfg, fold_kernel<16, 1, TO>, P, kCap) : cudaLaunchKernelEx(&cfg, fold_kernel<2, 4, TO>, P, kCap);
     if (e != cudaSuccess) {
       set_error("%s: launch of the folding kernel failed: %s", who, cudaGetErrorString(e));
       return SBK_E_LAUNCH;
