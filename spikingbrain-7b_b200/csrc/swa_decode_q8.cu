@@ -873,7 +873,8 @@ int stream_cache(const char* who, const Call& c, cudaStream_t st) {
   P.k_scale = (const uint8_t*)c.k_scale; P.v_scale = (const uint8_t*)c.v_scale; P.scale_block_stride = c.scale_block_stride;
   P.block_tables = c.block_tables; P.max_blocks = c.max_blocks; P.seq_lens = c.seq_lens;
   P.query_start_loc = c.query_start_loc; P.context_lens = c.context_lens; P.max_query_len = c.max_query_len;
-  P.per_seq = runs ? (c.max_query_len + 3) / 4 : 1;
+  const bool two = c.max_query_len <= 2;                 // (runs of one or two: one query group, two CTAs per SM)
+  P.per_seq = !runs || two ? 1 : (c.max_query_len + 3) / 4;
   P.H = c.H; P.num_blocks = c.num_blocks; P.block_size = c.block_size; P.window_left = c.window_left;
   P.scale_log2 = c.scale * kLog2e; P.out = c.out; P.out_stride = c.out_stride; P.lse_out = c.lse_out; P.status = c.status;
   P.cut = (int4*)c.workspace;
@@ -904,6 +905,7 @@ int stream_cache(const char* who, const Call& c, cudaStream_t st) {
     case 2: return launch<2, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);       \
     default: return launch<4, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);      \
   }
+  if (runs && two) { SBK_STREAM(2, 1, __nv_bfloat16) }
   if (runs) { SBK_STREAM(2, 2, __nv_bfloat16) }
   if (c.out_dtype == SBK_BF16) { SBK_STREAM(1, 1, __nv_bfloat16) } else { SBK_STREAM(1, 1, float) }
 #undef SBK_STREAM
