@@ -9,9 +9,17 @@
 //   HBM-bound in prompts (reads T * (2 kvh + H) * D elements, writes the rotated queries and 2 kvh (D + 1) bytes a token),
 //   latency-bound in decode steps.
 #include "kv_q8.cuh"
+#include "sbk_tcgen05.cuh"
 
 namespace sbk {
 namespace q8 {
+
+using namespace tc5;                  // packed fp32 pairs
+__device__ __forceinline__ f32x2 fmul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 template <typename T> struct Vec8;   // eight elements of a row
 template <> struct Vec8<__nv_bfloat16> {
@@ -54,13 +62,17 @@ struct AppendParams {
   int B, window_left; int32_t* retired_out; int max_retired; int32_t* status;
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128;
 
 // V = D / 8 vectors per row, V / 2 lanes, two vectors each: a rotated pair (j, j + half) lies in one lane, so the rotation needs
 // no exchange and its cosines are read once for both. Rows of a token: kvh of K, kvh of V, H of the query. CTAs past the
-// last row retire blocks.
+// last row retire blocks. Bound by the latency of position -> cosines and slot -> cache (a third of the DRAM
+// rate; the issue slots are 60 % busy), so by the rows in flight: twelve CTAs of 128 threads per SM. Measured on 8192 tokens,
+// 28 + 4 heads of 128 (142 MB, 22 us at the copy rate): 29 us; 31 us at the 47 registers the compiler takes when it may; 58 us
+// with one vector per lane and the partner's values by shuffles; 48 us with four query heads per lane group (fewer address
+// and table reads, a quarter of the threads).
 template <typename T, int V, bool ROPE>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_q8_kernel(const AppendParams p, int row_ctas) {
+__global__ void __launch_bounds__(kAppendThreads, 12) kv_append_q8_kernel(const AppendParams p, int row_ctas) {
   constexpr int D = 8 * V, LPR = V / 2, kRows = kAppendThreads / LPR, ES = (int)sizeof(T);
   if ((int)blockIdx.x >= row_ctas) {
     retire_rows(((int)blockIdx.x - row_ctas) * kAppendThreads + threadIdx.x, p.block_tables, p.max_blocks, p.seq_lens,
@@ -110,11 +122,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_q8_kernel(const Appe
       const uint8_t* tab = p.cos_sin + (pos * p.rot_dim + 8 * l) * ES;
       Vec8<T>::load(tab, c);
       Vec8<T>::load(tab + (p.rot_dim >> 1) * ES, s);
+      // products and sums of two values at a time, each rounded once as ever
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = a[i], y = b[i];
-        a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
-        b[i] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
+      for (int i = 0; i < 8; i += 2) {
+        const f32x2 x = pack2(a[i], a[i + 1]), y = pack2(b[i], b[i + 1]), cc = pack2(c[i], c[i + 1]), ss = pack2(s[i], s[i + 1]);
+        unpack2(ffma2(fmul2(y, ss), pack2(-1.f, -1.f), fmul2(x, cc)), a[i], a[i + 1]);
+        unpack2(fadd2(fmul2(y, cc), fmul2(x, ss)), b[i], b[i + 1]);
       }
     }
     if (is_q || p.key_in_place) {
