@@ -1,8 +1,14 @@
-// Sliding-window attention of one query token per sequence over the 8-bit paged K/V cache (format: kv_q8.cuh):
+// Sliding-window attention of one query token per sequence, or of a few, over the 8-bit paged K/V cache (format: kv_q8.cuh):
 //     s_j = scale * 2^ek_j * sum_d q_d ck_jd      o = sum_j softmax(s)_j * 2^ev_j * cv_jd      lse = log sum_j exp(s_j)
 // over the visible tokens j of a sequence, ck / cv being the e4m3 codes and ek / ev the exponents of a row.
 //
-// Bound by HBM: 2 kvh (D + 1) bytes per visible token, at 14 flops a byte.
+// Single tokens are bound by HBM: 2 kvh (D + 1) bytes per visible token, at 14 flops a byte. 28 + 4 heads of 128, window 4096:
+//   256 sequences of 8193 tokens 170 us (1.08 GB, 6.4 TB/s); 64 of 1025 ... 32769 54 us (4.9 TB/s; 11 us of it until the first
+//   bytes come and from the last ones to the folded rows); 4 of 131072, no window, 87 us (5.8 TB/s).
+// Runs of up to four queries to an item read the cache once for them, and are bound by the instructions around the products: 64 x 4
+//   queries 109 us (2.5 TB/s; 0.35 instructions issued per cycle and scheduler, eight consumer warps an SM being all that the
+//   accumulators leave room for). Two groups of four warps with two queries each, every code converted twice, took
+//   124 us; the weights of all four queries before one vote on the offsets, not query by query, 122 us.
 //
 // Products. Both run on mma.sync m16n8k16 in fp16, the codes converted in registers on their way into the A operand (exact, two codes
 //   per instruction), K and V taking the 16-row side and the query heads of a kv group (at most eight) the other:
@@ -10,7 +16,7 @@
 //   q is scaled by the power of two that takes its largest value under 448: a bf16 number is an fp16 number then (elements below
 //   2^-23 of the largest lose bits no score shows). Feeding the codes to the e4m3 MMA as they are, with query and
 //   probabilities split into two 4-bit parts, takes three times the instructions: the compiler expands that MMA into
-//   conversions of both operands and two fp16 ones (64 mixed sequences: 67 us against 5x us).
+//   conversions of both operands and two fp16 ones (64 mixed sequences: 72 us against 64 in fp16, the rest alike).
 // Softmax. The V scale belongs to the probability's exponent: with an offset m per head the normaliser sums p_j = 2^(s_j - m), and
 //   the product takes w_j = p_j 2^(ev_j - r), rounded to fp16's eleven bits. m and r are not the running maxima: they move only
 //   when a w would leave fp16 (or p grow past 2^40), to put the largest w of the item between 2^6 and 2^7; until the
@@ -22,7 +28,7 @@
 //   8-bit one) then come from eight different 16-byte columns of the 128-byte swizzle, eight rows at a time.
 // Data movement. One producer warp walks the block table and issues a TMA tensor copy per 16 tokens (kvh * 2 KiB of K, the same of V)
 //   into a ring of three 32 KiB stages; two CTAs per SM. The exponents, 16 bytes per head and 16 tokens, come beside them through
-//   the load path (cp.async): as bulk copies they took four of five requests of the copy engine (XX us). A stage holds 32
+//   the load path (cp.async): as bulk copies they took four of five requests of the copy engine (256 sequences: 214 us against 184). A stage holds 32
 //   tokens per consumer warp: warp w serves kv head w % kvh and the 32-token part w / kvh.
 // Partition. The units (one stage of tokens each) of all sequences, laid end to end with a fixed charge per sequence, are cut
 //   into one equal run per CTA. Only the first and the last sequence of a run can be cut, so a CTA writes at most two partial results
@@ -39,7 +45,6 @@ namespace decode_q8 {
 constexpr int kD = 128, kChunk = 16, kMaxG = 8;
 constexpr int kMaxSeqs = 1024;        // items (sequences, or groups of queries of one) per launch: lengths and prefix in shared memory
 constexpr int kMaxSms = 160;          // as many as the workspace is laid out for
-constexpr int kItemCost = 2;          // what starting and finishing an item is charged, in units
 constexpr int kTileBytes = 16384;     // K, or V, of a stage
 constexpr int kScaleBytes = 256;      // exponents of a stage: 128 of K, 128 of V
 constexpr int kStageBytes = 2 * kTileBytes;
@@ -52,16 +57,25 @@ enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8 };
 // part: partial slot of the item's result, or -1 (direct)
 struct StageInfo { int row, n_q, top, tok_base, lo, hi, flags, part; };
 
-// QG groups of four consumer warps, each with NQ queries of an item: one group and two CTAs per SM for single tokens, two
-// groups that read the same stages for runs of a few
-template <int QG>
+// Four consumer warps and a producer, two CTAs per SM. Up to two queries to an item live in registers. Four do not: their
+// fragments and the state of their softmax lie in shared memory, in place of a third stage, and the consumers take over the
+// registers that three idle warps beside the producer give up (what the block is launched with is what the two warpgroups
+// hold afterwards: 256 x 128 = 128 x 216 + 128 x 40).
+template <int NQ>
 struct Cfg {
-  static constexpr int kWarps = 4 * QG, kThreads = 32 * (kWarps + 1), kConsumers = 32 * kWarps;
-  static constexpr int kCtasPerSm = QG == 1 ? 2 : 1;
-  static constexpr int kMaxCtas = kMaxSms * kCtasPerSm;
-  static constexpr int kStages = 3 * QG;
+  static constexpr bool kShare = NQ > 2;
+  static constexpr int kWarps = 4, kConsumers = 32 * kWarps, kThreads = kShare ? 256 : 160;
+  static constexpr int kConsumerRegs = 216, kProducerRegs = 40;
+  static constexpr int kCtasPerSm = 2;
+  static constexpr int kStages = kShare ? 2 : 3;
+  // What starting and finishing an item is charged, in units. Measured: 1024 ragged sequences 121 us with 2, 123 with 4, 126
+  // with 8; runs 64 x 4: 124 us with 2, 120 with 4, 113 with 8, 109 with 12, 111 with 16
+  static constexpr int kItemCost = kShare ? 12 : 2;
   static constexpr int kScaleOff = kStages * kStageBytes;
-  static constexpr int kInfoOff = kScaleOff + kStages * kScaleBytes;
+  static constexpr int kQueryOff = kScaleOff + kStages * kScaleBytes;   // [warp][query][4][lane] 16 bytes: steps 2j and 2j + 1
+  static constexpr int kStateOff = kQueryOff + (kShare ? kWarps * NQ * 2048 : 0);   // [warp][query][t] (m, m, 2^-r, 2^-r)
+  static constexpr int kFactorOff = kStateOff + (kShare ? kWarps * NQ * 64 : 0);    // [warp][query][head] what a product is scaled by
+  static constexpr int kInfoOff = kFactorOff + (kShare ? kWarps * NQ * 32 : 0);
   static constexpr int kPreOff = kInfoOff + kStages * (int)sizeof(StageInfo);
   static constexpr int kLensOff = kPreOff + (kMaxSeqs + 4) * 4;
   static constexpr int kCntOff = kLensOff + kMaxSeqs * 4;
@@ -71,6 +85,8 @@ struct Cfg {
   static constexpr int kSmemBytes = kMiscOff + 64 + 1024;        // + slack to align the ring to 1 KiB
   static_assert(kSmemBytes * kCtasPerSm <= 230400, "the CTAs of an SM must fit its shared memory");
   static_assert(kWarps * kMergeWarpBytes <= kStageBytes, "the merge scratch lives inside one stage");
+  static_assert(!kShare || kConsumers * kConsumerRegs + (kThreads - kConsumers) * kProducerRegs <= kThreads * 128,
+                "the registers of the warpgroups must fit what the block is launched with");
 };
 
 struct Params {
@@ -102,7 +118,7 @@ __device__ __forceinline__ Span span_of(int top, int n_q, int window_left) {
 
 // D(16x8,f32) += A(16x16,f16,row) * B(16x8,f16,col)
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -155,12 +171,19 @@ __device__ __forceinline__ void store4(TO* p, float4 v) { store2(p, v.x, v.y); s
 __device__ __forceinline__ float row_lse(float m, float l) { return l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY; }
 __device__ __forceinline__ float inverse(float l) { return l != 0.f ? 1.f / l : 0.f; }
 
-template <int KVH, int NQ, int QG, typename TO>
-__global__ void __launch_bounds__(Cfg<QG>::kThreads, Cfg<QG>::kCtasPerSm)
+using namespace tc5;                  // packed fp32 pairs
+__device__ __forceinline__ f32x2 fmul2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+template <int KVH, int NQ, typename TO>
+__global__ void __launch_bounds__(Cfg<NQ>::kThreads, Cfg<NQ>::kCtasPerSm)
 stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
-  using C = Cfg<QG>;
+  using C = Cfg<NQ>;
   constexpr int kStages = C::kStages, kThreads = C::kThreads;
-  constexpr int kCap = NQ * QG;                       // queries of an item
+  constexpr int kCap = NQ;                            // queries of an item
   constexpr int kSub = 4 / KVH;                       // 32-token parts of a stage
   constexpr int kUnit = 32 * kSub;                    // tokens of a stage
   constexpr int kChunks = kUnit / kChunk;             // 16-token chunks of a stage
@@ -229,7 +252,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         if (top >= 0) {
           c = top > 0 ? span_of<kUnit>(top, n, P.window_left).units : 1;   // an empty one keeps a unit: somebody writes its zeros
           mx = max(mx, c);
-          c += kItemCost;
+          c += C::kItemCost;
         } else if (blockIdx.x == 0 && P.cut_by_item) {
           P.cut[b] = kNotCut;
         }
@@ -267,15 +290,19 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   if (per < 1) per = 1;
   // A batch of near-equal items that fills the CTAs evenly streams fastest as whole items: no partials to write and fold.
   const int rounds = (P.B + n_cta - 1) / n_cta;
-  const bool whole = 2 * P.B >= n_cta && (P.B <= n_cta || 10 * rounds * n_cta <= 11 * P.B) &&
-                     (int64_t)misc[1] * P.B <= ((int64_t)total - (int64_t)kItemCost * P.B) / 8 * 9;
+  const bool whole = 2 * P.B >= n_cta && ((P.B <= n_cta && !C::kShare) || 10 * rounds * n_cta <= 11 * P.B) &&
+                     (int64_t)misc[1] * P.B <= ((int64_t)total - (int64_t)C::kItemCost * P.B) / 8 * 9;
   auto first_row = [&](int b) {
     if (P.seq_lens) return P.item0 + b;
     const int v = P.item0 + b, s = v / P.per_seq;
     return P.query_start_loc[s] + (v - s * P.per_seq) * kCap;
   };
 
-  if (warp == C::kWarps) {
+  if (warp >= C::kWarps) {
+    if constexpr (C::kShare) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kProducerRegs));   // (every warp of the warpgroup)
+      if (warp > C::kWarps) return;
+    }
     // ================================= producer =================================
     int it = 0;
     bool aborted = false;
@@ -430,8 +457,8 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   }
 
   // ================================== consumers ==================================
-  const int qg = warp >> 2, w4 = warp & 3;            // query group, warp of the group
-  const int hk = w4 % KVH, sub = w4 / KVH, G = P.H / KVH;
+  if constexpr (C::kShare) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kConsumerRegs));
+  const int hk = warp % KVH, sub = warp / KVH, G = P.H / KVH;
   const int g = lane >> 2, t = lane & 3;
   TO* const out = reinterpret_cast<TO*>(P.out);
 
@@ -445,9 +472,19 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   const int xk = (tokk & 7) ^ (lane >> 4), xv = (tokv & 7) ^ (lane >> 4);
   const int ta = g, tb8 = 8 + (g ^ 4);             // a thread's tokens in every sixteen
 
-  uint32_t qf[NQ][8][2];
+  constexpr int kR = C::kShare ? 1 : NQ;           // queries whose fragments and state are in registers all along
+  uint32_t qf[kR][8][2];
   float acc[NQ][8][4];
-  float m[NQ][2], l[NQ][2], rs[NQ][2], qs[NQ][2];  // of heads 2t, 2t + 1 (rs = 2^-r)
+  float m[kR][2], l[NQ][2], rs[kR][2], qs[kR][2];  // of heads 2t, 2t + 1 (rs = 2^-r)
+  uint4* const q_sh = reinterpret_cast<uint4*>(smem + C::kQueryOff) + warp * NQ * 128 + lane;
+  float4* const st_sh = reinterpret_cast<float4*>(smem + C::kStateOff) + warp * NQ * 4 + t;
+  float* const fa_sh = reinterpret_cast<float*>(smem + C::kFactorOff) + warp * NQ * 8;
+  auto load_state = [&](int n) {                   // of query n, to the registers of its slot
+    if constexpr (C::kShare) {
+      const float4 x = st_sh[4 * n];
+      m[0][0] = x.x; m[0][1] = x.y; rs[0][0] = x.z; rs[0][1] = x.w;
+    }
+  };
   for (int it = 0;; ++it) {
     const int s = it % kStages;
     if (!mbar_wait_bounded(bar_full + 8 * s, (it / kStages) & 1)) {
@@ -458,14 +495,15 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     if (si.flags & kEnd) return;
     const uint32_t stage = ring + s * kStageBytes;
 
-    if (si.flags & kFirst) {
-#pragma unroll
+    if (__builtin_expect(si.flags & kFirst, 0)) {
+      if constexpr (C::kShare) __syncwarp();       // (the item before is done with its state)
+#pragma unroll(kR)
       for (int n = 0; n < NQ; ++n) {
+        const int r = C::kShare ? 0 : n;
         // q of head g: dims 16c + 4t ... + 3 (zeros for a head or a query that is not there)
-        const int qi = qg * NQ + n;
-        const bool head_ok = g < G && qi < si.n_q;
+        const bool head_ok = g < G && n < si.n_q;
         const __nv_bfloat16* qp =
-            P.q + (int64_t)(si.row + (head_ok ? qi : 0)) * P.q_stride + (int64_t)(hk * G + (head_ok ? g : 0)) * kD + 4 * t;
+            P.q + (int64_t)(si.row + (head_ok ? n : 0)) * P.q_stride + (int64_t)(hk * G + (head_ok ? g : 0)) * kD + 4 * t;
         uint32_t w[16];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -485,26 +523,38 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         const float inv = q8::pow2i(-e), mine = P.scale_log2 * q8::pow2i(e);
 #pragma unroll
         for (int i = 0; i < 16; ++i)         // (an infinity stays one: the head's scores are NaN or infinite)
-          qf[n][i >> 1][i & 1] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+          w[i] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);
+        if constexpr (C::kShare) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          qs[n][i] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + i));
-          m[n][i] = kNegBig;
-          l[n][i] = 0.f;
-          rs[n][i] = 1.f;
+          for (int j = 0; j < 4; ++j) q_sh[(n * 4 + j) * 32] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          if (t == 0) fa_sh[8 * n + g] = mine;
+          if (g == 0) st_sh[4 * n] = make_float4(kNegBig, kNegBig, 1.f, 1.f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) qf[r][i >> 1][i & 1] = w[i];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            qs[r][i] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + i));
+            m[r][i] = kNegBig;
+            rs[r][i] = 1.f;
+          }
         }
+      }
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        l[n][0] = l[n][1] = 0.f;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) acc[n][mt][0] = acc[n][mt][1] = acc[n][mt][2] = acc[n][mt][3] = 0.f;
       }
+      if constexpr (C::kShare) __syncwarp();
     }
 
     const int tb = si.tok_base + 32 * sub;                      // my 32 tokens
     const int vlo = si.lo > tb ? si.lo : tb, vhi = si.hi < tb + 32 ? si.hi : tb + 32;
-    if (!(si.flags & kBad) && vhi > vlo && (QG == 1 || qg * NQ < si.n_q)) {
+    if (!(si.flags & kBad) && vhi > vlo) {
       const bool edge = vlo > tb || vhi < tb + 32;
-      if (edge) {
+      if (__builtin_expect(edge, 0)) {
         // rows outside the visible range hold anything, or older data: a zero probability must not meet a NaN code
-        // (groups of warps that share the tile all write the same zeros)
         for (int row = lane >> 3; row < 32; row += 4)
           if (tb + row < vlo || tb + row >= vhi)
             *reinterpret_cast<uint4*>(smem + s * kStageBytes + kTileBytes + tile0 + (row >> 4) * kChunkBytes + (row & 15) * 128 +
@@ -512,35 +562,71 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         __syncwarp();
       }
       // ---- scores: [query][16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
-      float sc[NQ][2][4], ve[2][2];
+      float sc[NQ][2][4], ke[2][2], ve[2][2];
       const uint8_t* se = smem + C::kScaleOff + s * kScaleBytes + (sub * KVH + hk) * 32;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float ka = __uint_as_float((uint32_t)se[16 * h + ta] << 23), kb = __uint_as_float((uint32_t)se[16 * h + tb8] << 23);
-        ve[h][0] = __uint_as_float((uint32_t)se[128 + 16 * h + ta] << 23);
-        ve[h][1] = __uint_as_float((uint32_t)se[128 + 16 * h + tb8] << 23);
-        float ca[NQ][4], cb[NQ][4];
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ke[h][i] = __uint_as_float((uint32_t)se[16 * h + (i ? tb8 : ta)] << 23);
+          ve[h][i] = __uint_as_float((uint32_t)se[128 + 16 * h + (i ? tb8 : ta)] << 23);
+        }
+      if constexpr (C::kShare) {
+        // (one chain per query and half: there are enough of them)
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ca[n][i] = cb[n][i] = 0.f;
+          for (int i = 0; i < 4; ++i) sc[n][0][i] = sc[n][1][i] = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; c += 2) {
-          uint32_t w[4], a[4];
-          ldmatrix_x4(w, stage + h * kChunkBytes + k0 + ((c ^ xk) << 4));
-          widen(a, w[0], w[1]);
+          uint32_t w[2][4], a[2][4];
+          uint4 q4[NQ];
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) mma_f16(ca[n], a, qf[n][c][0], qf[n][c][1]);
-          widen(a, w[2], w[3]);
+          for (int n = 0; n < NQ; ++n) q4[n] = q_sh[(n * 4 + c / 2) * 32];
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) mma_f16(cb[n], a, qf[n][c + 1][0], qf[n][c + 1][1]);
+          for (int h = 0; h < 2; ++h) {
+            ldmatrix_x4(w[h], stage + h * kChunkBytes + k0 + ((c ^ xk) << 4));
+            widen(a[h], w[h][0], w[h][1]);
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            mma_f16(sc[n][0], a[0], q4[n].x, q4[n].y);
+            mma_f16(sc[n][1], a[1], q4[n].x, q4[n].y);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) widen(a[h], w[h][2], w[h][3]);
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            mma_f16(sc[n][0], a[0], q4[n].z, q4[n].w);
+            mma_f16(sc[n][1], a[1], q4[n].z, q4[n].w);
+          }
         }
+      } else {
 #pragma unroll
-        for (int n = 0; n < NQ; ++n)
+        for (int h = 0; h < 2; ++h) {
+          float cb[NQ][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[n][h][i] = (ca[n][i] + cb[n][i]) * (qs[n][i & 1] * (i < 2 ? ka : kb));
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[n][h][i] = cb[n][i] = 0.f;
+#pragma unroll
+          for (int c = 0; c < 8; c += 2) {
+            uint32_t w[4], a[4];
+            ldmatrix_x4(w, stage + h * kChunkBytes + k0 + ((c ^ xk) << 4));
+            widen(a, w[0], w[1]);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mma_f16(sc[n][h], a, qf[n][c][0], qf[n][c][1]);
+            widen(a, w[2], w[3]);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) mma_f16(cb[n], a, qf[n][c + 1][0], qf[n][c + 1][1]);
+          }
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[n][h][i] += cb[n][i];
+        }
       }
-      if (edge) {
+      if (__builtin_expect(edge, 0)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
@@ -551,15 +637,27 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       uint32_t pf[NQ][2][2];
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
+        const int r = C::kShare ? 0 : n;
+        load_state(n);
+        if constexpr (C::kShare) {
+          const float2 f = *reinterpret_cast<const float2*>(fa_sh + 8 * n + 2 * t);
+          qs[0][0] = f.x; qs[0][1] = f.y;
+        }
+        const f32x2 q2 = pack2(qs[r][0], qs[r][1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2)
+            unpack2(fmul2(pack2(sc[n][h][i], sc[n][h][i + 1]), fmul2(q2, pack2(ke[h][i >> 1], ke[h][i >> 1]))), sc[n][h][i], sc[n][h][i + 1]);
         // keys that this query sees; with several queries each has its own edge
         int nlo = vlo, nhi = vhi;
-        if (NQ * QG > 1) {
-          const int last = si.top - si.n_q + qg * NQ + n;            // the query's own position
+        if (NQ > 1) {
+          const int last = si.top - si.n_q + n;            // the query's own position
           const int first = P.window_left < 0 || last <= P.window_left ? 0 : last - P.window_left;
           nlo = first > vlo ? first : vlo;
           nhi = last + 1 < vhi ? last + 1 : vhi;
         }
-        if (nlo > tb || nhi < tb + 32) {
+        if (__builtin_expect(nlo > tb || nhi < tb + 32, 0)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
@@ -568,24 +666,26 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           }
         }
         // ---- p = 2^(s - m), w = p * 2^(ev - r) with the offsets in use; they move only when a w leaves fp16 ----
-        float p[2][4], w[2][4], wtop, ptop;
+        float w[2][4], ps[2], wtop;                 // (ps: sums of p)
         auto weigh = [&]() {
-          wtop = ptop = 0.f;
+          const f32x2 nm = pack2(-m[r][0], -m[r][1]), r2 = pack2(rs[r][0], rs[r][1]);
+          f32x2 sum = pack2(0.f, 0.f);
+          wtop = 0.f;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-#pragma unroll
-              for (int j = i; j < i + 2; ++j) {
-                p[h][j] = fast_exp2(sc[n][h][j] - m[n][j & 1]);
-                w[h][j] = p[h][j] * (ve[h][j >> 1] * rs[n][j & 1]);
-              }
+              float x, y;
+              unpack2(fadd2(pack2(sc[n][h][i], sc[n][h][i + 1]), nm), x, y);
+              const f32x2 p = pack2(fast_exp2(x), fast_exp2(y));
+              sum = fadd2(sum, p);
+              unpack2(fmul2(p, fmul2(r2, pack2(ve[h][i >> 1], ve[h][i >> 1]))), w[h][i], w[h][i + 1]);
               wtop = tc5::fmax3(wtop, w[h][i], w[h][i + 1]);
-              ptop = tc5::fmax3(ptop, p[h][i], p[h][i + 1]);
             }
+          unpack2(sum, ps[0], ps[1]);
         };
         weigh();
-        if (__any_sync(0xffffffffu, wtop > kMostW || ptop > kMostP)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, wtop > kMostW || fmaxf(ps[0], ps[1]) > kMostP), 0)) {
           // (rare: the first tokens of an item, and where a score or a V row outgrows all before it by 2^8)
           float mx[2], ne[2];
 #pragma unroll
@@ -598,10 +698,10 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float mn = fmaxf(m[n][i], mx[i]);
-            ne[i] = fast_exp2(m[n][i] - mn);
+            const float mn = fmaxf(m[r][i], mx[i]);
+            ne[i] = fast_exp2(m[r][i] - mn);
             l[n][i] *= ne[i];
-            m[n][i] = mn;
+            m[r][i] = mn;
             mx[i] = 0.f;                        // from here on: the largest p * 2^ev
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -617,20 +717,25 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             // 2^-r: the power of two that takes the largest w so far to [2^6, 2^7) (those before had one of 2^6 at least)
-            const float had = ne[i] * 64.f / rs[n][i];
+            const float had = ne[i] * 64.f / rs[r][i];
             int e = (int)(__float_as_uint(fmaxf(mx[i], had)) >> 23) - 127;
             e = e < -64 ? -64 : (e > 63 ? 63 : e);
-            const float rn = q8::pow2i(6 - e), al = ne[i] * (rn / rs[n][i]);
-            rs[n][i] = rn;
+            const float rn = q8::pow2i(6 - e), al = ne[i] * (rn / rs[r][i]);
+            rs[r][i] = rn;
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) { acc[n][mt][i] *= al; acc[n][mt][2 + i] *= al; }
           }
           weigh();
+          if constexpr (C::kShare) {
+            __syncwarp();
+            if (g == 0) st_sh[4 * n] = make_float4(m[0][0], m[0][1], rs[0][0], rs[0][1]);
+            __syncwarp();
+          }
         }
+        l[n][0] += ps[0];
+        l[n][1] += ps[1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          l[n][0] += p[h][0] + p[h][2];
-          l[n][1] += p[h][1] + p[h][3];
           pf[n][h][0] = movmatrix_trans(pack_f16x2(w[h][0], w[h][1]));
           pf[n][h][1] = movmatrix_trans(pack_f16x2(w[h][2], w[h][3]));
         }
@@ -653,8 +758,10 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     }
     __syncwarp();
     // the last stage of an item becomes the scratch of its output before it goes back to the producer
-    if (lane == 0 && !(si.flags & kLast)) mbar_arrive(bar_empty + 8 * s);
-    if (!(si.flags & kLast)) continue;
+    if (__builtin_expect(!(si.flags & kLast), 1)) {
+      if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+      continue;
+    }
 
     // ================= end of an item: its output rows, or its partials =================
     // [head][dim] floats of every warp in shared memory, four-float columns XOR-ed by the head (no bank is met twice);
@@ -664,13 +771,15 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     float* wml = reinterpret_cast<float*>(smem + C::kMlOff) + warp * 16;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
+      const int r = C::kShare ? 0 : n;
+      load_state(n);
       // (where nothing was visible m is kNegBig, l and O are 0)
       float fix[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], off);
-        fix[i] = 1.f / rs[n][i];
+        fix[i] = 1.f / rs[r][i];
       }
       consumer_bar<C::kConsumers>();          // every warp is done reading this stage, or the results of the query before
 #pragma unroll
@@ -682,29 +791,28 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           wo[hrow * kD + ((16 * mt + g + 8) ^ x)] = acc[n][mt][2 + i] * fix[i];
         }
       if (g == 0) {
-        wml[2 * t] = m[n][0]; wml[2 * t + 1] = m[n][1];
+        wml[2 * t] = m[r][0]; wml[2 * t + 1] = m[r][1];
         wml[8 + 2 * t] = l[n][0]; wml[8 + 2 * t + 1] = l[n][1];
       }
       if constexpr (kSub > 1) consumer_bar<C::kConsumers>(); else __syncwarp();
-      const int qi = qg * NQ + n;
-      if (qi < si.n_q) {
-        const int64_t orow = (int64_t)si.row + qi;
-        const int64_t prow = ((int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * kCap + qi) * P.H;
-        // heads go round the group's warps (one warp to a kv head: its own heads), a lane takes four dims
-        const int h_lo = kSub > 1 ? w4 : hk * G, h_hi = kSub > 1 ? P.H : hk * G + G, h_step = kSub > 1 ? 4 : 1;
+      if (n < si.n_q) {
+        const int64_t orow = (int64_t)si.row + n;
+        const int64_t prow = ((int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * kCap + n) * P.H;
+        // heads go round the warps (one warp to a kv head: its own heads), a lane takes four dims
+        const int h_lo = kSub > 1 ? warp : hk * G, h_hi = kSub > 1 ? P.H : hk * G + G, h_step = kSub > 1 ? 4 : 1;
 #pragma unroll 2
         for (int h = h_lo; h < h_hi; h += h_step) {
           const int kh = h / G, row = h - kh * G;
           float M = -INFINITY;
 #pragma unroll
           for (int w2 = 0; w2 < kSub; ++w2)
-            M = fmaxf(M, reinterpret_cast<const float*>(smem + C::kMlOff)[(qg * 4 + kh + KVH * w2) * 16 + row]);
+            M = fmaxf(M, reinterpret_cast<const float*>(smem + C::kMlOff)[(kh + KVH * w2) * 16 + row]);
           const float Ms = fmaxf(M, kNegBig);
           float L = 0.f;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w2 = 0; w2 < kSub; ++w2) {
-            const int src = qg * 4 + kh + KVH * w2;
+            const int src = kh + KVH * w2;
             const float* po = reinterpret_cast<const float*>(mbuf + src * kMergeWarpBytes);
             const float* ml = reinterpret_cast<const float*>(smem + C::kMlOff) + src * 16;
             const float wgt = kSub > 1 ? fast_exp2(ml[row] - Ms) : 1.f;
@@ -797,15 +905,15 @@ __global__ void __launch_bounds__(32 * WPH * HPC) fold_kernel(const Params P, in
   if (P.lse_out && lane == 0) P.lse_out[(int64_t)(cut.x + qi) * P.H + h] = row_lse(Mt, Lt);
 }
 
-constexpr int kMaxPartials = 2 * 2 * kMaxSms;          // two per CTA, two CTAs per SM with one query group
+constexpr int kMaxPartials = 2 * 2 * kMaxSms;          // two per CTA, two CTAs per SM
 static size_t cut_bytes() { return (size_t)(2 * kMaxSms) * sizeof(int4); }
 
-template <int KVH, int NQ, int QG, typename TO>
+template <int KVH, int NQ, typename TO>
 static int launch(const char* who, const Params& P0, int64_t items, int sms, const CUtensorMap& map_k, const CUtensorMap& map_v,
                   cudaStream_t st) {
-  using C = Cfg<QG>;
-  constexpr int kCap = NQ * QG, kUnit = 32 * 4 / KVH;
-  auto kern = stream_kernel<KVH, NQ, QG, TO>;
+  using C = Cfg<NQ>;
+  constexpr int kCap = NQ, kUnit = 32 * 4 / KVH;
+  auto kern = stream_kernel<KVH, NQ, TO>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -814,6 +922,15 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
     if (e != cudaSuccess) {
       set_error("%s: cannot opt in to %d bytes of shared memory: %s", who, C::kSmemBytes, cudaGetErrorString(e));
       return SBK_E_LAUNCH;
+    }
+    if (C::kShare) {      // (a split of the registers that the launch does not bring would wait forever)
+      cudaFuncAttributes fa;
+      const cudaError_t ea = cudaFuncGetAttributes(&fa, kern);
+      if (ea != cudaSuccess ||
+          fa.numRegs * C::kThreads < C::kConsumers * C::kConsumerRegs + (C::kThreads - C::kConsumers) * C::kProducerRegs) {
+        set_error("%s: the kernel was built with %d registers per thread", who, ea == cudaSuccess ? fa.numRegs : -1);
+        return SBK_E_LAUNCH;
+      }
     }
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
@@ -825,10 +942,11 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
     // no more CTAs than there can be units of work
     const int64_t width = (int64_t)P.max_blocks * P.block_size, seen = (int64_t)P.window_left + kCap;
     const int64_t vis = P.window_left < 0 || width < seen ? width : seen;
-    const int64_t most = (int64_t)P.B * (vis / kUnit + 2 + kItemCost);
+    const int64_t most = (int64_t)P.B * (vis / kUnit + 2 + C::kItemCost);
     int grid = (int)(most < n_ctas ? most : n_ctas);
-    // a batch between one and two items per SM: one CTA each, so that every SM has work either way of cutting
-    if (2 * P.B >= n_ctas && P.B < n_ctas) grid = P.B;
+    // a batch between one and two items per SM: one CTA each, so that every SM has work either way of cutting (four queries
+    // to an item are bound by instructions, not by the copies that a lone CTA can keep up: there both CTAs of an SM share)
+    if (!C::kShare && 2 * P.B >= n_ctas && P.B < n_ctas) grid = P.B;
     P.cut_by_item = P.B < grid;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -845,8 +963,10 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
       set_error("%s: launch failed: %s", who, cudaGetErrorString(e));
       return SBK_E_LAUNCH;
     }
-    // Few items are cut into many pieces: sixteen warps to a head. Else four heads to a block of eight warps.
-    const bool few = P.B <= 32;
+    // Few rows of output, each cut into two pieces a warp at least: sixteen warps to one, as long as the SMs hold them all at once.
+    // Else four to a block of eight warps. (8 sequences x 1 token: 18.1 us against 19.3 the other way, 16 x 1: 25.6 against 28.7;
+    // 8 x 4: 35 against 41; 8 x 16: 66 against 96)
+    const bool few = (int64_t)P.B * P.H * kCap <= 4 * sms && grid >= 32 * P.B;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(P.cut_by_item ? P.B : grid, few ? P.H * kCap : (P.H * kCap + 3) / 4);
     cfg.blockDim = dim3(few ? 512 : 256);
@@ -862,8 +982,8 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
   return SBK_OK;
 }
 
-// rows of partials per head: runs have half the CTAs (two query groups each) and four queries to an item
-static size_t partial_rows(bool runs) { return (size_t)kMaxPartials * (runs ? 2 : 1); }
+// rows of partials per head: runs have up to four queries to an item
+static size_t partial_rows(bool runs) { return (size_t)kMaxPartials * (runs ? 4 : 1); }
 size_t workspace_bytes(int H, bool runs) { return cut_bytes() + partial_rows(runs) * H * (kD + 2) * sizeof(float); }
 
 int stream_cache(const char* who, const Call& c, cudaStream_t st) {
@@ -873,7 +993,7 @@ int stream_cache(const char* who, const Call& c, cudaStream_t st) {
   P.k_scale = (const uint8_t*)c.k_scale; P.v_scale = (const uint8_t*)c.v_scale; P.scale_block_stride = c.scale_block_stride;
   P.block_tables = c.block_tables; P.max_blocks = c.max_blocks; P.seq_lens = c.seq_lens;
   P.query_start_loc = c.query_start_loc; P.context_lens = c.context_lens; P.max_query_len = c.max_query_len;
-  const bool two = c.max_query_len <= 2;                 // (runs of one or two: one query group, two CTAs per SM)
+  const bool two = c.max_query_len <= 2;                 // (what the registers hold)
   P.per_seq = !runs || two ? 1 : (c.max_query_len + 3) / 4;
   P.H = c.H; P.num_blocks = c.num_blocks; P.block_size = c.block_size; P.window_left = c.window_left;
   P.scale_log2 = c.scale * kLog2e; P.out = c.out; P.out_stride = c.out_stride; P.lse_out = c.lse_out; P.status = c.status;
@@ -899,15 +1019,15 @@ int stream_cache(const char* who, const Call& c, cudaStream_t st) {
     return SBK_E_ARG;
   }
   const int64_t items = (int64_t)c.n_seqs * P.per_seq;
-#define SBK_STREAM(NQ, QG, TO)                                                            \
+#define SBK_STREAM(NQ, TO)                                                                \
   switch (c.kvh) {                                                                        \
-    case 1: return launch<1, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);       \
-    case 2: return launch<2, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);       \
-    default: return launch<4, NQ, QG, TO>(who, P, items, sms, maps[0], maps[1], st);      \
+    case 1: return launch<1, NQ, TO>(who, P, items, sms, maps[0], maps[1], st);           \
+    case 2: return launch<2, NQ, TO>(who, P, items, sms, maps[0], maps[1], st);           \
+    default: return launch<4, NQ, TO>(who, P, items, sms, maps[0], maps[1], st);          \
   }
-  if (runs && two) { SBK_STREAM(2, 1, __nv_bfloat16) }
-  if (runs) { SBK_STREAM(2, 2, __nv_bfloat16) }
-  if (c.out_dtype == SBK_BF16) { SBK_STREAM(1, 1, __nv_bfloat16) } else { SBK_STREAM(1, 1, float) }
+  if (runs && two) { SBK_STREAM(2, __nv_bfloat16) }
+  if (runs) { SBK_STREAM(4, __nv_bfloat16) }
+  if (c.out_dtype == SBK_BF16) { SBK_STREAM(1, __nv_bfloat16) } else { SBK_STREAM(1, float) }
 #undef SBK_STREAM
 }
 

@@ -440,7 +440,8 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 }
 
 // Runs of at most kFew queries go through the kernel of the single tokens, which reads the cache once for four queries and
-// expands nothing.
+// expands nothing. Measured there against here, us, window 4096 on 8190 cached tokens: 64 runs of 4 109 / 381, of 8 187 / 375,
+// of 16 336 / 384, of 20 407 / 413; 256 of 16 1162, of 20 1495 / 1391; 8 of 16 66 / 103; 1 of 16 32 / 87, of 32 40 / 90.
 constexpr int kFew = 16;
 static bool few_queries(int max_query_len, int kvh) { return max_query_len <= kFew && (kvh == 1 || kvh == 2 || kvh == 4); }
 

@@ -514,7 +514,7 @@ def test_decode_reads_far_into_a_large_pool(ops):
     assert torch.equal(codes[1, nb - 1, bs - 1].cpu(), ref.quantise(new[0])[0]) and st.item() == 0
 
 
-def _runs(ops, ctx, new, wl, H, kvh, bs, seed, spread=3.0, qmag=1.0):
+def _runs(ops, ctx, new, wl, H, kvh, bs, seed, spread=3.0, qmag=1.0, scale=128 ** -0.5):
     lens = [a + b for a, b in zip(ctx, new)]
     codes, scales, table = (t.to(DEV) for t in _pool(lens, wl, kvh, 128, bs, seed, spread, n_new=new))
     T = sum(new)
@@ -523,10 +523,10 @@ def _runs(ops, ctx, new, wl, H, kvh, bs, seed, spread=3.0, qmag=1.0):
     start = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device=DEV)
     st = _status()
     ops.swa_prefill_q8(q, codes[0], codes[1], scales[0], scales[1], table, start,
-                       torch.tensor(ctx, dtype=torch.int32, device=DEV), max(new), window_left=wl, out=out, status=st)
+                       torch.tensor(ctx, dtype=torch.int32, device=DEV), max(new), window_left=wl, scale=scale, out=out, status=st)
     assert st.item() == 0
     assert (out[T:] == 7.0).all()                                            # rows behind the last sequence stay
-    _check(out[:T], None, ref.runs(q[:T], codes, scales, table, ctx, new, wl, 128 ** -0.5))
+    _check(out[:T], None, ref.runs(q[:T], codes, scales, table, ctx, new, wl, scale))
 
 
 @gpu
@@ -558,6 +558,55 @@ def test_runs_of_a_few_tokens_on_many_sequences(ops, new):
 @pytest.mark.parametrize("spread,qmag", [(60.0, 1.0), (0.0, 60.0), (10.0, 1e-3)])
 def test_runs_magnitudes(ops, spread, qmag):
     _runs(ops, [500, 3], [40, 300], 350, 28, 4, 16, seed=48, spread=spread, qmag=qmag)
+
+
+SHORT = ([0, 5, 300, 1500, 31, 2000, 0], [16, 1, 7, 4, 0, 13, 3])            # runs that stream the cache, four queries at a time
+
+
+@gpu
+@pytest.mark.parametrize("wl", [0, 1, 14, 15, 16, 31, 127, 1000, -1])
+def test_short_runs_windows(ops, wl):
+    _runs(ops, *SHORT, wl, 28, 4, 16, seed=90)
+
+
+@gpu
+@pytest.mark.parametrize("H,kvh,bs", [(7, 1, 16), (14, 2, 32), (32, 4, 64), (4, 4, 16), (16, 2, 128), (3, 1, 48), (2, 2, 16), (8, 1, 16)])
+@pytest.mark.parametrize("most", [2, 16])
+def test_short_runs_head_layouts_and_block_sizes(ops, H, kvh, bs, most):
+    _runs(ops, SHORT[0], [min(n, most) for n in SHORT[1]], 700, H, kvh, bs, seed=92)
+
+
+@gpu
+@pytest.mark.parametrize("spread,qmag,scale", [(60.0, 1.0, 128 ** -0.5), (0.0, 60.0, 128 ** -0.5), (10.0, 1e-3, 128 ** -0.5),
+                                               (3.0, 1.0, -0.1), (3.0, 1.0, 0.0), (80.0, 1e-4, 1.0)])
+def test_short_runs_magnitudes_and_scales(ops, spread, qmag, scale):
+    _runs(ops, *SHORT, 700, 28, 4, 16, seed=94, spread=spread, qmag=qmag, scale=scale)
+
+
+@gpu
+@pytest.mark.parametrize("ctx,new", [([20000], [4]), ([9000, 3, 40000], [11, 16, 5]), ([100] * 350, [12] * 350),
+                                     ([130, 0, 4000] * 110, [3, 4, 2] * 110)])
+def test_short_runs_cut_into_pieces_and_in_several_launches(ops, ctx, new):
+    _runs(ops, ctx, new, -1 if len(ctx) < 4 else 600, 14, 2, 16, seed=96)
+
+
+@gpu
+def test_short_runs_keep_nan_and_bad_blocks_to_their_own_rows(ops):
+    ctx, new = [60, 60, 60], [4, 4, 4]
+    codes, scales, table = _pool([64, 64, 64], -1, 1, 128, 16, seed=98)
+    codes.view(torch.uint8)[0, int(table[1, 3]), 15, 0, 5] = 0x7F            # the newest key of sequence 1: its last query alone
+    table[2, 1] = -1
+    codes, scales, table = codes.to(DEV), scales.to(DEV), table.to(DEV)
+    q = _rows((12, 7, 128), 99).bfloat16()
+    q[2, 4, 9] = math.inf
+    st = _status()
+    out = ops.swa_prefill_q8(q.to(DEV), codes[0], codes[1], scales[0], scales[1], table,
+                             torch.tensor([0, 4, 8, 12], dtype=torch.int32, device=DEV),
+                             torch.tensor(ctx, dtype=torch.int32, device=DEV), 4, window_left=-1, status=st)
+    bad = torch.isnan(out.float()).all(-1).cpu()
+    want = torch.zeros(12, 7, dtype=torch.bool)
+    want[2, 4], want[7] = True, True
+    assert st.item() == 2 and torch.equal(bad, want) and torch.isfinite(out.float()[~bad.to(DEV)]).all()
 
 
 @gpu
