@@ -986,6 +986,19 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
 static size_t partial_rows(bool runs) { return (size_t)kMaxPartials * (runs ? 4 : 1); }
 size_t workspace_bytes(int H, bool runs) { return cut_bytes() + partial_rows(runs) * H * (kD + 2) * sizeof(float); }
 
+int device_sms() {
+  static int sm_count[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int sms = dev >= 0 && dev < 64 ? sm_count[dev] : 0;
+  if (sms == 0) {
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (sms <= 0) sms = 148;
+    if (dev >= 0 && dev < 64) sm_count[dev] = sms;
+  }
+  return sms;
+}
+
 int stream_cache(const char* who, const Call& c, cudaStream_t st) {
   const bool runs = c.seq_lens == nullptr;
   Params P = {};
@@ -1000,15 +1013,7 @@ int stream_cache(const char* who, const Call& c, cudaStream_t st) {
   P.cut = (int4*)c.workspace;
   P.ws_o = (float*)((uint8_t*)c.workspace + cut_bytes());
   P.ws_ml = (float2*)(P.ws_o + partial_rows(runs) * c.H * kD);
-  static int sm_count[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  int sms = dev >= 0 && dev < 64 ? sm_count[dev] : 0;
-  if (sms == 0) {
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (sms <= 0) sms = 148;
-    if (dev >= 0 && dev < 64) sm_count[dev] = sms;
-  }
+  const int sms = device_sms();
   MapKey keys[2] = {MapKey{c.k_cache, c.kvh, c.num_blocks, c.block_size, c.cache_block_stride, c.kvh},
                     MapKey{c.v_cache, c.kvh, c.num_blocks, c.block_size, c.cache_block_stride, c.kvh}};
   for (MapKey& k : keys) { k.tok_stride = (int64_t)c.kvh * kD; k.rows = c.kvh; }

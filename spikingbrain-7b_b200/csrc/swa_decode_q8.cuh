@@ -19,6 +19,7 @@ struct Call {
   void* workspace; int32_t* status;
 };
 size_t workspace_bytes(int H, bool runs);
+int device_sms();                                        // multiprocessors of the current device
 int stream_cache(const char* who, const Call& c, cudaStream_t st);
 
 }  // namespace decode_q8

@@ -47,6 +47,8 @@ struct Params {
   int seq0;               // first sequence of this launch; its dense rows start at row 0
   int rows_per_seq;       // dense rows of a sequence, a multiple of 128
   int pairs;              // query tile pairs per sequence
+  int pairs_per_head;     // of the sequences of this launch
+  int split;              // pairs from here on are two CTAs' (of all heads, laid end to end)
   int max_query_len, H, G, bq, window_left; float scale_log2;   // >= 0: a negative scale's sign goes into q
   uint32_t q_sign;
   __nv_bfloat16* out; int64_t out_tok_stride; int32_t* status;
@@ -118,6 +120,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// one lane of a converged warp, always the same
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 // ---- 2. attention of the runs over the dense rows ----
 __global__ void __launch_bounds__(kThreads, 1)
 attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -132,17 +141,24 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kBarOff + 192);
   volatile uint8_t* abort_flag = smem + kBarOff + 208;
 
-  const int sl = blockIdx.x / P.pairs, s = P.seq0 + sl;
+  // pairs of tiles [0, split) are a CTA's each, the others two CTAs'
+  int item = blockIdx.x, tile = -1;
+  if (item >= P.split) {
+    tile = (item - P.split) & 1;
+    item = P.split + ((item - P.split) >> 1);
+  }
+  const int hk = item / P.pairs_per_head, kBQ = P.bq, G = P.G;
+  item -= hk * P.pairs_per_head;
+  const int sl = item / P.pairs, s = P.seq0 + sl;
   // later queries see more keys: they are launched first, so the long items do not start last
-  const int j = P.pairs - 1 - (int)(blockIdx.x - sl * P.pairs);
-  const int hk = blockIdx.y, kBQ = P.bq, G = P.G;
+  const int q0 = (P.pairs - 1 - (item - sl * P.pairs)) * 2 * kBQ + (tile == 1 ? kBQ : 0), most = tile < 0 ? 2 * kBQ : kBQ;
   const Keys ks = keys_of(P.query_start_loc, P.context_lens, s, P.window_left, P.max_query_len);
-  if (j * 2 * kBQ >= ks.n_q) return;   // whole CTA, before anything is allocated
-  const int nq_pair = ks.n_q - j * 2 * kBQ < 2 * kBQ ? ks.n_q - j * 2 * kBQ : 2 * kBQ;
+  if (q0 >= ks.n_q) return;            // whole CTA, before anything is allocated
+  const int nq_pair = ks.n_q - q0 < most ? ks.n_q - q0 : most;
   const bool has_b = nq_pair > kBQ;
-  const int qs = P.query_start_loc[s] + j * 2 * kBQ;       // row of the pair's first query
+  const int qs = P.query_start_loc[s] + q0;                // row of the pair's first query
   // in dense rows (row 0 = key ks.first): the last key of the pair's first query, the first key it sees, one past the last key
-  const int p0 = ks.n - ks.n_q + j * 2 * kBQ;
+  const int p0 = ks.n - ks.n_q + q0;
   const int lo = P.window_left < 0 || p0 <= P.window_left ? 0 : p0 - P.window_left;
   const int t_lo = lo / kTile, n_tiles = (p0 + nq_pair - 1) / kTile - t_lo + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -191,9 +207,12 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
   } else if (warp == kSoftmaxWarps + 2) {
     // ================================= MMA issuer =================================
+    // (with `lane == 0` in place of an elected lane every MMA was issued some forty cycles later, and this warp is on the way from
+    // one softmax to the next: 8192 queries 618 us)
+    const bool leader = elect_one();
     const uint32_t idesc_qk = instr_desc(0), idesc_pv = instr_desc(1);
     auto issue_s = [&](int X, int t) {     // S_X(t) = Q_X . K(t)^T
-      if (lane == 0) {
+      if (leader) {
         const uint32_t q_addr = sbase + kQOff + X * kOperandBytes;
         const uint32_t k_addr = sbase + kKOff + (t % kStagesK) * kOperandBytes;
 #pragma unroll
@@ -208,7 +227,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     // O_X += P_X(t) . V(t) for one half of the keys: steps of 16 keys, whose P is 8 columns of packed pairs at the head of
     // the 32 columns its scores came from
     auto issue_pv = [&](int X, int t, int half) {
-      if (lane == 0) {
+      if (leader) {
         const uint32_t v_addr = sbase + kVOff + (t % kStagesV) * kOperandBytes;
 #pragma unroll
         for (int k4 = 0; k4 < 4; ++k4) {
@@ -220,7 +239,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       __syncwarp();
     };
     auto commit = [&](uint32_t bar) {
-      if (lane == 0) umma_commit(bar);
+      if (leader) umma_commit(bar);
       __syncwarp();
     };
     auto k_full = [&](int t) { return mbar_wait_bounded(bar_kf + 8 * (t % kStagesK), (t / kStagesK) & 1) && !*abort_flag; };
@@ -533,7 +552,7 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
   const int64_t rows = y.rows_per_seq * y.group;
   const int bq = 128 / (H / kvh);
   const int pairs = (max_query_len + 2 * bq - 1) / (2 * bq);
-  if (rows > 2147483647LL || (int64_t)y.group * pairs > 2147483647LL || kvh > 65535 || y.group > 65535) {
+  if (rows > 2147483647LL || (int64_t)y.group * pairs * kvh > 1 << 30 || y.group > 65535) {
     set_error("sbk_swa_prefill_q8: grid or scratch too large");
     return SBK_E_ARG;
   }
@@ -556,6 +575,7 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     }
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
+  const int sms = decode_q8::device_sms();
   cudaStream_t st = (cudaStream_t)stream;
   Params P = {};
   P.q = (const __nv_bfloat16*)q; P.q_tok_stride = q_tok_stride;
@@ -575,7 +595,13 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     int rc = check_launch("sbk_swa_prefill_q8");
     if (rc != SBK_OK) return rc;
     P.seq0 = s0;
-    attend_kernel<<<dim3(n * pairs, kvh), kThreads, kSmemBytes, st>>>(P, maps[0], maps[1]);
+    // What is left for the last, partly filled round of CTAs takes one tile to a CTA if the SMs have room for twice as many: half
+    // the queries take less than a pair, though more than half of it
+    const int64_t total = (int64_t)n * pairs * kvh;
+    const int rest = (int)(total % sms);
+    P.pairs_per_head = n * pairs;
+    P.split = (int)(2 * rest <= sms ? total - rest : total);
+    attend_kernel<<<(unsigned)(2 * total - P.split), kThreads, kSmemBytes, st>>>(P, maps[0], maps[1]);
     rc = check_launch("sbk_swa_prefill_q8");
     if (rc != SBK_OK) return rc;
   }
