@@ -15,8 +15,16 @@
 //    the output's own rounding does), nothing has to be converted, and a tile of 128 keys is one copy per 64 dims.
 //    Tensor memory (512 columns): S_A / P_A [0,128), S_B / P_B [128,256), O_A [256,384), O_B [384,512). The softmax offset of a row
 //    moves only when its maximum has grown by more than 2^8, so O is rescaled in tensor memory almost only on the first tile.
-//    Roles (352 threads): warps 0-3 softmax / epilogue of tile A, 4-7 of tile B, 8 producer of the K ring, 9 of the V ring, 10 tensor
-//    memory and MMA issue. Every wait is bounded.
+//    Roles (384 threads): warps 0-3 softmax / epilogue of tile A, 4-7 of tile B, 8 producer of the K ring, 9 of the V ring, 10 tensor
+//    memory and MMA issue; 11 is there for its registers: the softmax warps hold a row's 128 scores at once, with what the last
+//    four warps give up. Every wait is bounded.
+// Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 578 us, 832 TFLOP/s of useful products (4 H D
+//    a visible pair; 0.50 of what a large matrix product reaches). A tile pair takes about 3900 cycles per 128 keys, of which the tensor
+//    core works 2050: the rest is the way from a tile's last P over the MMAs still to be issued to its next scores, and the
+//    softmax (two warps per scheduler, 1900 cycles alone, 2700 when A's and B's overlap). Tried and slower (us, the first form of this
+//    kernel being 624): scores read twice instead of held 598 against 581; tiles of 64 keys with two S buffers each 711; two
+//    threads per row 592; part of the exponentials as a polynomial 0 to 5 % more; P in halves 581; MMAs issued
+//    under `lane == 0` 618 against 598.
 #include <math.h>
 
 #include "kv_q8.cuh"
@@ -36,7 +44,10 @@ constexpr int kStagesK = 2, kStagesV = 3;
 constexpr int kQOff = 0, kKOff = 2 * kOperandBytes, kVOff = kKOff + kStagesK * kOperandBytes;
 constexpr int kBarOff = kVOff + kStagesV * kOperandBytes;
 constexpr int kSmemBytes = kBarOff + 256 + 1024;
-constexpr int kSoftmaxWarps = 8, kThreads = 32 * (kSoftmaxWarps + 3);
+constexpr int kSoftmaxWarps = 8, kThreads = 32 * (kSoftmaxWarps + 4);
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;   // registers of a thread after the block has started with 168
+static_assert(32 * kSoftmaxWarps * kSoftmaxRegs + (kThreads - 32 * kSoftmaxWarps) * kOtherRegs <= kThreads * 168,
+              "the registers of the warpgroups must fit what the block is launched with");
 constexpr int kTmemCols = 512, kOCol = 256;
 constexpr float kLog2e = 1.4426950408889634f, kNegBig = -1.0e30f;
 constexpr int64_t kScratchTarget = (int64_t)1 << 28;   // 256 MiB of dense rows at a time, or one sequence's where that is more
@@ -133,11 +144,11 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  // barriers: K ring full / empty, V ring full / empty; per tile: S ready, P ready (two halves of the keys); Q staged; all done.
+  // barriers: K ring full / empty, V ring full / empty; per tile: S ready, P ready (four quarters of the keys); Q staged; all done.
   // S and P of a tile take turns strictly, so one barrier each and phase t & 1.
   const uint32_t bar_kf = sbase + kBarOff, bar_ke = bar_kf + 8 * kStagesK;
   const uint32_t bar_vf = bar_ke + 8 * kStagesK, bar_ve = bar_vf + 8 * kStagesV;
-  const uint32_t bar_s = bar_ve + 8 * kStagesV, bar_p = bar_s + 16, bar_q = bar_p + 32, bar_done = bar_q + 8;
+  const uint32_t bar_s = bar_ve + 8 * kStagesV, bar_p = bar_s + 16, bar_q = bar_p + 64, bar_done = bar_q + 8;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kBarOff + 192);
   volatile uint8_t* abort_flag = smem + kBarOff + 208;
 
@@ -167,7 +178,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     for (int i = 0; i < kStagesK; ++i) { mbar_init(bar_kf + 8 * i, 1); mbar_init(bar_ke + 8 * i, 1); }
     for (int i = 0; i < kStagesV; ++i) { mbar_init(bar_vf + 8 * i, 1); mbar_init(bar_ve + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) mbar_init(bar_s + 8 * i, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(bar_p + 8 * i, 4);      // one arrival per warp of the tile
+    for (int i = 0; i < 8; ++i) mbar_init(bar_p + 8 * i, 4);      // one arrival per warp of the tile
     mbar_init(bar_q, kSoftmaxWarps);
     mbar_init(bar_done, 1);
     *abort_flag = 0;
@@ -183,104 +194,118 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == kSoftmaxWarps || warp == kSoftmaxWarps + 1) {
-    // ===== producers: one warp per ring, a tile is two copies of [128 rows][64 dims] =====
-    const int kind = warp - kSoftmaxWarps;
-    const int stages = kind ? kStagesV : kStagesK;
-    bool ok = true;
-    for (int t = 0; ok && t < n_tiles; ++t) {
-      const int slot = t % stages, use = t / stages;
-      const uint32_t bar_e = (kind ? bar_ve : bar_ke) + 8 * slot, bar_f = (kind ? bar_vf : bar_kf) + 8 * slot;
-      if (use > 0 && !mbar_wait_bounded(bar_e, (use - 1) & 1)) ok = false;
-      if (*abort_flag) ok = false;
-      if (!ok) break;
-      if (lane == 0) {
-        const uint32_t dst = sbase + (kind ? kVOff : kKOff) + slot * kOperandBytes;
-        const CUtensorMap* map = kind ? &map_v : &map_k;
-        const int row = sl * P.rows_per_seq + (t_lo + t) * kTile;
-        mbar_arrive_expect_tx(bar_f, kOperandBytes);
-        tma_load_3d(dst, map, 0, row, hk, bar_f);
-        tma_load_3d(dst + kPanelBytes, map, 64, row, hk, bar_f);
-      }
-      __syncwarp();
+  // everyone meets here, then the allocating warp returns the tensor memory
+  auto finish = [&]() {
+    if (*abort_flag) {
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies and MMAs in flight land
     }
-    if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
-  } else if (warp == kSoftmaxWarps + 2) {
-    // ================================= MMA issuer =================================
-    // (with `lane == 0` in place of an elected lane every MMA was issued some forty cycles later, and this warp is on the way from
-    // one softmax to the next: 8192 queries 618 us)
-    const bool leader = elect_one();
-    const uint32_t idesc_qk = instr_desc(0), idesc_pv = instr_desc(1);
-    auto issue_s = [&](int X, int t) {     // S_X(t) = Q_X . K(t)^T
-      if (leader) {
-        const uint32_t q_addr = sbase + kQOff + X * kOperandBytes;
-        const uint32_t k_addr = sbase + kKOff + (t % kStagesK) * kOperandBytes;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kPanelBytes + (k & 3) * 32;
-          umma_bf16(tmem + X * 128, smem_desc(q_addr + off, 16), smem_desc(k_addr + off, 16), idesc_qk, k > 0);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kSoftmaxWarps + 2) tmem_dealloc(tmem, kTmemCols);
+  };
+  if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kSoftmaxWarps || warp == kSoftmaxWarps + 1) {
+      // ===== producers: one warp per ring, a tile is two copies of [128 rows][64 dims] =====
+      const int kind = warp - kSoftmaxWarps;
+      const int stages = kind ? kStagesV : kStagesK;
+      bool ok = true;
+      for (int t = 0; ok && t < n_tiles; ++t) {
+        const int slot = t % stages, use = t / stages;
+        const uint32_t bar_e = (kind ? bar_ve : bar_ke) + 8 * slot, bar_f = (kind ? bar_vf : bar_kf) + 8 * slot;
+        if (use > 0 && !mbar_wait_bounded(bar_e, (use - 1) & 1)) ok = false;
+        if (*abort_flag) ok = false;
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t dst = sbase + (kind ? kVOff : kKOff) + slot * kOperandBytes;
+          const CUtensorMap* map = kind ? &map_v : &map_k;
+          const int row = sl * P.rows_per_seq + (t_lo + t) * kTile;
+          mbar_arrive_expect_tx(bar_f, kOperandBytes);
+          tma_load_3d(dst, map, 0, row, hk, bar_f);
+          tma_load_3d(dst + kPanelBytes, map, 64, row, hk, bar_f);
         }
-        umma_commit(bar_s + 8 * X);
+        __syncwarp();
       }
-      __syncwarp();
-    };
-    // O_X += P_X(t) . V(t) for one half of the keys: steps of 16 keys, whose P is 8 columns of packed pairs at the head of
-    // the 32 columns its scores came from
-    auto issue_pv = [&](int X, int t, int half) {
-      if (leader) {
-        const uint32_t v_addr = sbase + kVOff + (t % kStagesV) * kOperandBytes;
+      if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+    } else if (warp == kSoftmaxWarps + 2) {
+      // ================================= MMA issuer =================================
+      // (an elected lane: behind `lane == 0` every MMA was issued some forty cycles later)
+      const bool leader = elect_one();
+      const uint32_t idesc_qk = instr_desc(0), idesc_pv = instr_desc(1);
+      auto issue_s = [&](int X, int t) {     // S_X(t) = Q_X . K(t)^T
+        if (leader) {
+          const uint32_t q_addr = sbase + kQOff + X * kOperandBytes;
+          const uint32_t k_addr = sbase + kKOff + (t % kStagesK) * kOperandBytes;
 #pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const int k = 4 * half + k4;
-          umma_bf16_ts(tmem + kOCol + X * 128, tmem + X * 128 + 32 * (k >> 1) + 8 * (k & 1), smem_desc(v_addr + k * 2048, kPanelBytes),
-                       idesc_pv, (t > 0) || (k > 0));
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = (k >> 2) * kPanelBytes + (k & 3) * 32;
+            umma_bf16(tmem + X * 128, smem_desc(q_addr + off, 16), smem_desc(k_addr + off, 16), idesc_qk, k > 0);
+          }
+          umma_commit(bar_s + 8 * X);
         }
+        __syncwarp();
+      };
+      // O_X += P_X(t) . V(t) for a quarter of the keys: steps of 16 keys, whose P is 8 columns of packed pairs at the head of
+      // the 32 columns its scores came from
+      auto issue_pv = [&](int X, int t, int quarter) {
+        if (leader) {
+          const uint32_t v_addr = sbase + kVOff + (t % kStagesV) * kOperandBytes;
+#pragma unroll
+          for (int k4 = 0; k4 < 2; ++k4) {
+            const int k = 2 * quarter + k4;
+            umma_bf16_ts(tmem + kOCol + X * 128, tmem + X * 128 + 32 * (k >> 1) + 8 * (k & 1), smem_desc(v_addr + k * 2048, kPanelBytes),
+                         idesc_pv, (t > 0) || (k > 0));
+          }
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint32_t bar) {
+        if (leader) umma_commit(bar);
+        __syncwarp();
+      };
+      auto k_full = [&](int t) { return mbar_wait_bounded(bar_kf + 8 * (t % kStagesK), (t / kStagesK) & 1) && !*abort_flag; };
+      bool ok = mbar_wait_bounded(bar_q, 0) && k_full(0);
+      if (ok) {
+        tc_fence_after();
+        issue_s(0, 0);
+        if (has_b) issue_s(1, 0);
+        commit(bar_ke);
       }
-      __syncwarp();
-    };
-    auto commit = [&](uint32_t bar) {
-      if (leader) umma_commit(bar);
-      __syncwarp();
-    };
-    auto k_full = [&](int t) { return mbar_wait_bounded(bar_kf + 8 * (t % kStagesK), (t / kStagesK) & 1) && !*abort_flag; };
-    bool ok = mbar_wait_bounded(bar_q, 0) && k_full(0);
-    if (ok) {
-      tc_fence_after();
-      issue_s(0, 0);
-      if (has_b) issue_s(1, 0);
-      commit(bar_ke);
-    }
-    for (int t = 0; ok && t < n_tiles; ++t) {
-      const int vslot = t % kStagesV;
-      const bool more = t + 1 < n_tiles;
-      for (int X = 0; ok && X < (has_b ? 2 : 1); ++X) {
-        const bool last = X == (has_b ? 1 : 0);
-        // P_X(t), the first 64 keys and then the rest: the product of the first half runs while the threads work on the second;
-        // with the second S_X(t) has been read, so S_X(t + 1) may follow
-        ok = mbar_wait_bounded(bar_p + 16 * X, t & 1) && mbar_wait_bounded(bar_vf + 8 * vslot, (t / kStagesV) & 1);
-        if (!ok || *abort_flag) break;
-        tc_fence_after();
-        issue_pv(X, t, 0);
-        ok = mbar_wait_bounded(bar_p + 16 * X + 8, t & 1);
-        if (!ok || *abort_flag) break;
-        tc_fence_after();
-        issue_pv(X, t, 1);
-        if (last) commit(bar_ve + 8 * vslot);
-        if (more) {
-          if (X == 0) {
-            ok = k_full(t + 1);
+      for (int t = 0; ok && t < n_tiles; ++t) {
+        const int vslot = t % kStagesV;
+        const bool more = t + 1 < n_tiles;
+        for (int X = 0; ok && X < (has_b ? 2 : 1); ++X) {
+          const bool last = X == (has_b ? 1 : 0);
+          // P_X(t), 32 keys at a time: the product of a quarter runs while the threads work on the next; behind the last one
+          // S_X(t + 1) may take the place of P_X(t)
+          ok = mbar_wait_bounded(bar_vf + 8 * vslot, (t / kStagesV) & 1);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            ok = ok && mbar_wait_bounded(bar_p + 32 * X + 8 * c, t & 1) && !*abort_flag;
             if (!ok) break;
             tc_fence_after();
+            issue_pv(X, t, c);
           }
-          issue_s(X, t + 1);
-          if (last) commit(bar_ke + 8 * ((t + 1) % kStagesK));
+          if (!ok) break;
+          if (last) commit(bar_ve + 8 * vslot);
+          if (more) {
+            if (X == 0) {
+              ok = k_full(t + 1);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            issue_s(X, t + 1);
+            if (last) commit(bar_ke + 8 * ((t + 1) % kStagesK));
+          }
         }
+        if (*abort_flag) ok = false;
       }
-      if (*abort_flag) ok = false;
+      if (ok) commit(bar_done);
+      if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
     }
-    if (ok) commit(bar_done);
-    if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+    finish();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ====================== softmax / epilogue: one thread per row ======================
     const int X = warp >> 2;
     const int r = (warp & 3) * 32 + lane;        // row of the MMA tile = tensor-memory lane
@@ -319,32 +344,26 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         v_lo = v_lo < 0 ? 0 : v_lo;
         v_hi = v_hi > kTile ? kTile : v_hi;
         const bool full = __all_sync(0xffffffffu, v_lo == 0 && v_hi == kTile);   // the warp takes one path
-        // ---- first pass: the row maximum, 64 columns at a time ----
+        // ---- the row's scores and their maximum ----
+        uint32_t sr4[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_col + 32 * c, sr4[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_fence(sr4[c]);
         float both;
         {
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (full) {
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t s0[32], s1[32];
-            tmem_ld32_issue(s_col + 64 * hf, s0);
-            tmem_ld32_issue(s_col + 64 * hf + 32, s1);
-            tmem_ld_fence(s0); tmem_ld_fence(s1);
-            if (full) {
+            for (int i = 0; i < 32; i += 2)
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                mx[0] = fmax3(mx[0], __uint_as_float(s0[i]), __uint_as_float(s0[i + 1]));
-                mx[1] = fmax3(mx[1], __uint_as_float(s0[i + 2]), __uint_as_float(s0[i + 3]));
-                mx[2] = fmax3(mx[2], __uint_as_float(s1[i]), __uint_as_float(s1[i + 1]));
-                mx[3] = fmax3(mx[3], __uint_as_float(s1[i + 2]), __uint_as_float(s1[i + 3]));
-              }
-            } else {
+              for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], __uint_as_float(sr4[c][i]), __uint_as_float(sr4[c][i + 1]));
+          } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const int col = 64 * hf + i;
-                if (col >= v_lo && col < v_hi) mx[i & 1] = fmaxf(mx[i & 1], __uint_as_float(s0[i]));
-                if (col + 32 >= v_lo && col + 32 < v_hi) mx[2 + (i & 1)] = fmaxf(mx[2 + (i & 1)], __uint_as_float(s1[i]));
-              }
-            }
+            for (int i = 0; i < 32; ++i)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (32 * c + i >= v_lo && 32 * c + i < v_hi) mx[c] = fmaxf(mx[c], __uint_as_float(sr4[c][i]));
           }
           both = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         }
@@ -370,18 +389,14 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
             tmem_st32(o_col + 32 * c, orr);
           }
         }
-        // ---- second pass: probabilities in place of the scores, each half reported as soon as it is stored ----
+        // ---- probabilities in place of the scores, each quarter reported as soon as it is stored ----
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
         const f32x2 sc2 = pack2(P.scale_log2, P.scale_log2), nm2 = pack2(-m_s, -m_s);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          uint32_t sa[32], sb[32];
-          tmem_ld32_issue(s_col + 64 * hf, sa);
-          tmem_ld32_issue(s_col + 64 * hf + 32, sb);
-          tmem_ld_fence(sa); tmem_ld_fence(sb);
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
-            uint32_t (&sr)[32] = cc ? sb : sa;
+            uint32_t (&sr)[32] = sr4[2 * hf + cc];
             const int col0 = 64 * hf + 32 * cc;
             uint32_t ph[16];               // packed bf16 pairs, key 2e in the low half
             if (fast) {
@@ -414,11 +429,11 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
               }
             }
             tmem_st16(s_col + col0, ph);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p + 32 * X + 16 * hf + 8 * cc);
           }
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_p + 16 * X + 8 * hf);
         }
         l_run = l_run * alpha + (ls[0] + ls[1]) + (ls[2] + ls[3]);
       }
@@ -447,20 +462,13 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       }
     }
     if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+    finish();
   }
-
-  // ---- everyone meets here, then the allocating warp returns the tensor memory ----
-  if (*abort_flag) {
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);   // copies and MMAs in flight land
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == kSoftmaxWarps + 2) tmem_dealloc(tmem, kTmemCols);
 }
 
 // Runs of at most kFew queries go through the kernel of the single tokens, which reads the cache once for four queries and
-// expands nothing. Measured there against here, us, window 4096 on 8190 cached tokens: 64 runs of 4 109 / 381, of 8 187 / 375,
-// of 16 336 / 384, of 20 407 / 413; 256 of 16 1162, of 20 1495 / 1391; 8 of 16 66 / 103; 1 of 16 32 / 87, of 32 40 / 90.
+// expands nothing. Measured there against here, us, window 4096 on 8190 cached tokens: 64 runs of 8 187 / 375, of 16 336 / 384, of
+// 20 407 / 390; 256 runs of 16 1160, of 20 1495 / 1346; 8 of 20 76 / 89; one of 20 34 / 70.
 constexpr int kFew = 16;
 static bool few_queries(int max_query_len, int kvh) { return max_query_len <= kFew && (kvh == 1 || kvh == 2 || kvh == 4); }
 
@@ -571,6 +579,14 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     const cudaError_t e = cudaFuncSetAttribute(attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) {
       set_error("sbk_swa_prefill_q8: cannot opt in to %d bytes of shared memory: %s", kSmemBytes, cudaGetErrorString(e));
+      return SBK_E_LAUNCH;
+    }
+    // (a split of the registers that the launch does not bring would wait forever)
+    cudaFuncAttributes fa;
+    const cudaError_t ea = cudaFuncGetAttributes(&fa, attend_kernel);
+    if (ea != cudaSuccess ||
+        fa.numRegs * kThreads < 32 * kSoftmaxWarps * kSoftmaxRegs + (kThreads - 32 * kSoftmaxWarps) * kOtherRegs) {
+      set_error("sbk_swa_prefill_q8: the kernel was built with %d registers per thread", ea == cudaSuccess ? fa.numRegs : -1);
       return SBK_E_LAUNCH;
     }
     if (dev >= 0 && dev < 64) configured[dev] = true;
