@@ -19,7 +19,7 @@
 //    memory and MMA issue; 11 is there for its registers: the softmax warps hold a row's 128 scores at once, with what the last
 //    four warps give up. Every wait is bounded.
 // Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 578 us, 832 TFLOP/s of useful products (4 H D
-//    a visible pair; 0.50 of what a large matrix product reaches). A tile pair takes about 3900 cycles per 128 keys, of which the tensor
+//    a visible pair; 0.50 of what a large matrix product reaches). A tile pair takes about 4000 cycles per 128 keys, of which the tensor
 //    core works 2050: the rest is the way from a tile's last P over the MMAs still to be issued to its next scores, and the
 //    softmax (two warps per scheduler, 1900 cycles alone, 2700 when A's and B's overlap). Tried and slower (us, the first form of this
 //    kernel being 624): scores read twice instead of held 598 against 581; tiles of 64 keys with two S buffers each 711; two
