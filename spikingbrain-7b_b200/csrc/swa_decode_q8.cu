@@ -388,7 +388,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     };
 
     if (whole) {
-      if (lane == 0) P.cut[me] = kNotCut;      // (a whole batch has as many items as CTAs at least: entries are per CTA)
+      if (lane == 0) P.cut[me] = kNotCut;      // (entries per item, where they are that, are fewer than CTAs)
       for (int b = me; b < P.B && !aborted; b += n_cta) {
         if (tops[b] < 0) continue;
         const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left);
@@ -935,14 +935,17 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int n_ctas = C::kCtasPerSm * (sms < kMaxSms ? sms : kMaxSms);
-  for (int64_t b0 = 0; b0 < items; b0 += kMaxSeqs) {
+  const int64_t width = (int64_t)P0.max_blocks * P0.block_size, seen = (int64_t)P0.window_left + kCap;
+  const int64_t vis = P0.window_left < 0 || width < seen ? width : seen;
+  const int64_t per_item = vis / kUnit + 2 + C::kItemCost;     // units of an item, at the most
+  int64_t step = 2147483647LL / per_item;                      // the units of a launch are counted in 32 bits
+  step = step < 1 ? 1 : (step < kMaxSeqs ? step : kMaxSeqs);
+  for (int64_t b0 = 0; b0 < items; b0 += step) {
     Params P = P0;
     P.item0 = (int)b0;
-    P.B = items - b0 < kMaxSeqs ? (int)(items - b0) : kMaxSeqs;
+    P.B = (int)(items - b0 < step ? items - b0 : step);
     // no more CTAs than there can be units of work
-    const int64_t width = (int64_t)P.max_blocks * P.block_size, seen = (int64_t)P.window_left + kCap;
-    const int64_t vis = P.window_left < 0 || width < seen ? width : seen;
-    const int64_t most = (int64_t)P.B * (vis / kUnit + 2 + C::kItemCost);
+    const int64_t most = (int64_t)P.B * per_item;
     int grid = (int)(most < n_ctas ? most : n_ctas);
     // a batch between one and two items per SM: one CTA each, so that every SM has work either way of cutting (four queries
     // to an item are bound by instructions, not by the copies that a lone CTA can keep up: there both CTAs of an SM share)

@@ -862,6 +862,8 @@ def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         n = _decode_q8_workspace_bytes(B, H, d)
         workspace = q.new_empty((n,), dtype=torch.uint8)
     else:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         n = workspace.numel() * workspace.element_size()
     _call_on(dev, "sbk_swa_decode_q8", q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
              v_scale.data_ptr(), block_tables.data_ptr(), max_blocks, seq_lens.data_ptr(), B, H, kvh, d, nb, bs, cs, ss,
@@ -905,6 +907,8 @@ def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if workspace is None and n_seqs:
         workspace = swa_prefill_q8_workspace(n_seqs, max_query_len, max_blocks, kvh, d, q.device, block_size=bs,
                                              window_left=window_left)
+    elif workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     _call_on(dev, "sbk_swa_prefill_q8", _ptr(q), q.stride(0) if T > 1 else H * d, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
              _ptr(v_scale), _ptr(block_tables), max_blocks, _ptr(query_start_loc), _ptr(context_lens), n_seqs,
              max_query_len, H, kvh, d, nb, bs, cs, ss, window_left, d ** -0.5 if scale is None else float(scale),

@@ -456,6 +456,24 @@ def test_decode_strided_rows_and_workspace_of_the_caller(ops):
 
 
 @gpu
+def test_attention_refuses_a_workspace_with_gaps_or_too_small(ops):
+    codes, scales, table = (t.to(DEV) for t in _pool([40], -1, 1, 128, 16, seed=86))
+    q = _rows((1, 7, 128), 87).bfloat16().to(DEV)
+    one = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    n = ops.swa_decode_q8_workspace(1, 7, 128, DEV).numel()
+    gaps = torch.empty(n, 2, dtype=torch.uint8, device=DEV)[:, 0]
+    spread = torch.empty(1, dtype=torch.uint8, device=DEV).expand(1 << 28)
+    for ws in (gaps, spread):
+        with pytest.raises(ValueError, match="contiguous"):
+            ops.swa_decode_q8(q, *codes, *scales, table, one(40), window_left=-1, workspace=ws)
+        with pytest.raises(ValueError, match="contiguous"):
+            ops.swa_prefill_q8(q, *codes, *scales, table, one(0, 1), one(39), 1, window_left=-1, workspace=ws)
+    small = torch.empty(n - 16, dtype=torch.uint8, device=DEV)
+    with pytest.raises(RuntimeError):
+        ops.swa_decode_q8(q, *codes, *scales, table, one(40), window_left=-1, workspace=small)
+
+
+@gpu
 def test_decode_bad_block_is_reported_and_contained(ops):
     lens = [300, 300, 300]
     codes, scales, table = _pool(lens, -1, 4, 128, 16, seed=32)
@@ -585,7 +603,7 @@ def test_short_runs_magnitudes_and_scales(ops, spread, qmag, scale):
 
 @gpu
 @pytest.mark.parametrize("ctx,new", [([20000], [4]), ([9000, 3, 40000], [11, 16, 5]), ([100] * 350, [12] * 350),
-                                     ([130, 0, 4000] * 110, [3, 4, 2] * 110)])
+                                     ([130, 0, 4000] * 110, [3, 4, 2] * 110), ([500] * 283, [4] * 283)])
 def test_short_runs_cut_into_pieces_and_in_several_launches(ops, ctx, new):
     _runs(ops, ctx, new, -1 if len(ctx) < 4 else 600, 14, 2, 16, seed=96)
 
