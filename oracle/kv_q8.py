@@ -1,7 +1,7 @@
 """The 8-bit K/V cache in 64 bits: the format by its definition (a search over exponents, the table of the 256 codes)
 and attention over the values it stands for, with the error a kernel may make on the way. Test infrastructure."""
 import math
-from typing import List, Tuple
+from typing import List, NamedTuple, Optional, Tuple
 
 import torch
 
@@ -46,15 +46,33 @@ def quantise(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return code.to(torch.uint8), (e + 127).to(torch.uint8)
 
 
-def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor, scale: float):
-    """One sequence in float64: q [m, H, D], k and v [n, kvh, D] (values), seen [m, n]. Returns (out [m, H, D], lse [m, H],
-    err_out [m, H, D], err_lse [m, H]); the last two bound what a kernel may add before it rounds the output:
-      * scores: the query as two 4-bit pieces relative to its largest value loses at most 2^-18 of that value per product
-        (one piece in 16 bits loses less), and fp32 sums of D products 2^-20 of the sum of magnitudes;
+class Weights(NamedTuple):
+    """How a kernel holds the softmax weights for the product with V: what a weight may be off by relative to itself, and relative to
+    the largest weight (times the scale of its V row) of its query."""
+    step: float
+    floor: float
+    adds: int           # products that enter the sums of one step of 16 keys
+
+
+# One number in fp16 (half a step: 2^-11). The largest one of a query is at least 2^6 when its offset is chosen, so half of
+# fp16's smallest step, 2^-25, is 2^-31 of it at the most.
+FP16 = Weights(2.0 ** -11, 2.0 ** -31, 17)
+# Two bf16 numbers: the first is off by 2^-8 of the weight, the second by 2^-8 of that rest. No floor (bf16 has fp32's exponents).
+TWO_BF16 = Weights(2.0 ** -16, 0.0, 34)
+
+
+def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor, scale: float, weights: Optional[Weights] = None):
+    """One sequence in float64: q [m, H, D], k and v [n, kvh, D] (values), seen [m, n]. A key that a query does not see has no
+    part in its row, whatever it holds. Returns (out [m, H, D], lse [m, H], err_out [m, H, D], err_lse [m, H]); the last two
+    bound what a kernel may add before it rounds the output. With `weights`:
+      * scores: the query loses nothing. A matrix instruction adds 16 products and the sum so far, each cut at 2^-24 of the
+        largest; eight of them make a score: 8 * 17 * 2^-24, under 2^-16.9 of the sum of magnitudes;
       * a score off by d moves every weight by at most 2 d of itself (numerator and normaliser);
-      * probabilities as two 4-bit pieces are off by at most 2^-4 * 2^-4 of themselves, and by 2^-22 of the largest
-        (probability * scale of its V row) where they are too small for the pieces; a code is at most 448;
-      * exponentials, fp32 sums and the division: 2^-18."""
+      * weights: their rounding, above;
+      * the sums over the keys, cut in the same way, a step for every 16 keys: n / 16 * adds * 2^-24;
+      * exponentials, the normaliser and the division: 2^-18.
+    Without, a wider bound that also holds for query and weights as two 4-bit pieces each: 2^-18 of the query's largest value
+    per product, 2^-8 of every weight, and n * 2^-22 of the largest."""
     m, H, D = q.shape
     n, kvh, _ = k.shape
     G = H // kvh
@@ -65,15 +83,24 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor
     p = torch.where(seen[:, None, None, :], torch.exp(s - lse.clamp_min(-1e300).unsqueeze(-1)), 0.0)
     any_seen = seen.any(-1)
     kk = torch.where(seen.any(0)[:, None, None], k, 0.0)
-    vv = torch.where(seen.any(0)[:, None, None], v, 0.0)
+    odd = torch.isnan(v) & seen.any(0)[:, None, None]
+    vv = torch.where(seen.any(0)[:, None, None] & ~odd, v, 0.0)
     out = torch.einsum("mhgn,nhd->mhgd", p, vv)
     mag = torch.einsum("mhgd,nhd->mhgn", q.abs(), kk.abs()) * abs(scale)
-    floor = q.abs().amax(-1, keepdim=True) * kk.abs().sum(-1).t()[None, :, None, :] * abs(scale)
-    d = (2.0 ** -18 * floor + 2.0 ** -20 * mag).masked_fill(~seen[:, None, None, :], 0.0).amax(-1)
+    hidden = ~seen[:, None, None, :]
     A = torch.einsum("mhgn,nhd->mhgd", p, vv.abs())
     top = 2.0 * vv.abs().amax(-1)                                # at least 448 * 2^e of the row
-    small = n * 2.0 ** -22 * (p * top.t()[None, :, None, :]).amax(-1)
-    err = A * (2 * d + 2.0 ** -8 + 2.0 ** -18).unsqueeze(-1) + small.unsqueeze(-1)
+    most = (p * top.t()[None, :, None, :]).amax(-1)
+    if weights is None:
+        floor = q.abs().amax(-1, keepdim=True) * kk.abs().sum(-1).t()[None, :, None, :] * abs(scale)
+        d = (2.0 ** -18 * floor + 2.0 ** -20 * mag).masked_fill(hidden, 0.0).amax(-1)
+        err = A * (2 * d + 2.0 ** -8 + 2.0 ** -18).unsqueeze(-1) + (n * 2.0 ** -22 * most).unsqueeze(-1)
+    else:
+        d = (8 * 17 * 2.0 ** -24 * mag).masked_fill(hidden, 0.0).amax(-1)
+        sums = -(-n // 16) * weights.adds * 2.0 ** -24
+        err = A * (2 * d + weights.step + sums + 2.0 ** -18).unsqueeze(-1) + (n * weights.floor * most).unsqueeze(-1)
+    hit = torch.einsum("mn,nhd->mhd", seen.double(), odd.double()) > 0
+    out = out.masked_fill(hit.unsqueeze(2), math.nan)            # a NaN reaches its own dim of the queries that see it
     zero = ~any_seen[:, None, None]
     out = torch.where(zero.unsqueeze(-1), 0.0, out)
     err_lse = d + 2.0 ** -18 + 2.0 ** -22 * lse.abs().clamp(max=1e300)
@@ -89,13 +116,14 @@ def window_values(codes: torch.Tensor, scale: torch.Tensor, table: torch.Tensor,
     return values(codes.view(torch.uint8)[blk, t % bs], scale[blk, :, t % bs])
 
 
-def decode(q, codes, scales, table, lens: List[int], window_left: int, scale: float):
+def decode(q, codes, scales, table, lens: List[int], window_left: int, scale: float, weights: Optional[Weights] = None):
     """codes [2, ...], scales [2, ...]; q [B, H, D] -> the four tensors of attend, rows stacked."""
     return runs(q, codes, scales, table, [max(0, n - 1) for n in lens], [min(1, n) for n in lens], window_left, scale,
-                one_row_each=True)
+                one_row_each=True, weights=weights)
 
 
-def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: int, scale: float, one_row_each=False):
+def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: int, scale: float, one_row_each=False,
+         weights: Optional[Weights] = None):
     """Runs of queries: sequence s owns the next new[s] rows of q, behind ctx[s] cached tokens."""
     H, D = q.shape[1:]
     dev = q.device
@@ -115,6 +143,6 @@ def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: i
             qp = torch.arange(c + i, c + i + m, device=dev)[:, None]
             kp = torch.arange(lo, c + n, device=dev)[None]
             seen = (kp <= qp) & ((kp >= qp - window_left) if window_left >= 0 else (kp >= 0))
-            res.append(attend(q[row + i:row + i + m], k, v, seen, scale))
+            res.append(attend(q[row + i:row + i + m], k, v, seen, scale, weights))
         row += n
     return tuple(torch.cat([r[j] for r in res]) for j in range(4))

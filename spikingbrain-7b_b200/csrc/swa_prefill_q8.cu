@@ -11,16 +11,18 @@
 //        tensor core:  S_A(0) S_B(0) | P_A(0).V S_A(1) | P_B(0).V S_B(1) | ...
 //        warps 0-3  :  softmax A(0)  |                 | softmax A(1)    ...
 //        warps 4-7  :                | softmax B(0)    |                 ...
-//    Unlike there P and V are bf16 (a V row may have any exponent, which fp16 does not hold; P loses 2^-9 of itself, half of what
-//    the output's own rounding does), nothing has to be converted, and a tile of 128 keys is one copy per 64 dims.
+//    Unlike there V is bf16 (a V row may have any exponent, which fp16 does not hold), and P goes in as a bf16 head and a bf16 remainder,
+//    two products, so that it loses 2^-16 of itself (the head alone loses 2^-8, as much as the output's own rounding: mean relative
+//    error 1.6e-3 against 64 bits, over the 1e-3 that the framework's attention kernels keep). Nothing has to be converted, and a tile of
+//    128 keys is one copy per 64 dims.
 //    Tensor memory (512 columns): S_A / P_A [0,128), S_B / P_B [128,256), O_A [256,384), O_B [384,512). The softmax offset of a row
 //    moves only when its maximum has grown by more than 2^8, so O is rescaled in tensor memory almost only on the first tile.
 //    Roles (384 threads): warps 0-3 softmax / epilogue of tile A, 4-7 of tile B, 8 producer of the K ring, 9 of the V ring, 10 tensor
 //    memory and MMA issue; 11 is there for its registers: the softmax warps hold a row's 128 scores at once, with what the last
 //    four warps give up. Every wait is bounded.
-// Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 578 us, 832 TFLOP/s of useful products (4 H D
-//    a visible pair; 0.50 of what a large matrix product reaches). A tile pair takes about 4000 cycles per 128 keys, of which the tensor
-//    core works 2050: the rest is the way from a tile's last P over the MMAs still to be issued to its next scores, and the
+// Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 725 us, 664 TFLOP/s of useful products (4 H D
+//    a visible pair; with the heads of P alone it took 578). Then a tile pair took about 4000 cycles per 128 keys, of which the tensor
+//    core worked 2050: the rest is the way from a tile's last P over the MMAs still to be issued to its next scores, and the
 //    softmax (two warps per scheduler, 1900 cycles alone, 2700 when A's and B's overlap). Tried and slower (us, the first form of this
 //    kernel being 624): scores read twice instead of held 598 against 581; tiles of 64 keys with two S buffers each 711; two
 //    threads per row 592; part of the exponentials as a polynomial 0 to 5 % more; P in halves 581; MMAs issued
@@ -245,16 +247,18 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         }
         __syncwarp();
       };
-      // O_X += P_X(t) . V(t) for a quarter of the keys: steps of 16 keys, whose P is 8 columns of packed pairs at the head of
-      // the 32 columns its scores came from
+      // O_X += P_X(t) . V(t) for a quarter of the keys: steps of 16 keys, whose P is 8 columns of packed pairs (heads) at the
+      // beginning of the 32 columns its scores came from, and 8 of remainders 16 columns further
       auto issue_pv = [&](int X, int t, int quarter) {
         if (leader) {
           const uint32_t v_addr = sbase + kVOff + (t % kStagesV) * kOperandBytes;
 #pragma unroll
           for (int k4 = 0; k4 < 2; ++k4) {
             const int k = 2 * quarter + k4;
-            umma_bf16_ts(tmem + kOCol + X * 128, tmem + X * 128 + 32 * (k >> 1) + 8 * (k & 1), smem_desc(v_addr + k * 2048, kPanelBytes),
-                         idesc_pv, (t > 0) || (k > 0));
+            const uint32_t p_addr = tmem + X * 128 + 32 * quarter + 8 * k4;
+            const uint64_t vd = smem_desc(v_addr + k * 2048, kPanelBytes);
+            umma_bf16_ts(tmem + kOCol + X * 128, p_addr, vd, idesc_pv, (t > 0) || (k > 0));
+            umma_bf16_ts(tmem + kOCol + X * 128, p_addr + 16, vd, idesc_pv, 1u);
           }
         }
         __syncwarp();
@@ -398,7 +402,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           for (int cc = 0; cc < 2; ++cc) {
             uint32_t (&sr)[32] = sr4[2 * hf + cc];
             const int col0 = 64 * hf + 32 * cc;
-            uint32_t ph[16];               // packed bf16 pairs, key 2e in the low half
+            uint32_t ph[32];               // packed bf16 pairs, key 2e in the low half: [0, 16) heads, [16, 32) remainders
             if (fast) {
               f32x2 la = 0ull, lb = 0ull;
 #pragma unroll
@@ -409,8 +413,8 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                 const float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
                 la = fadd2(la, pack2(e0, e1));
                 lb = fadd2(lb, pack2(e2, e3));
-                ph[i >> 1] = pack_bf16x2(e0, e1);
-                ph[(i >> 1) + 1] = pack_bf16x2(e2, e3);
+                split_bf16x2(e0, e1, ph[i >> 1], ph[16 + (i >> 1)]);
+                split_bf16x2(e2, e3, ph[(i >> 1) + 1], ph[17 + (i >> 1)]);
               }
               float a0, a1, b0, b1;
               unpack2(la, a0, a1);
@@ -425,10 +429,10 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                 if (col0 + i + 1 < v_lo || col0 + i + 1 >= v_hi) pb = 0.f;
                 ls[i & 3] += pa;
                 ls[(i + 1) & 3] += pb;
-                ph[i >> 1] = pack_bf16x2(pa, pb);
+                split_bf16x2(pa, pb, ph[i >> 1], ph[16 + (i >> 1)]);
               }
             }
-            tmem_st16(s_col + col0, ph);
+            tmem_st32(s_col + col0, ph);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
