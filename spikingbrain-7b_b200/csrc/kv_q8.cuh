@@ -10,7 +10,8 @@
 // own: what is stored for a token depends on that token alone, not on what else was written to its block, in which
 // order, or in how many calls.
 //   inf and NaN become the NaN code; finite magnitudes above 448 * 2^kMaxExp saturate; an all-zero row takes kMinExp.
-//   The range [-64, 63] keeps every product of a K or V value with the 2^+-64 of another row inside fp32.
+//   The range [-64, 63] keeps every product of a K or V value with the 2^+-64 of another row inside fp32 (not every product of
+//   two such scales: the attention kernels multiply by one after the other).
 #pragma once
 
 #include <cuda_fp16.h>

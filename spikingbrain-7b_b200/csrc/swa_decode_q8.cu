@@ -679,7 +679,8 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
               unpack2(fadd2(pack2(sc[n][h][i], sc[n][h][i + 1]), nm), x, y);
               const f32x2 p = pack2(fast_exp2(x), fast_exp2(y));
               sum = fadd2(sum, p);
-              unpack2(fmul2(p, fmul2(r2, pack2(ve[h][i >> 1], ve[h][i >> 1]))), w[h][i], w[h][i + 1]);
+              // (in this order: 2^-r is up to 2^70, 2^ev up to 2^63, and a weight of zero must not meet their product)
+              unpack2(fmul2(fmul2(p, r2), pack2(ve[h][i >> 1], ve[h][i >> 1])), w[h][i], w[h][i + 1]);
               wtop = tc5::fmax3(wtop, w[h][i], w[h][i + 1]);
             }
           unpack2(sum, ps[0], ps[1]);

@@ -62,3 +62,42 @@ def test_long_runs_hold_their_weights_in_more_bits_than_the_output(ops, ctx, new
     want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=_weights_of(new))
     _check(out, None, want)
     assert mean_rel(out.float(), want[0].bfloat16().float()) <= MEAN_REL
+
+
+# ------------------------------------------------------------------------------------- the ends of the exponents' range
+def _row(codes, scales, table, which, seq, tok, head):
+    """The codes [D] of a token's row of K (0) or V (1), and the place of its exponent byte."""
+    bs = codes.shape[2]
+    blk = int(table[seq, tok // bs])
+    return codes.view(torch.uint8)[which, blk, tok % bs, head], (which, blk, head, tok % bs)
+
+
+@gpu
+@pytest.mark.parametrize("new", [None, 2, 3, 4, 16, 40])
+@pytest.mark.parametrize("exponent", [57, 58, 63])
+@pytest.mark.parametrize("peaked", [False, True])
+def test_an_empty_v_row_beside_the_largest_ones(ops, new, exponent, peaked):
+    """Token 0 holds zeros (the smallest exponent), the others V rows of the largest. Queries that see token 0 alone, or whose
+    softmax leaves nothing for the others, give zeros; the others finite values."""
+    H, kvh, n = 28, 4, new or 1
+    ctx = [0, 21]
+    lens = [2, 22] if new is None else [c + n for c in ctx]
+    codes, scales, table = _pool(lens, -1, kvh, 128, 16, seed=210, spread=0.5, n_new=[n, n])
+    g = torch.Generator().manual_seed(211)
+    u = torch.where(torch.rand(128, generator=g) < 0.5, -1.0, 1.0)
+    for s, L in enumerate(lens):
+        for h in range(kvh):
+            for t in range(L):
+                row, at = _row(codes, scales, table, 1, s, t, h)
+                if t == 0:
+                    row.zero_()
+                    key, key_at = _row(codes, scales, table, 0, s, 0, h)
+                    key.copy_(u.to(torch.float8_e4m3fn).view(torch.uint8))
+                    scales[key_at] = 127
+                scales[at] = 63 if t == 0 else 127 + exponent
+    q = torch.randn(2 * n, H, 128, generator=g)
+    q = ((60.0 * u).expand(2 * n, H, 128) if peaked else q).bfloat16().contiguous()
+    out = _attend(ops, q, codes, scales, table, lens if new is None else ctx, None if new is None else [n, n], -1)
+    dev = [t.to(DEV) for t in (q, codes, scales, table)]
+    want = ref.decode(*dev, lens, -1, SCALE, ref.FP16) if new is None else ref.runs(*dev, ctx, [n, n], -1, SCALE, weights=_weights_of([n]))
+    _check(out, None, want)
