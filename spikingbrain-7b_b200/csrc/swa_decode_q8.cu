@@ -13,8 +13,8 @@
 // Products. Both run on mma.sync m16n8k16 in fp16, the codes converted in registers on their way into the A operand (exact, two codes
 //   per instruction), K and V taking the 16-row side and the query heads of a kv group (at most eight) the other:
 //       S^T[16 tokens, 8 heads] = K . Q^T            O^T[16 dims, 8 heads] = V^T . W^T
-//   q is scaled by the power of two that takes its largest value under 448: a bf16 number is an fp16 number then (elements below
-//   2^-23 of the largest lose bits no score shows). Feeding the codes to the e4m3 MMA as they are, with query and
+//   q is scaled by the power of two that takes its largest value to (2^13.8, 2^14.8]: a bf16 number is an fp16 number then, down to 2^-30
+//   of the largest (below, an element is off by 2^-38 of the largest at the most). Feeding the codes to the e4m3 MMA as they are, with query and
 //   probabilities split into two 4-bit parts, takes three times the instructions: the compiler expands that MMA into
 //   conversions of both operands and two fp16 ones (64 mixed sequences: 72 us against 64 in fp16, the rest alike).
 // Softmax. The V scale belongs to the probability's exponent: with an offset m per head the normaliser sums p_j = 2^(s_j - m), and
@@ -520,7 +520,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = q8::row_exponent(top);
-        const float inv = q8::pow2i(-e), mine = P.scale_log2 * q8::pow2i(e);
+        const float inv = q8::pow2i(6 - e), mine = P.scale_log2 * q8::pow2i(e - 6);   // 448 * 2^6 = 28672: inside fp16
 #pragma unroll
         for (int i = 0; i < 16; ++i)         // (an infinity stays one: the head's scores are NaN or infinite)
           w[i] = pack_f16x2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv);

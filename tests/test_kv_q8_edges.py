@@ -101,3 +101,22 @@ def test_an_empty_v_row_beside_the_largest_ones(ops, new, exponent, peaked):
     dev = [t.to(DEV) for t in (q, codes, scales, table)]
     want = ref.decode(*dev, lens, -1, SCALE, ref.FP16) if new is None else ref.runs(*dev, ctx, [n, n], -1, SCALE, weights=_weights_of([n]))
     _check(out, None, want)
+
+
+@gpu
+@pytest.mark.parametrize("new", [None, 2, 4, 40])
+def test_small_elements_of_a_query_count_where_its_large_ones_meet_zeros(ops, new):
+    """Scores made by elements 2^-27 of the query's largest, whose keys hold zero in the largest one's place."""
+    H, kvh, n = 14, 2, new or 1
+    ctx, lens = [50, 7], [50 + n, 7 + n]
+    codes, scales, table = _pool(lens, -1, kvh, 128, 16, seed=214, spread=0.0, n_new=[n, n])
+    codes.view(torch.uint8)[0, :, :, :, 0] = 0
+    scales[0] = 127 + 19
+    g = torch.Generator().manual_seed(215)
+    q = torch.randn(2 * n, H, 128, generator=g) * 2.0 ** -27
+    q[..., 0] = 1.0
+    q = q.bfloat16()
+    out = _attend(ops, q, codes, scales, table, lens if new is None else ctx, None if new is None else [n, n], -1)
+    dev = [t.to(DEV) for t in (q, codes, scales, table)]
+    want = ref.decode(*dev, lens, -1, SCALE, ref.FP16) if new is None else ref.runs(*dev, ctx, [n, n], -1, SCALE, weights=_weights_of([n]))
+    _check(out, None, want)
