@@ -75,7 +75,8 @@ struct Cfg {
   static constexpr int kQueryOff = kScaleOff + kStages * kScaleBytes;   // [warp][query][4][lane] 16 bytes: steps 2j and 2j + 1
   static constexpr int kStateOff = kQueryOff + (kShare ? kWarps * NQ * 2048 : 0);   // [warp][query][t] (m, m, 2^-r, 2^-r)
   static constexpr int kFactorOff = kStateOff + (kShare ? kWarps * NQ * 64 : 0);    // [warp][query][head] what a product is scaled by
-  static constexpr int kInfoOff = kFactorOff + (kShare ? kWarps * NQ * 32 : 0);
+  static constexpr int kNanOff = kFactorOff + (kShare ? kWarps * NQ * 32 : 0);      // [warp][query] dims of the output that are NaN, a bit each
+  static constexpr int kInfoOff = kNanOff + (NQ > 1 ? kWarps * NQ * 16 : 0);
   static constexpr int kPreOff = kInfoOff + kStages * (int)sizeof(StageInfo);
   static constexpr int kLensOff = kPreOff + (kMaxSeqs + 4) * 4;
   static constexpr int kCntOff = kLensOff + kMaxSeqs * 4;
@@ -479,6 +480,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   uint4* const q_sh = reinterpret_cast<uint4*>(smem + C::kQueryOff) + warp * NQ * 128 + lane;
   float4* const st_sh = reinterpret_cast<float4*>(smem + C::kStateOff) + warp * NQ * 4 + t;
   float* const fa_sh = reinterpret_cast<float*>(smem + C::kFactorOff) + warp * NQ * 8;
+  uint32_t* const nan_sh = reinterpret_cast<uint32_t*>(smem + C::kNanOff) + warp * NQ * 4;
   auto load_state = [&](int n) {                   // of query n, to the registers of its slot
     if constexpr (C::kShare) {
       const float4 x = st_sh[4 * n];
@@ -496,7 +498,10 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     const uint32_t stage = ring + s * kStageBytes;
 
     if (__builtin_expect(si.flags & kFirst, 0)) {
-      if constexpr (C::kShare) __syncwarp();       // (the item before is done with its state)
+      if constexpr (NQ > 1) {
+        __syncwarp();                              // (the item before is done with its state)
+        if (lane < NQ * 4) nan_sh[lane] = 0u;
+      }
 #pragma unroll(kR)
       for (int n = 0; n < NQ; ++n) {
         const int r = C::kShare ? 0 : n;
@@ -546,7 +551,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) acc[n][mt][0] = acc[n][mt][1] = acc[n][mt][2] = acc[n][mt][3] = 0.f;
       }
-      if constexpr (C::kShare) __syncwarp();
+      if constexpr (NQ > 1) __syncwarp();
     }
 
     const int tb = si.tok_base + 32 * sub;                      // my 32 tokens
@@ -560,6 +565,34 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
             *reinterpret_cast<uint4*>(smem + s * kStageBytes + kTileBytes + tile0 + (row >> 4) * kChunkBytes + (row & 15) * 128 +
                                       (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
+      }
+      bool cleared = edge;
+      if constexpr (NQ > 1) {
+        // Keys that only some of the item's queries see (in front of the last one's window, behind the first one's own key): their
+        // weights are zero for the others, and a zero must not meet a NaN code. Such a code goes out of the tile, and the
+        // queries that see it get its NaN at the end of the item.
+        const int own = si.top - si.n_q;                       // the first query's own key
+        const int common = P.window_left < 0 || si.top - 1 <= P.window_left ? 0 : si.top - 1 - P.window_left;
+        if (__builtin_expect(vlo < common || vhi > own + 1, 0)) {
+#pragma unroll 1
+          for (int tok = vlo; tok < vhi; ++tok) {
+            if (tok >= common && tok <= own) { tok = own; continue; }
+            const int r = tok - tb;
+            uint8_t* row = smem + s * kStageBytes + kTileBytes + tile0 + (r >> 4) * kChunkBytes + (r & 15) * 128;
+            uint32_t* word = reinterpret_cast<uint32_t*>(row + (((lane >> 2) ^ (r & 7)) << 4)) + (lane & 3);
+            const uint32_t nan = (((*word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;    // 1 in every byte that is NaN
+            if (__builtin_expect(!__any_sync(0xffffffffu, nan), 1)) continue;
+            // (a lane's word is dims 4 lane ... 4 lane + 3: eight lanes to a word of the mask)
+            uint32_t bits = ((nan & 1u) | (nan >> 7 & 2u) | (nan >> 14 & 4u) | (nan >> 21 & 8u)) << (4 * (lane & 7));
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, off);
+            for (int n = 0; n < si.n_q; ++n)
+              if ((lane & 7) == 0 && tok <= own + n && (P.window_left < 0 || tok >= own + n - P.window_left)) nan_sh[n * 4 + (lane >> 3)] |= bits;
+            *word &= ~(nan * 255u);
+            __syncwarp();
+            cleared = true;
+          }
+        }
       }
       // ---- scores: [query][16-token half][token ta: heads 2t, 2t+1; token tb8: the same] ----
       float sc[NQ][2][4], ke[2][2], ve[2][2];
@@ -755,7 +788,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           for (int n = 0; n < NQ; ++n) mma_f16(acc[n][c + 1], a, pf[n][h][0], pf[n][h][1]);
         }
       }
-      if (edge) fence_proxy_async_smem();   // my zero fill precedes the next copy into these rows
+      if (cleared) fence_proxy_async_smem();   // what I wrote precedes the next copy into these rows
     }
     __syncwarp();
     // the last stage of an item becomes the scratch of its output before it goes back to the producer
@@ -820,6 +853,13 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
             const float4 o = *reinterpret_cast<const float4*>(po + row * kD + ((4 * lane) ^ ((row & 7) << 2)));
             L += ml[8 + row] * wgt;
             O.x += o.x * wgt; O.y += o.y * wgt; O.z += o.z * wgt; O.w += o.w * wgt;
+            if constexpr (NQ > 1) {
+              const uint32_t nan = reinterpret_cast<const uint32_t*>(smem + C::kNanOff)[(src * NQ + n) * 4 + (lane >> 3)] >> (4 * (lane & 7));
+              if (nan & 1u) O.x = __uint_as_float(0x7fffffffu);
+              if (nan & 2u) O.y = __uint_as_float(0x7fffffffu);
+              if (nan & 4u) O.z = __uint_as_float(0x7fffffffu);
+              if (nan & 8u) O.w = __uint_as_float(0x7fffffffu);
+            }
           }
           if (si.part < 0) {
             const float f = inverse(L);

@@ -120,3 +120,36 @@ def test_small_elements_of_a_query_count_where_its_large_ones_meet_zeros(ops, ne
     dev = [t.to(DEV) for t in (q, codes, scales, table)]
     want = ref.decode(*dev, lens, -1, SCALE, ref.FP16) if new is None else ref.runs(*dev, ctx, [n, n], -1, SCALE, weights=_weights_of([n]))
     _check(out, None, want)
+
+
+# ------------------------------------------------------------------------------------- NaN reaches those who see it, and nobody else
+def _check_with_nan(out, want):
+    o, l, err_o, err_l = want
+    odd = torch.isnan(o)
+    assert odd.any() and torch.equal(torch.isnan(out), odd), (int((torch.isnan(out) & ~odd).sum()), int((~torch.isnan(out) & odd).sum()))
+    _check(out.masked_fill(odd, 0.0), None, (o.masked_fill(odd, 0.0), l, err_o.masked_fill(odd, 0.0), err_l))
+
+
+def _with_nan_values(ctx, new, wl, H, kvh, seed):
+    """A cache and queries; sequence 1 has NaN codes in V at its newest token, in the middle of its run, and at the first two
+    tokens of the first query's window, each in a dim and a head of its own."""
+    lens = [a + b for a, b in zip(ctx, new)]
+    codes, scales, table = _pool(lens, wl, kvh, 128, 16, seed=seed, spread=0.5, n_new=new)
+    first = max(0, ctx[1] - wl) if wl >= 0 else 0
+    for i, t in enumerate((lens[1] - 1, ctx[1] + new[1] // 2, first, first + 1)):
+        row, _ = _row(codes, scales, table, 1, 1, t, i % kvh)
+        row[(5, 64, 127, 0)[i]] = 0x7F if i % 2 else 0xFF
+    q = torch.randn(sum(new), H, 128, generator=torch.Generator().manual_seed(seed + 1)).bfloat16()
+    return q, codes, scales, table
+
+
+@gpu
+@pytest.mark.parametrize("n,ctx,wl,H,kvh", [
+    (2, 200, 64, 28, 4), (3, 200, 64, 28, 4), (4, 200, 64, 28, 4), (16, 200, 64, 28, 4), (16, 0, 5, 7, 1), (2, 31, 16, 14, 2), (5, 77, 3, 14, 2),
+    (4, 200, -1, 4, 4), (13, 0, 0, 7, 1)])
+def test_a_nan_value_reaches_the_queries_that_see_it_in_short_runs(ops, n, ctx, wl, H, kvh):
+    ctx, new = [40, ctx, 60], [n, n, n]
+    q, codes, scales, table = _with_nan_values(ctx, new, wl, H, kvh, 220)
+    out = _attend(ops, q, codes, scales, table, ctx, new, wl)
+    want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=ref.FP16)
+    _check_with_nan(out, want)
