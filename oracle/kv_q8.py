@@ -124,7 +124,8 @@ def decode(q, codes, scales, table, lens: List[int], window_left: int, scale: fl
 
 def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: int, scale: float, one_row_each=False,
          weights: Optional[Weights] = None):
-    """Runs of queries: sequence s owns the next new[s] rows of q, behind ctx[s] cached tokens."""
+    """Runs of queries: sequence s owns the next new[s] rows of q, behind ctx[s] cached tokens. Tokens behind the end of the table's
+    row are as if they were not there."""
     H, D = q.shape[1:]
     dev = q.device
     res, row = [], 0
@@ -136,12 +137,18 @@ def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: i
                 row += 1
             continue
         lo = 0 if window_left < 0 else max(0, c - window_left)
-        k = window_values(codes[0], scales[0], table[s], lo, c + n)
-        v = window_values(codes[1], scales[1], table[s], lo, c + n)
+        hi = min(c + n, table.shape[1] * codes.shape[2])
+        if hi <= lo:
+            z = torch.zeros(n, H, D, dtype=torch.float64, device=dev)
+            res.append((z, torch.full((n, H), -math.inf, dtype=torch.float64, device=dev), z, z[..., 0]))
+            row += n
+            continue
+        k = window_values(codes[0], scales[0], table[s], lo, hi)
+        v = window_values(codes[1], scales[1], table[s], lo, hi)
         for i in range(0, n, 256):
             m = min(256, n - i)
             qp = torch.arange(c + i, c + i + m, device=dev)[:, None]
-            kp = torch.arange(lo, c + n, device=dev)[None]
+            kp = torch.arange(lo, hi, device=dev)[None]
             seen = (kp <= qp) & ((kp >= qp - window_left) if window_left >= 0 else (kp >= 0))
             res.append(attend(q[row + i:row + i + m], k, v, seen, scale, weights))
         row += n

@@ -53,7 +53,7 @@ constexpr float kMostW = 32768.f, kMostP = 1.099511627776e12f;   // 2^15, 2^40: 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kNegBig = -1.0e30f;
 enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8 };
 
-// row: the item's first query row; n_q: its queries; top: one past the last key of the last of them;
+// row: the item's first query row; n_q: its queries; top: one past the last key of the last of them (the table may end before);
 // part: partial slot of the item's result, or -1 (direct)
 struct StageInfo { int row, n_q, top, tok_base, lo, hi, flags, part; };
 
@@ -108,12 +108,16 @@ struct Params {
 };
 
 struct Span { int first, units; };    // units [first, first + units) of the token axis hold the visible tokens
+// width: tokens that a row of the block table has entries for
 template <int UNIT>
-__device__ __forceinline__ Span span_of(int top, int n_q, int window_left) {
+__device__ __forceinline__ Span span_of(int top, int n_q, int window_left, int64_t width) {
   Span s;
-  if (top <= 0) { s.first = 0; s.units = 0; return s; }
-  s.first = first_visible(top, n_q, window_left) / UNIT;
-  s.units = (top - 1) / UNIT - s.first + 1;
+  s.first = s.units = 0;
+  if (top <= 0) return s;
+  const int t0 = first_visible(top, n_q, window_left), end = top < width ? top : (int)width;
+  if (end <= t0) return s;
+  s.first = t0 / UNIT;
+  s.units = (end - 1) / UNIT - s.first + 1;
   return s;
 }
 
@@ -200,6 +204,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   volatile int* misc = reinterpret_cast<volatile int*>(smem + C::kMiscOff);   // [0] abort, [1] longest, [2..] scan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 kNotCut = make_int4(-1, 0, 0, 0);
+  const int64_t width = (int64_t)P.max_blocks * P.block_size;
 
   // the folding kernel may be set up while this one runs (it waits for this one's end before it reads anything)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -242,16 +247,13 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           ctx = ctx < 0 ? 0 : (ctx > (1 << 30) ? (1 << 30) : ctx);
           top = n > 0 ? ctx + q0 + n : -1;   // -1: no such queries, nothing to write
         }
-        const int64_t width = (int64_t)P.max_blocks * P.block_size;
-        if (top > width) {                   // tokens that the table has no entry for
-          top = (int)width;
-          if (blockIdx.x == 0) raise_status(P.status, SBK_ST_BAD_BLOCK);
-        }
+        // (tokens that the table has no entry for are not there)
+        if (top > width && blockIdx.x == 0) raise_status(P.status, SBK_ST_BAD_BLOCK);
         tops[b] = top;
         cnts[b] = (uint8_t)(n > 0 ? n : 0);
         if (top < 0 && P.seq_lens) tops[b] = top = 0;
         if (top >= 0) {
-          c = top > 0 ? span_of<kUnit>(top, n, P.window_left).units : 1;   // an empty one keeps a unit: somebody writes its zeros
+          c = max(span_of<kUnit>(top, n, P.window_left, width).units, 1);   // an empty one keeps a unit: somebody writes its zeros
           mx = max(mx, c);
           c += C::kItemCost;
         } else if (blockIdx.x == 0 && P.cut_by_item) {
@@ -339,6 +341,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         const int base = c0 * kChunk;
         const int lo = base > t0 ? base : t0;
         int hi = base + kUnit < top ? base + kUnit : top;
+        if (hi > width) hi = (int)width;
         if (n_units == 0 || hi < lo) hi = lo;
         // chunks of this stage that hold visible tokens: [ca, cb)
         const int ca = (lo - base) / kChunk, cb = hi > lo ? (hi - 1 - base) / kChunk + 1 : ca;
@@ -392,7 +395,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       if (lane == 0) P.cut[me] = kNotCut;      // (entries per item, where they are that, are fewer than CTAs)
       for (int b = me; b < P.B && !aborted; b += n_cta) {
         if (tops[b] < 0) continue;
-        const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left);
+        const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left, width);
         stream_item(b, sp.first, sp.units, -1);
       }
     } else {
@@ -414,7 +417,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           const int mid = (e + he) >> 1;
           if (pre[mid] <= g1 - 1) e = mid; else he = mid;
         }
-        const int cr = tops[e] > 0 ? span_of<kUnit>(tops[e], cnts[e], P.window_left).units : 1;
+        const int cr = max(span_of<kUnit>(tops[e], cnts[e], P.window_left, width).units, 1);
         if (pre[e] >= g0 && pre[e] + cr > g1) cut = make_int4(first_row(e), me, (pre[e] + cr - 1) / per - me + 1, cnts[e]);
       }
       // (before anything is streamed: the folding kernel reads every entry, also of a launch that gave up on a wait)
@@ -427,7 +430,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       if (g0 < total) {
         for (int b = b0; b < P.B && pre[b] < g1 && !aborted; ++b) {
           if (tops[b] < 0) continue;
-          const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left);
+          const Span sp = span_of<kUnit>(tops[b], cnts[b], P.window_left, width);
           const int cr = sp.units > 0 ? sp.units : 1;
           const int va = (int)(g0 > pre[b] ? g0 - pre[b] : 0);
           if (va >= cr) continue;                               // only charged slots of b fall into this run

@@ -59,6 +59,7 @@ struct Params {
   const int32_t* query_start_loc; const int32_t* context_lens;
   int seq0;               // first sequence of this launch; its dense rows start at row 0
   int rows_per_seq;       // dense rows of a sequence, a multiple of 128
+  int64_t width;          // tokens that a row of the block table has entries for
   int pairs;              // query tile pairs per sequence
   int pairs_per_head;     // of the sequences of this launch
   int split;              // pairs from here on are two CTAs' (of all heads, laid end to end)
@@ -67,9 +68,10 @@ struct Params {
   __nv_bfloat16* out; int64_t out_tok_stride; int32_t* status;
 };
 
-// what a sequence's run sees: keys [first, first + n) of its token axis
-struct Keys { int first, n, n_q; };
-__device__ __forceinline__ Keys keys_of(const int32_t* qsl, const int32_t* ctx_lens, int s, int window_left, int max_query_len) {
+// what a sequence's run sees: keys [first, first + n) of its token axis, of which the block table has entries for `there`
+struct Keys { int first, n, there, n_q; };
+__device__ __forceinline__ Keys keys_of(const int32_t* qsl, const int32_t* ctx_lens, int s, int window_left, int max_query_len,
+                                        int64_t width) {
   Keys k;
   k.n_q = qsl[s + 1] - qsl[s];
   if (k.n_q > max_query_len) k.n_q = max_query_len;
@@ -78,6 +80,7 @@ __device__ __forceinline__ Keys keys_of(const int32_t* qsl, const int32_t* ctx_l
   ctx = ctx < 0 ? 0 : (ctx > (1 << 30) ? (1 << 30) : ctx);
   k.first = window_left < 0 || ctx <= window_left ? 0 : ctx - window_left;
   k.n = k.n_q > 0 ? ctx - k.first + k.n_q : 0;
+  k.there = k.n <= width - k.first ? k.n : (width > k.first ? (int)(width - k.first) : 0);
   return k;
 }
 
@@ -90,21 +93,19 @@ unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v
               int max_query_len, int rows_per_seq, int64_t rows_total, uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out,
               int32_t* status) {
   const int s = seq0 + (int)blockIdx.y;
-  Keys ks = keys_of(query_start_loc, context_lens, s, window_left, max_query_len);
-  if (ks.n > rows_per_seq) {             // a run that goes past its row of the block table
-    if (blockIdx.x == 0 && threadIdx.x == 0) raise_status(status, SBK_ST_BAD_BLOCK);
-    ks.n = rows_per_seq;
-  }
-  const int n_pad = (ks.n + kTile - 1) / kTile * kTile;
+  const Keys ks = keys_of(query_start_loc, context_lens, s, window_left, max_query_len, (int64_t)max_blocks * block_size);
+  if (ks.n > ks.there && blockIdx.x == 0 && threadIdx.x == 0) raise_status(status, SBK_ST_BAD_BLOCK);
+  // (a run that sees nothing still reads a tile of zeros)
+  const int n_pad = ks.n_q == 0 ? 0 : (ks.there > kTile ? (ks.there + kTile - 1) / kTile * kTile : kTile);
   const int l = threadIdx.x & 15;
   const int32_t* table = block_tables + (int64_t)s * max_blocks;
   // consecutive groups of lanes walk the heads of a token: the rows of a token are contiguous in the cache
   for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < (int64_t)n_pad * kvh; i += (int64_t)gridDim.x * 16) {
     const int r = (int)(i / kvh), h = (int)(i - (int64_t)r * kvh);
     uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
-    if (r < ks.n) {
+    if (r < ks.there) {
       const int tok = ks.first + r, lb = tok / block_size, off = tok - lb * block_size;
-      const int32_t pb = lb < max_blocks ? table[lb] : -1;
+      const int32_t pb = table[lb];
       if (pb < 0 || pb >= num_blocks) {
         if (l == 0) raise_status(status, SBK_ST_BAD_BLOCK);
       } else {
@@ -165,7 +166,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   const int sl = item / P.pairs, s = P.seq0 + sl;
   // later queries see more keys: they are launched first, so the long items do not start last
   const int q0 = (P.pairs - 1 - (item - sl * P.pairs)) * 2 * kBQ + (tile == 1 ? kBQ : 0), most = tile < 0 ? 2 * kBQ : kBQ;
-  const Keys ks = keys_of(P.query_start_loc, P.context_lens, s, P.window_left, P.max_query_len);
+  const Keys ks = keys_of(P.query_start_loc, P.context_lens, s, P.window_left, P.max_query_len, P.width);
   if (q0 >= ks.n_q) return;            // whole CTA, before anything is allocated
   const int nq_pair = ks.n_q - q0 < most ? ks.n_q - q0 : most;
   const bool has_b = nq_pair > kBQ;
@@ -173,7 +174,9 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   // in dense rows (row 0 = key ks.first): the last key of the pair's first query, the first key it sees, one past the last key
   const int p0 = ks.n - ks.n_q + q0;
   const int lo = P.window_left < 0 || p0 <= P.window_left ? 0 : p0 - P.window_left;
-  const int t_lo = lo / kTile, n_tiles = (p0 + nq_pair - 1) / kTile - t_lo + 1;
+  // one past the last key of the pair; where the table ends in front of the first one, a tile that is masked altogether
+  const int key_end = p0 + nq_pair < ks.there ? p0 + nq_pair : ks.there;
+  const int t_lo = key_end > lo ? lo / kTile : 0, n_tiles = key_end > lo ? (key_end - 1) / kTile - t_lo + 1 : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -344,7 +347,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         if (!ok || *abort_flag) break;
         tc_fence_after();
         const int tb = (t_lo + t) * kTile;
-        int v_lo = lo_row - tb, v_hi = p_row + 1 - tb;            // columns this row may see: [v_lo, v_hi)
+        int v_lo = lo_row - tb, v_hi = (p_row < ks.there ? p_row + 1 : ks.there) - tb;   // columns this row may see: [v_lo, v_hi)
         v_lo = v_lo < 0 ? 0 : v_lo;
         v_hi = v_hi > kTile ? kTile : v_hi;
         const bool full = __all_sync(0xffffffffu, v_lo == 0 && v_hi == kTile);   // the warp takes one path
@@ -600,7 +603,7 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
   Params P = {};
   P.q = (const __nv_bfloat16*)q; P.q_tok_stride = q_tok_stride;
   P.query_start_loc = query_start_loc; P.context_lens = context_lens;
-  P.rows_per_seq = (int)y.rows_per_seq; P.pairs = pairs; P.max_query_len = max_query_len; P.H = H; P.G = H / kvh; P.bq = bq;
+  P.rows_per_seq = (int)y.rows_per_seq; P.width = (int64_t)max_blocks * block_size; P.pairs = pairs; P.max_query_len = max_query_len; P.H = H; P.G = H / kvh; P.bq = bq;
   P.window_left = window_left; P.scale_log2 = fabsf(scale) * kLog2e; P.q_sign = scale < 0.f ? 0x80008000u : 0u;
   P.out = (__nv_bfloat16*)out; P.out_tok_stride = out_tok_stride; P.status = status;
   // groups of sequences share the scratch, one after the other on the stream

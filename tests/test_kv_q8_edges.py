@@ -153,3 +153,28 @@ def test_a_nan_value_reaches_the_queries_that_see_it_in_short_runs(ops, n, ctx, 
     out = _attend(ops, q, codes, scales, table, ctx, new, wl)
     want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=ref.FP16)
     _check_with_nan(out, want)
+
+
+# ------------------------------------------------------------------------------------- lengths that go past the block table
+@gpu
+@pytest.mark.parametrize("new", [None, 1, 2, 5, 16, 20, 300])
+@pytest.mark.parametrize("ctx,wl,H,kvh", [(500, -1, 28, 4), (390, -1, 7, 1), (500, 150, 14, 2), (395, 40, 28, 4), (900, 100, 28, 4),
+                                          (3000, 2000, 4, 4), (399, 0, 7, 1)])
+def test_tokens_without_a_table_entry_take_no_part(ops, new, ctx, wl, H, kvh):
+    """Sequences 0 and 2 are longer than their row of the table (400 tokens; a few cases end just inside): reported, and the tokens behind it are as if they were
+    not there; nothing of their neighbours gets into them."""
+    n = new or 1
+    ctxs, news = [ctx, 60, ctx + 7, 20], [n, min(n, 300), max(1, n - 1), n]
+    lens = [a + b for a, b in zip(ctxs, news)]
+    codes, scales, table = _pool(lens, wl, kvh, 128, 16, seed=230, spread=0.5, n_new=news)
+    table = table[:, :25].contiguous()
+    q = torch.randn(sum(news), H, 128, generator=torch.Generator().manual_seed(231)).bfloat16()
+    dev = [t.to(DEV) for t in (q, codes, scales, table)]
+    status = 2 if max(lens) > 400 else 0
+    if new is None:
+        lse = torch.empty(4, H, device=DEV)
+        out = _attend(ops, q, codes, scales, table, lens, None, wl, status=status, lse=lse)
+        _check(out, lse, ref.decode(*dev, lens, wl, SCALE, ref.FP16))
+    else:
+        out = _attend(ops, q, codes, scales, table, ctxs, news, wl, status=status)
+        _check(out, None, ref.runs(*dev, ctxs, news, wl, SCALE, weights=_weights_of(news)))
