@@ -18,8 +18,8 @@
 //    Tensor memory (512 columns): S_A / P_A [0,128), S_B / P_B [128,256), O_A [256,384), O_B [384,512). The softmax offset of a row
 //    moves only when its maximum has grown by more than 2^8, so O is rescaled in tensor memory almost only on the first tile.
 //    Roles (384 threads): warps 0-3 softmax / epilogue of tile A, 4-7 of tile B, 8 producer of the K ring, 9 of the V ring, 10 tensor
-//    memory and MMA issue; 11 is there for its registers: the softmax warps hold a row's 128 scores at once, with what the last
-//    four warps give up. Every wait is bounded.
+//    memory and MMA issue; 11 looks through the tiles' flags, and is there for its registers: the softmax warps hold a row's 128 scores
+//    at once, with what the last four warps give up. Every wait is bounded.
 // Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 725 us, 664 TFLOP/s of useful products (4 H D
 //    a visible pair; with the heads of P alone it took 578). Then a tile pair took about 4000 cycles per 128 keys, of which the tensor
 //    core worked 2050: the rest is the way from a tile's last P over the MMAs still to be issued to its next scores, and the
@@ -65,6 +65,8 @@ struct Params {
   int split;              // pairs from here on are two CTAs' (of all heads, laid end to end)
   int max_query_len, H, G, bq, window_left; float scale_log2;   // >= 0: a negative scale's sign goes into q
   uint32_t q_sign;
+  const uint16_t* v_rows; int64_t rows_total;    // the dense V rows, for what the tensor core must not see: where a tile's flag
+  const uint32_t* nan_tiles;                     // [head][rows_total / 128] says so
   __nv_bfloat16* out; int64_t out_tok_stride; int32_t* status;
 };
 
@@ -84,24 +86,33 @@ __device__ __forceinline__ Keys keys_of(const int32_t* qsl, const int32_t* ctx_l
   return k;
 }
 
-// ---- 1. the visible keys of sequences seq0 ... as dense rows; 16 lanes per row, eight values each ----
+// A NaN code of V stands in the dense rows as this bf16 number, which no code gives (it is below their smallest by a factor of 2^60)
+// and which no sum notices: a weight of zero must not meet a NaN. The queries that see it get their NaN at the end.
+constexpr uint32_t kNanMark = 1u;
+// NaN codes of four: 1 in every byte that is one
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }
+
+// ---- 1. the visible keys of sequences seq0 ... as dense rows: a CTA per tile of 128 keys and head, 16 lanes per row, eight values each ----
 __global__ void __launch_bounds__(256)
 unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const uint8_t* __restrict__ k_scale,
               const uint8_t* __restrict__ v_scale, const int32_t* __restrict__ block_tables, int max_blocks,
               const int32_t* __restrict__ query_start_loc, const int32_t* __restrict__ context_lens, int seq0, int kvh,
               int64_t num_blocks, int block_size, int64_t cache_block_stride, int64_t scale_block_stride, int window_left,
               int max_query_len, int rows_per_seq, int64_t rows_total, uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out,
-              int32_t* status) {
+              uint32_t* __restrict__ nan_tiles, int32_t* status) {
   const int s = seq0 + (int)blockIdx.y;
   const Keys ks = keys_of(query_start_loc, context_lens, s, window_left, max_query_len, (int64_t)max_blocks * block_size);
   if (ks.n > ks.there && blockIdx.x == 0 && threadIdx.x == 0) raise_status(status, SBK_ST_BAD_BLOCK);
-  // (a run that sees nothing still reads a tile of zeros)
-  const int n_pad = ks.n_q == 0 ? 0 : (ks.there > kTile ? (ks.there + kTile - 1) / kTile * kTile : kTile);
+  // consecutive CTAs take the heads of a tile: the rows of a token are contiguous in the cache
+  const int tile = (int)blockIdx.x / kvh, h = (int)blockIdx.x - tile * kvh;
+  if (ks.n_q == 0 || (tile > 0 && tile * kTile >= ks.there)) return;      // (a run that sees nothing still reads a tile of zeros)
   const int l = threadIdx.x & 15;
   const int32_t* table = block_tables + (int64_t)s * max_blocks;
-  // consecutive groups of lanes walk the heads of a token: the rows of a token are contiguous in the cache
-  for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < (int64_t)n_pad * kvh; i += (int64_t)gridDim.x * 16) {
-    const int r = (int)(i / kvh), h = (int)(i - (int64_t)r * kvh);
+  const int64_t row0 = (int64_t)blockIdx.y * rows_per_seq + tile * kTile;
+  bool any_nan = false;
+#pragma unroll 4
+  for (int i = threadIdx.x >> 4; i < kTile; i += 16) {
+    const int r = tile * kTile + i;
     uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
     if (r < ks.there) {
       const int tok = ks.first + r, lb = tok / block_size, off = tok - lb * block_size;
@@ -119,12 +130,24 @@ unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v
         };
         kw = make_uint4(two(kc.x & 0xffffu, kf), two(kc.x >> 16, kf), two(kc.y & 0xffffu, kf), two(kc.y >> 16, kf));
         vw = make_uint4(two(vc.x & 0xffffu, vf), two(vc.x >> 16, vf), two(vc.y & 0xffffu, vf), two(vc.y >> 16, vf));
+        const uint32_t nx = nan_bytes(vc.x), ny = nan_bytes(vc.y);
+        if (__builtin_expect(nx | ny, 0)) {
+          auto mark = [](uint32_t w, uint32_t n) {
+            if (n & 1u) w = (w & 0xffff0000u) | kNanMark;
+            if (n & 0x100u) w = (w & 0xffffu) | kNanMark << 16;
+            return w;
+          };
+          vw = make_uint4(mark(vw.x, nx), mark(vw.y, nx >> 16), mark(vw.z, ny), mark(vw.w, ny >> 16));
+          any_nan = true;
+        }
       }
     }
-    const int64_t o = (((int64_t)h * rows_total + (int64_t)blockIdx.y * rows_per_seq + r) * kD + 8 * l) * 2;
+    const int64_t o = (((int64_t)h * rows_total + row0 + i) * kD + 8 * l) * 2;
     *reinterpret_cast<uint4*>(k_out + o) = kw;
     *reinterpret_cast<uint4*>(v_out + o) = vw;
   }
+  any_nan = __syncthreads_or(any_nan);
+  if (threadIdx.x == 0) nan_tiles[(int64_t)h * (rows_total / kTile) + row0 / kTile] = any_nan;
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
@@ -147,13 +170,14 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  // barriers: K ring full / empty, V ring full / empty; per tile: S ready, P ready (four quarters of the keys); Q staged; all done.
+  // barriers: K ring full / empty, V ring full / empty; per tile: S ready, P ready (four quarters of the keys); Q staged; all done; tiles' flags read.
   // S and P of a tile take turns strictly, so one barrier each and phase t & 1.
   const uint32_t bar_kf = sbase + kBarOff, bar_ke = bar_kf + 8 * kStagesK;
   const uint32_t bar_vf = bar_ke + 8 * kStagesK, bar_ve = bar_vf + 8 * kStagesV;
-  const uint32_t bar_s = bar_ve + 8 * kStagesV, bar_p = bar_s + 16, bar_q = bar_p + 64, bar_done = bar_q + 8;
+  const uint32_t bar_s = bar_ve + 8 * kStagesV, bar_p = bar_s + 16, bar_q = bar_p + 64, bar_done = bar_q + 8, bar_info = bar_done + 8;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + kBarOff + 192);
   volatile uint8_t* abort_flag = smem + kBarOff + 208;
+  volatile uint8_t* info = smem + kBarOff + 209;               // what the flags of this pair's tiles hold
 
   // pairs of tiles [0, split) are a CTA's each, the others two CTAs'
   int item = blockIdx.x, tile = -1;
@@ -186,6 +210,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     for (int i = 0; i < 8; ++i) mbar_init(bar_p + 8 * i, 4);      // one arrival per warp of the tile
     mbar_init(bar_q, kSoftmaxWarps);
     mbar_init(bar_done, 1);
+    mbar_init(bar_info, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -309,6 +334,15 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       }
       if (ok) commit(bar_done);
       if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
+    } else {
+      const uint32_t* nan_tiles = P.nan_tiles + ((int64_t)hk * P.rows_total + (int64_t)sl * P.rows_per_seq) / kTile + t_lo;
+      uint32_t any = 0u;
+      for (int t = lane; t < n_tiles; t += 32) any |= nan_tiles[t];
+      any = __reduce_or_sync(0xffffffffu, any);
+      if (lane == 0) {
+        *info = (uint8_t)any;
+        mbar_arrive(bar_info);
+      }
     }
     finish();
   } else {
@@ -445,7 +479,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         l_run = l_run * alpha + (ls[0] + ls[1]) + (ls[2] + ls[3]);
       }
       if (ok && !*abort_flag) {
-        ok = mbar_wait_bounded(bar_done, 0);
+        ok = mbar_wait_bounded(bar_done, 0) && mbar_wait_bounded(bar_info, 0);
         if (ok) {
           tc_fence_after();
           const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
@@ -463,6 +497,33 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                     pack_bf16x2(__uint_as_float(orr[e * 8 + 2]) * inv, __uint_as_float(orr[e * 8 + 3]) * inv),
                     pack_bf16x2(__uint_as_float(orr[e * 8 + 4]) * inv, __uint_as_float(orr[e * 8 + 5]) * inv),
                     pack_bf16x2(__uint_as_float(orr[e * 8 + 6]) * inv, __uint_as_float(orr[e * 8 + 7]) * inv));
+            }
+          }
+          if (__builtin_expect(*info != 0, 0)) {
+            // the marked dims of the keys that this row sees: dim 4 l + i is bit l of word i
+            uint32_t bits[4] = {0u, 0u, 0u, 0u};
+            const int64_t row0 = (int64_t)hk * P.rows_total + (int64_t)sl * P.rows_per_seq;
+#pragma unroll 1
+            for (int t = t_lo; t < t_lo + n_tiles; ++t) {
+              if (!P.nan_tiles[row0 / kTile + t]) continue;
+              const int key0 = t * kTile;
+              const uint16_t* rows = P.v_rows + (row0 + key0) * kD + 4 * lane;
+#pragma unroll 1
+              for (int j = 0; j < kTile; ++j) {
+                const ushort4 v = *reinterpret_cast<const ushort4*>(rows + (int64_t)j * kD);
+                const bool sees = key0 + j >= lo_row && key0 + j <= p_row;
+                const uint32_t b[4] = {__ballot_sync(0xffffffffu, v.x == kNanMark), __ballot_sync(0xffffffffu, v.y == kNanMark),
+                                       __ballot_sync(0xffffffffu, v.z == kNanMark), __ballot_sync(0xffffffffu, v.w == kNanMark)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (sees) bits[i] |= b[i];
+              }
+            }
+            if (row_ok) {
+              uint16_t* o = reinterpret_cast<uint16_t*>(op);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                for (uint32_t b = bits[i]; b; b &= b - 1) o[4 * (__ffs(b) - 1) + i] = 0x7fffu;
             }
           }
         }
@@ -493,6 +554,9 @@ static Layout layout_of(int n_seqs, int max_query_len, int max_blocks, int kvh, 
   y.group = (int)(g < n_seqs ? g : n_seqs);
   return y;
 }
+// the workspace: dense K rows, dense V rows, a flag per head and tile
+static size_t dense_bytes(const Layout& y, int kvh) { return (size_t)(y.rows_per_seq * y.group) * kvh * kD * 4; }
+static size_t scratch_bytes(const Layout& y, int kvh) { return dense_bytes(y, kvh) + (size_t)(y.rows_per_seq / kTile * y.group) * kvh * 4; }
 
 }  // namespace prefill_q8
 }  // namespace sbk
@@ -502,8 +566,7 @@ extern "C" size_t sbk_swa_prefill_q8_workspace_bytes(int n_seqs, int max_query_l
   using namespace sbk::prefill_q8;
   if (n_seqs <= 0 || max_query_len <= 0 || max_blocks <= 0 || kvh <= 0 || D <= 0 || block_size <= 0) return 0;
   if (few_queries(max_query_len, kvh)) return sbk::decode_q8::workspace_bytes(8 * kvh, true);   // H is 8 * kvh at the most
-  const Layout y = layout_of(n_seqs, max_query_len, max_blocks, kvh, block_size, window_left);
-  return (size_t)(y.rows_per_seq * y.group) * kvh * D * 4;
+  return scratch_bytes(layout_of(n_seqs, max_query_len, max_blocks, kvh, block_size, window_left), kvh);
 }
 
 extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const void* k_cache, const void* v_cache,
@@ -571,7 +634,7 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     set_error("sbk_swa_prefill_q8: grid or scratch too large");
     return SBK_E_ARG;
   }
-  const size_t half = (size_t)rows * kvh * D * 2;
+  const size_t half = dense_bytes(y, kvh) / 2;
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     if (!encode_rows_map(&maps[i], (uint8_t*)workspace + i * half, rows, kvh)) {
@@ -603,18 +666,20 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
   Params P = {};
   P.q = (const __nv_bfloat16*)q; P.q_tok_stride = q_tok_stride;
   P.query_start_loc = query_start_loc; P.context_lens = context_lens;
-  P.rows_per_seq = (int)y.rows_per_seq; P.width = (int64_t)max_blocks * block_size; P.pairs = pairs; P.max_query_len = max_query_len; P.H = H; P.G = H / kvh; P.bq = bq;
+  P.rows_per_seq = (int)y.rows_per_seq; P.width = (int64_t)max_blocks * block_size; P.pairs = pairs;
+  P.max_query_len = max_query_len; P.H = H; P.G = H / kvh; P.bq = bq;
   P.window_left = window_left; P.scale_log2 = fabsf(scale) * kLog2e; P.q_sign = scale < 0.f ? 0x80008000u : 0u;
   P.out = (__nv_bfloat16*)out; P.out_tok_stride = out_tok_stride; P.status = status;
+  uint32_t* const nan_tiles = reinterpret_cast<uint32_t*>((uint8_t*)workspace + 2 * half);
+  P.v_rows = reinterpret_cast<const uint16_t*>((const uint8_t*)workspace + half); P.rows_total = rows; P.nan_tiles = nan_tiles;
   // groups of sequences share the scratch, one after the other on the stream
   for (int s0 = 0; s0 < n_seqs; s0 += y.group) {
     const int n = n_seqs - s0 < y.group ? n_seqs - s0 : y.group;
-    const int64_t ctas = (y.rows_per_seq * kvh + 63) / 64;           // four rows per group of lanes
-    unpack_kernel<<<dim3((unsigned)(ctas < 65535 ? ctas : 65535), n), 256, 0, st>>>(
+    unpack_kernel<<<dim3((unsigned)(y.rows_per_seq / kTile * kvh), n), 256, 0, st>>>(
         (const uint8_t*)k_cache, (const uint8_t*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_tables,
         max_blocks, query_start_loc, context_lens, s0, kvh, num_blocks, block_size, cache_block_stride_bytes,
         scale_block_stride_bytes, window_left, max_query_len, P.rows_per_seq, rows, (uint8_t*)workspace,
-        (uint8_t*)workspace + half, status);
+        (uint8_t*)workspace + half, nan_tiles, status);
     int rc = check_launch("sbk_swa_prefill_q8");
     if (rc != SBK_OK) return rc;
     P.seq0 = s0;

@@ -155,6 +155,33 @@ def test_a_nan_value_reaches_the_queries_that_see_it_in_short_runs(ops, n, ctx, 
     _check_with_nan(out, want)
 
 
+@gpu
+@pytest.mark.parametrize("n,ctx,wl,H,kvh", [
+    (40, 200, 64, 28, 4), (300, 200, 64, 28, 4), (300, 200, 64, 4, 4), (20, 0, 5, 7, 1), (130, 31, -1, 14, 2), (257, 1000, 127, 8, 1), (17, 4000, 0, 6, 2)])
+def test_a_nan_value_reaches_the_queries_that_see_it_in_long_runs(ops, n, ctx, wl, H, kvh):
+    ctx, new = [40, ctx, 60], [n, n, n]
+    q, codes, scales, table = _with_nan_values(ctx, new, wl, H, kvh, 222)
+    out = _attend(ops, q, codes, scales, table, ctx, new, wl)
+    want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=ref.TWO_BF16)
+    _check_with_nan(out, want)
+
+
+@gpu
+@pytest.mark.parametrize("n", [20, 150])
+def test_a_nan_key_reaches_the_queries_that_see_it_in_long_runs(ops, n):
+    ctx, new, wl = [40, 90], [n, n], 64
+    codes, scales, table = _pool([a + n for a in ctx], wl, 4, 128, 16, seed=224, n_new=new)
+    for t in (ctx[1] + n // 2, ctx[1] - wl):
+        _row(codes, scales, table, 0, 1, t, 2)[0][9] = 0x7F
+    q = torch.randn(2 * n, 28, 128, generator=torch.Generator().manual_seed(225)).bfloat16()
+    out = _attend(ops, q, codes, scales, table, ctx, new, wl)
+    rows = torch.zeros(2 * n, 28, dtype=torch.bool)
+    for i in range(n):
+        pos = ctx[1] + i
+        rows[n + i, 14:21] = any(pos - wl <= t <= pos for t in (ctx[1] + n // 2, ctx[1] - wl))
+    assert torch.equal(torch.isnan(out).all(-1).cpu(), rows) and torch.isfinite(out.float()[~rows.to(DEV)]).all()
+
+
 # ------------------------------------------------------------------------------------- lengths that go past the block table
 @gpu
 @pytest.mark.parametrize("new", [None, 1, 2, 5, 16, 20, 300])
