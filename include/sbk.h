@@ -325,9 +325,12 @@ int sbk_kv_gather_q8(const void* k_cache, const void* v_cache, const void* k_sca
 
 /*
  * Sliding-window attention over the 8-bit cache: sbk_swa_decode (one query token per sequence) and sbk_swa_prefill (runs of
- * query tokens) with the cache as above. q bf16; a query sees what it sees there; a sequence of length 0 gets zeros and
- * lse -inf; a block-table entry outside the pool raises SBK_ST_BAD_BLOCK. Equal to the attention over the bf16 values that
- * sbk_kv_gather_q8 returns, up to the rounding of the sums.
+ * query tokens) with the cache as above. q bf16; a query sees what it sees there; a row that sees nothing gets zeros and
+ * lse -inf. Tokens whose block-table entry is outside the pool, and tokens behind the end of the table's row, raise
+ * SBK_ST_BAD_BLOCK and take no part, as if they were not there. A NaN in a K row makes the rows of the queries that see the token NaN, a
+ * NaN in a V row its own dim of them; queries that do not see the token keep their values. Equal to the attention over
+ * the bf16 values that sbk_kv_gather_q8 returns, up to the rounding of the weights (fp16 for single tokens and short runs, two bf16
+ * numbers for long ones) and of the sums (fp32).
  *  workspace    at least sbk_swa_decode_q8_workspace_bytes(B, H, D) or sbk_swa_prefill_q8_workspace_bytes(...) bytes,
  *               16-byte aligned (may be NULL when that is 0). Its contents need no initialisation and mean nothing between calls.
  *               Calls that overlap on the GPU need workspaces of their own. For runs of more than 16 queries (or kvh not

@@ -112,7 +112,7 @@ def window_values(codes: torch.Tensor, scale: torch.Tensor, table: torch.Tensor,
     [blocks, kvh, bs]."""
     bs = codes.shape[1]
     t = torch.arange(lo, hi, device=codes.device)
-    blk = table[t // bs].long()
+    blk = table[t // bs].long().clamp(0, codes.shape[0] - 1)
     return values(codes.view(torch.uint8)[blk, t % bs], scale[blk, :, t % bs])
 
 
@@ -125,7 +125,7 @@ def decode(q, codes, scales, table, lens: List[int], window_left: int, scale: fl
 def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: int, scale: float, one_row_each=False,
          weights: Optional[Weights] = None):
     """Runs of queries: sequence s owns the next new[s] rows of q, behind ctx[s] cached tokens. Tokens behind the end of the table's
-    row are as if they were not there."""
+    row, and those whose entry is outside the pool, are as if they were not there."""
     H, D = q.shape[1:]
     dev = q.device
     res, row = [], 0
@@ -145,11 +145,13 @@ def runs(q, codes, scales, table, ctx: List[int], new: List[int], window_left: i
             continue
         k = window_values(codes[0], scales[0], table[s], lo, hi)
         v = window_values(codes[1], scales[1], table[s], lo, hi)
+        entry = table[s][torch.arange(lo, hi, device=dev) // codes.shape[2]]
+        there = ((entry >= 0) & (entry < codes.shape[1]))[None]
         for i in range(0, n, 256):
             m = min(256, n - i)
             qp = torch.arange(c + i, c + i + m, device=dev)[:, None]
             kp = torch.arange(lo, hi, device=dev)[None]
-            seen = (kp <= qp) & ((kp >= qp - window_left) if window_left >= 0 else (kp >= 0))
+            seen = there & (kp <= qp) & ((kp >= qp - window_left) if window_left >= 0 else (kp >= 0))
             res.append(attend(q[row + i:row + i + m], k, v, seen, scale, weights))
         row += n
     return tuple(torch.cat([r[j] for r in res]) for j in range(4))

@@ -51,7 +51,7 @@ constexpr int kStageBytes = 2 * kTileBytes;
 constexpr int kMergeWarpBytes = kMaxG * kD * 4;
 constexpr float kMostW = 32768.f, kMostP = 1.099511627776e12f;   // 2^15, 2^40: where the offsets of the softmax move
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f, kNegBig = -1.0e30f;
-enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8 };
+enum : int { kFirst = 1, kLast = 2, kEnd = 4, kGoneShift = 8 };   // from kGoneShift on: a bit for each 16 tokens that the pool does not hold
 
 // row: the item's first query row; n_q: its queries; top: one past the last key of the last of them (the table may end before);
 // part: partial slot of the item's result, or -1 (direct)
@@ -353,17 +353,18 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         src = src < 0 ? 0 : (src > 31 ? 31 : src);
         const int64_t pb = __shfl_sync(0xffffffffu, pb_lane, src);
         const bool in = c >= ca && c < cb;
-        const bool bad = __any_sync(0xffffffffu, in && (pb < 0 || pb >= P.num_blocks));
+        const bool bad = in && (pb < 0 || pb >= P.num_blocks);
+        const uint32_t gone = __ballot_sync(0xffffffffu, bad) >> 16 & ((1u << kChunks) - 1u);   // (lanes 16 ...: chunks 0 ...)
         if (lane == 0) {
           StageInfo si;
           si.row = row; si.n_q = n_q; si.top = top; si.tok_base = base; si.lo = lo; si.hi = hi; si.part = part;
-          si.flags = (j == 0 ? kFirst : 0) | (j == n - 1 ? kLast : 0) | (bad ? kBad : 0);
+          si.flags = (j == 0 ? kFirst : 0) | (j == n - 1 ? kLast : 0) | (int)(gone << kGoneShift);
           info[s] = si;
-          if (bad) raise_status(P.status, SBK_ST_BAD_BLOCK);
-          mbar_arrive_expect_tx(bar_full + 8 * s, bad ? 0u : (uint32_t)(cb - ca) * 2u * kChunkBytes);
+          if (gone) raise_status(P.status, SBK_ST_BAD_BLOCK);
+          mbar_arrive_expect_tx(bar_full + 8 * s, (uint32_t)(cb - ca - __popc(gone)) * 2u * kChunkBytes);
         }
         __syncwarp();
-        if (!bad && in) {
+        if (in && !bad) {
           const int tin = (base + c * kChunk) % P.block_size;
           const uint32_t bar = bar_full + 8 * s;
           if (!is_tile) {
@@ -559,12 +560,13 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 
     const int tb = si.tok_base + 32 * sub;                      // my 32 tokens
     const int vlo = si.lo > tb ? si.lo : tb, vhi = si.hi < tb + 32 ? si.hi : tb + 32;
-    if (!(si.flags & kBad) && vhi > vlo) {
-      const bool edge = vlo > tb || vhi < tb + 32;
+    if (vhi > vlo) {
+      const uint32_t gone = (uint32_t)si.flags >> (kGoneShift + 2 * sub) & 3u;
+      const bool edge = vlo > tb || vhi < tb + 32 || gone;
       if (__builtin_expect(edge, 0)) {
         // rows outside the visible range hold anything, or older data: a zero probability must not meet a NaN code
         for (int row = lane >> 3; row < 32; row += 4)
-          if (tb + row < vlo || tb + row >= vhi)
+          if (tb + row < vlo || tb + row >= vhi || (gone >> (row >> 4) & 1u))
             *reinterpret_cast<uint4*>(smem + s * kStageBytes + kTileBytes + tile0 + (row >> 4) * kChunkBytes + (row & 15) * 128 +
                                       (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
@@ -666,8 +668,8 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
-          if (a < vlo || a >= vhi) ve[h][0] = 0.f;
-          if (b < vlo || b >= vhi) ve[h][1] = 0.f;
+          if (a < vlo || a >= vhi || (gone >> h & 1u)) ve[h][0] = 0.f;
+          if (b < vlo || b >= vhi || (gone >> h & 1u)) ve[h][1] = 0.f;
         }
       }
       uint32_t pf[NQ][2][2];
@@ -693,12 +695,12 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           nlo = first > vlo ? first : vlo;
           nhi = last + 1 < vhi ? last + 1 : vhi;
         }
-        if (__builtin_expect(nlo > tb || nhi < tb + 32, 0)) {
+        if (__builtin_expect(nlo > tb || nhi < tb + 32 || gone, 0)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int a = tb + 16 * h + ta, b = tb + 16 * h + tb8;
-            if (a < nlo || a >= nhi) sc[n][h][0] = sc[n][h][1] = -INFINITY;
-            if (b < nlo || b >= nhi) sc[n][h][2] = sc[n][h][3] = -INFINITY;
+            if (a < nlo || a >= nhi || (gone >> h & 1u)) sc[n][h][0] = sc[n][h][1] = -INFINITY;
+            if (b < nlo || b >= nhi || (gone >> h & 1u)) sc[n][h][2] = sc[n][h][3] = -INFINITY;
           }
         }
         // ---- p = 2^(s - m), w = p * 2^(ev - r) with the offsets in use; they move only when a w leaves fp16 ----

@@ -65,8 +65,8 @@ struct Params {
   int split;              // pairs from here on are two CTAs' (of all heads, laid end to end)
   int max_query_len, H, G, bq, window_left; float scale_log2;   // >= 0: a negative scale's sign goes into q
   uint32_t q_sign;
-  const uint16_t* v_rows; int64_t rows_total;    // the dense V rows, for what the tensor core must not see: where a tile's flag
-  const uint32_t* nan_tiles;                     // [head][rows_total / 128] says so
+  const uint16_t* v_rows; int64_t rows_total;    // the dense V rows, for what the tensor core must not see
+  const uint4* gone; const uint32_t* tile_flags; // of every head and tile [kvh][rows_total / 128]: rows that the pool does not hold, flags
   __nv_bfloat16* out; int64_t out_tok_stride; int32_t* status;
 };
 
@@ -89,6 +89,7 @@ __device__ __forceinline__ Keys keys_of(const int32_t* qsl, const int32_t* ctx_l
 // A NaN code of V stands in the dense rows as this bf16 number, which no code gives (it is below their smallest by a factor of 2^60)
 // and which no sum notices: a weight of zero must not meet a NaN. The queries that see it get their NaN at the end.
 constexpr uint32_t kNanMark = 1u;
+enum : uint32_t { kTileNan = 1, kTileGone = 2 };     // flags of a tile: marked values in its V rows; rows that take no part (a bit each)
 // NaN codes of four: 1 in every byte that is one
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7; }
 
@@ -99,7 +100,7 @@ unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v
               const int32_t* __restrict__ query_start_loc, const int32_t* __restrict__ context_lens, int seq0, int kvh,
               int64_t num_blocks, int block_size, int64_t cache_block_stride, int64_t scale_block_stride, int window_left,
               int max_query_len, int rows_per_seq, int64_t rows_total, uint8_t* __restrict__ k_out, uint8_t* __restrict__ v_out,
-              uint32_t* __restrict__ nan_tiles, int32_t* status) {
+              uint4* __restrict__ gone, uint32_t* __restrict__ tile_flags, int32_t* status) {
   const int s = seq0 + (int)blockIdx.y;
   const Keys ks = keys_of(query_start_loc, context_lens, s, window_left, max_query_len, (int64_t)max_blocks * block_size);
   if (ks.n > ks.there && blockIdx.x == 0 && threadIdx.x == 0) raise_status(status, SBK_ST_BAD_BLOCK);
@@ -109,6 +110,9 @@ unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v
   const int l = threadIdx.x & 15;
   const int32_t* table = block_tables + (int64_t)s * max_blocks;
   const int64_t row0 = (int64_t)blockIdx.y * rows_per_seq + tile * kTile;
+  __shared__ uint32_t miss[4];
+  if (threadIdx.x < 4) miss[threadIdx.x] = 0u;
+  __syncthreads();
   bool any_nan = false;
 #pragma unroll 4
   for (int i = threadIdx.x >> 4; i < kTile; i += 16) {
@@ -118,7 +122,10 @@ unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v
       const int tok = ks.first + r, lb = tok / block_size, off = tok - lb * block_size;
       const int32_t pb = table[lb];
       if (pb < 0 || pb >= num_blocks) {
-        if (l == 0) raise_status(status, SBK_ST_BAD_BLOCK);
+        if (l == 0) {
+          raise_status(status, SBK_ST_BAD_BLOCK);
+          atomicOr(&miss[i >> 5], 1u << (i & 31));
+        }
       } else {
         const int64_t at = (int64_t)pb * cache_block_stride + ((int64_t)off * kvh + h) * kD + 8 * l;
         const int64_t sa = (int64_t)pb * scale_block_stride + (int64_t)h * block_size + off;
@@ -147,7 +154,13 @@ unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v
     *reinterpret_cast<uint4*>(v_out + o) = vw;
   }
   any_nan = __syncthreads_or(any_nan);
-  if (threadIdx.x == 0) nan_tiles[(int64_t)h * (rows_total / kTile) + row0 / kTile] = any_nan;
+  if (threadIdx.x == 0) {
+    const int64_t at = (h * rows_total + row0) / kTile;
+    const uint4 m = make_uint4(miss[0], miss[1], miss[2], miss[3]);
+    const bool any_gone = m.x | m.y | m.z | m.w;
+    if (any_gone) gone[at] = m;
+    tile_flags[at] = (any_nan ? kTileNan : 0u) | (any_gone ? kTileGone : 0u);
+  }
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
@@ -335,9 +348,9 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       if (ok) commit(bar_done);
       if (!ok && lane == 0 && !*abort_flag) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); *abort_flag = 1; }
     } else {
-      const uint32_t* nan_tiles = P.nan_tiles + ((int64_t)hk * P.rows_total + (int64_t)sl * P.rows_per_seq) / kTile + t_lo;
+      const uint32_t* flags = P.tile_flags + ((int64_t)hk * P.rows_total + (int64_t)sl * P.rows_per_seq) / kTile + t_lo;
       uint32_t any = 0u;
-      for (int t = lane; t < n_tiles; t += 32) any |= nan_tiles[t];
+      for (int t = lane; t < n_tiles; t += 32) any |= flags[t];
       any = __reduce_or_sync(0xffffffffu, any);
       if (lane == 0) {
         *info = (uint8_t)any;
@@ -374,9 +387,9 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t s_col = t_lane + X * 128, o_col = t_lane + kOCol + X * 128;
     float m_run = -INFINITY, mr = -INFINITY, l_run = 0.f;
-    bool ok = true;
+    bool ok = mbar_wait_bounded(bar_info, 0);
     if (X == 0 || has_b) {
-      for (int t = 0; t < n_tiles; ++t) {
+      for (int t = 0; ok && t < n_tiles; ++t) {
         ok = mbar_wait_bounded(bar_s + 8 * X, t & 1);
         if (!ok || *abort_flag) break;
         tc_fence_after();
@@ -384,7 +397,8 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         int v_lo = lo_row - tb, v_hi = (p_row < ks.there ? p_row + 1 : ks.there) - tb;   // columns this row may see: [v_lo, v_hi)
         v_lo = v_lo < 0 ? 0 : v_lo;
         v_hi = v_hi > kTile ? kTile : v_hi;
-        const bool full = __all_sync(0xffffffffu, v_lo == 0 && v_hi == kTile);   // the warp takes one path
+        const bool holes = *info & kTileGone;
+        const bool full = __all_sync(0xffffffffu, v_lo == 0 && v_hi == kTile && !holes);   // the warp takes one path
         // ---- the row's scores and their maximum ----
         uint32_t sr4[4][32];
 #pragma unroll
@@ -400,11 +414,26 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 #pragma unroll
               for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], __uint_as_float(sr4[c][i]), __uint_as_float(sr4[c][i + 1]));
           } else {
+            // what the row does not see becomes -inf
+            uint32_t hid[4] = {0u, 0u, 0u, 0u};
+            if (holes) {
+              const int64_t at = ((int64_t)hk * P.rows_total + (int64_t)sl * P.rows_per_seq) / kTile + t_lo + t;
+              if (P.tile_flags[at] & kTileGone) {
+                const uint4 g = P.gone[at];
+                hid[0] = g.x; hid[1] = g.y; hid[2] = g.z; hid[3] = g.w;
+              }
+            }
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int c = 0; c < 4; ++c) {
+              const int a = v_lo - 32 * c, b = v_hi - 32 * c;
+              if (a > 0) hid[c] |= a > 31 ? 0xffffffffu : (1u << a) - 1u;
+              if (b < 32) hid[c] |= b <= 0 ? 0xffffffffu : 0xffffffffu << b;
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
-                if (32 * c + i >= v_lo && 32 * c + i < v_hi) mx[c] = fmaxf(mx[c], __uint_as_float(sr4[c][i]));
+              for (int i = 0; i < 32; ++i) {
+                if (hid[c] >> i & 1u) sr4[c][i] = __float_as_uint(-INFINITY);
+                mx[c] = fmaxf(mx[c], __uint_as_float(sr4[c][i]));
+              }
+            }
           }
           both = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         }
@@ -462,8 +491,8 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
               for (int i = 0; i < 32; i += 2) {
                 float pa = fast_exp2((__uint_as_float(sr[i]) - mr) * P.scale_log2);
                 float pb = fast_exp2((__uint_as_float(sr[i + 1]) - mr) * P.scale_log2);
-                if (col0 + i < v_lo || col0 + i >= v_hi) pa = 0.f;
-                if (col0 + i + 1 < v_lo || col0 + i + 1 >= v_hi) pb = 0.f;
+                if (__uint_as_float(sr[i]) == -INFINITY) pa = 0.f;
+                if (__uint_as_float(sr[i + 1]) == -INFINITY) pb = 0.f;
                 ls[i & 3] += pa;
                 ls[(i + 1) & 3] += pb;
                 split_bf16x2(pa, pb, ph[i >> 1], ph[16 + (i >> 1)]);
@@ -479,7 +508,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         l_run = l_run * alpha + (ls[0] + ls[1]) + (ls[2] + ls[3]);
       }
       if (ok && !*abort_flag) {
-        ok = mbar_wait_bounded(bar_done, 0) && mbar_wait_bounded(bar_info, 0);
+        ok = mbar_wait_bounded(bar_done, 0);
         if (ok) {
           tc_fence_after();
           const float inv = l_run != 0.f ? 1.f / l_run : 0.f;
@@ -499,13 +528,13 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                     pack_bf16x2(__uint_as_float(orr[e * 8 + 6]) * inv, __uint_as_float(orr[e * 8 + 7]) * inv));
             }
           }
-          if (__builtin_expect(*info != 0, 0)) {
+          if (__builtin_expect(*info & kTileNan, 0)) {
             // the marked dims of the keys that this row sees: dim 4 l + i is bit l of word i
             uint32_t bits[4] = {0u, 0u, 0u, 0u};
             const int64_t row0 = (int64_t)hk * P.rows_total + (int64_t)sl * P.rows_per_seq;
 #pragma unroll 1
             for (int t = t_lo; t < t_lo + n_tiles; ++t) {
-              if (!P.nan_tiles[row0 / kTile + t]) continue;
+              if (!(P.tile_flags[row0 / kTile + t] & kTileNan)) continue;
               const int key0 = t * kTile;
               const uint16_t* rows = P.v_rows + (row0 + key0) * kD + 4 * lane;
 #pragma unroll 1
@@ -554,9 +583,9 @@ static Layout layout_of(int n_seqs, int max_query_len, int max_blocks, int kvh, 
   y.group = (int)(g < n_seqs ? g : n_seqs);
   return y;
 }
-// the workspace: dense K rows, dense V rows, a flag per head and tile
+// the workspace: dense K rows, dense V rows, for every head and tile 16 bytes of missing rows and the flags
 static size_t dense_bytes(const Layout& y, int kvh) { return (size_t)(y.rows_per_seq * y.group) * kvh * kD * 4; }
-static size_t scratch_bytes(const Layout& y, int kvh) { return dense_bytes(y, kvh) + (size_t)(y.rows_per_seq / kTile * y.group) * kvh * 4; }
+static size_t scratch_bytes(const Layout& y, int kvh) { return dense_bytes(y, kvh) + (size_t)(y.rows_per_seq / kTile * y.group) * kvh * 20; }
 
 }  // namespace prefill_q8
 }  // namespace sbk
@@ -670,8 +699,10 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
   P.max_query_len = max_query_len; P.H = H; P.G = H / kvh; P.bq = bq;
   P.window_left = window_left; P.scale_log2 = fabsf(scale) * kLog2e; P.q_sign = scale < 0.f ? 0x80008000u : 0u;
   P.out = (__nv_bfloat16*)out; P.out_tok_stride = out_tok_stride; P.status = status;
-  uint32_t* const nan_tiles = reinterpret_cast<uint32_t*>((uint8_t*)workspace + 2 * half);
-  P.v_rows = reinterpret_cast<const uint16_t*>((const uint8_t*)workspace + half); P.rows_total = rows; P.nan_tiles = nan_tiles;
+  uint4* const gone = reinterpret_cast<uint4*>((uint8_t*)workspace + 2 * half);
+  uint32_t* const tile_flags = reinterpret_cast<uint32_t*>(gone + rows / kTile * kvh);
+  P.v_rows = reinterpret_cast<const uint16_t*>((const uint8_t*)workspace + half); P.rows_total = rows;
+  P.gone = gone; P.tile_flags = tile_flags;
   // groups of sequences share the scratch, one after the other on the stream
   for (int s0 = 0; s0 < n_seqs; s0 += y.group) {
     const int n = n_seqs - s0 < y.group ? n_seqs - s0 : y.group;
@@ -679,7 +710,7 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
         (const uint8_t*)k_cache, (const uint8_t*)v_cache, (const uint8_t*)k_scale, (const uint8_t*)v_scale, block_tables,
         max_blocks, query_start_loc, context_lens, s0, kvh, num_blocks, block_size, cache_block_stride_bytes,
         scale_block_stride_bytes, window_left, max_query_len, P.rows_per_seq, rows, (uint8_t*)workspace,
-        (uint8_t*)workspace + half, nan_tiles, status);
+        (uint8_t*)workspace + half, gone, tile_flags, status);
     int rc = check_launch("sbk_swa_prefill_q8");
     if (rc != SBK_OK) return rc;
     P.seq0 = s0;

@@ -205,3 +205,27 @@ def test_tokens_without_a_table_entry_take_no_part(ops, new, ctx, wl, H, kvh):
     else:
         out = _attend(ops, q, codes, scales, table, ctxs, news, wl, status=status)
         _check(out, None, ref.runs(*dev, ctxs, news, wl, SCALE, weights=_weights_of(news)))
+
+
+@gpu
+@pytest.mark.parametrize("new", [None, 1, 2, 4, 16, 40, 300])
+@pytest.mark.parametrize("H,kvh,bs,wl", [(28, 4, 16, -1), (28, 4, 16, 90), (7, 1, 16, -1), (14, 2, 48, 200), (4, 4, 32, 64), (8, 1, 16, 120)])
+def test_tokens_of_an_entry_outside_the_pool_take_no_part(ops, new, H, kvh, bs, wl):
+    """Sequence 1 has such entries in and around its window, sequence 2 nothing else: reported, and exactly their tokens are as if
+    they were not there, whichever kernel serves the run."""
+    n = new or 1
+    ctx, news = [300, 333, 200, 64], [n, n, n, max(1, n - 3)]
+    lens = [a + b for a, b in zip(ctx, news)]
+    codes, scales, table = _pool(lens, wl, kvh, 128, bs, seed=240, spread=0.5, n_new=news)
+    lo = max(0, ctx[1] - wl) // bs if wl >= 0 else 0
+    table[1, lo], table[1, lo + 2], table[1, (lens[1] - 1) // bs] = -1, 10 ** 6, codes.shape[1]
+    table[2] = -2 ** 31
+    q = torch.randn(sum(news), H, 128, generator=torch.Generator().manual_seed(241)).bfloat16()
+    dev = [t.to(DEV) for t in (q, codes, scales, table)]
+    if new is None:
+        lse = torch.empty(4, H, device=DEV)
+        out = _attend(ops, q, codes, scales, table, lens, None, wl, status=2, lse=lse)
+        _check(out, lse, ref.decode(*dev, lens, wl, SCALE, ref.FP16))
+    else:
+        out = _attend(ops, q, codes, scales, table, ctx, news, wl, status=2)
+        _check(out, None, ref.runs(*dev, ctx, news, wl, SCALE, weights=_weights_of(news)))
