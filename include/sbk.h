@@ -334,8 +334,10 @@ int sbk_kv_gather_q8(const void* k_cache, const void* v_cache, const void* k_sca
  *  workspace    at least sbk_swa_decode_q8_workspace_bytes(B, H, D) or sbk_swa_prefill_q8_workspace_bytes(...) bytes,
  *               16-byte aligned (may be NULL when that is 0). Its contents need no initialisation and mean nothing between calls.
  *               Calls that overlap on the GPU need workspaces of their own. For runs of more than 16 queries (or kvh not
- *               1, 2 or 4) it holds the visible keys as dense bf16 rows: up to 256 MiB, or one sequence's worth where that
- *               is more (the sequences take turns); else partial results, as for single tokens.
+ *               1, 2 or 4) it holds the visible keys as dense bf16 rows, laid out for the most that a run can see: window_left +
+ *               max_query_len keys, or max_blocks * block_size where that is less, 512 kvh bytes each. Sequences share 256
+ *               MiB, or one sequence's worth where that is more, in turn: without a window, a table no wider than the longest
+ *               sequence keeps both the workspace and the number of turns small. Else partial results, as for single tokens.
  * Supported: D == 128, H % kvh == 0, H/kvh <= 8, block_size % 16 == 0; sbk_swa_decode_q8: kvh in {1,2,4}; sbk_swa_prefill_q8:
  * q, out 16-byte aligned with token strides that are multiples of 8 elements.
  */

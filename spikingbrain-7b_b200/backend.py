@@ -588,7 +588,7 @@ class MetaAttentionImpl:
             self._runs(pq, kv_cache, cache, prefill_meta.block_tables.contiguous(),
                        prefill_meta.query_start_loc.to(torch.int32).contiguous(),
                        prefill_meta.context_lens_tensor.to(torch.int32).contiguous(),
-                       prefill_meta.max_query_len, window_left, tmp, key2, value2)
+                       prefill_meta.max_query_len, window_left, tmp, key2, value2, prefill_meta.max_prefill_seq_len)
             if tmp is not po:
                 po.copy_(tmp)
 
@@ -614,15 +614,18 @@ class MetaAttentionImpl:
         return output
 
     def _runs(self, q, kv_cache, cache8, block_tables, query_start_loc, context_lens, max_query_len, window_left, out,
-              key2, value2) -> None:
+              key2, value2, max_seq_len=None) -> None:
         """Runs of query tokens over the paged cache, bf16 or (cache8) 8-bit."""
         if cache8 is not None:
+            if not max_seq_len or torch.cuda.is_current_stream_capturing():   # (a replay may bring longer sequences)
+                max_seq_len = None
             if q.data_ptr() % 16 or (q.shape[0] > 1 and q.stride(0) % 8):
                 q = q.clone(memory_format=torch.contiguous_format)
             dst = out if out.data_ptr() % 16 == 0 and (out.shape[0] < 2 or out.stride(0) % 8 == 0) else torch.empty(
                 out.shape, dtype=out.dtype, device=out.device)
             ops.swa_prefill_q8(q, *cache8, block_tables, query_start_loc, context_lens, max_query_len,
-                               window_left=window_left, scale=self.scale, out=dst, status=self._status)
+                               window_left=window_left, scale=self.scale, out=dst, status=self._status,
+                               max_seq_len=max_seq_len)
             if dst is not out:
                 out.copy_(dst)
             return

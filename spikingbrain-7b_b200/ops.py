@@ -872,10 +872,24 @@ def swa_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     return out
 
 
+def _prefill_q8_columns(max_blocks: int, block_size: int, kvh: int, max_query_len: int, window_left: int,
+                        max_seq_len: Optional[int]) -> int:
+    """Columns of the block table that a call with this bound on its lengths works on."""
+    if max_seq_len is None or (max_query_len <= 16 and kvh in (1, 2, 4)):    # (short runs need no dense rows)
+        return max_blocks
+    need = max(1, -(-int(max_seq_len) // block_size))
+    if need >= max_blocks or 0 <= window_left <= need * block_size - max_query_len:    # (the window bounds them already)
+        return max_blocks
+    return need
+
+
 def swa_prefill_q8_workspace(n_seqs: int, max_query_len: int, max_blocks: int, kvh: int, D: int, device, *, block_size: int,
-                             window_left: int) -> Optional[torch.Tensor]:
-    """Scratch for swa_prefill_q8 calls of these sizes (None when it needs none): the visible keys as dense bf16 rows. Its
-    contents need no initialisation; calls that can overlap on the GPU need one each."""
+                             window_left: int, max_seq_len: Optional[int] = None) -> Optional[torch.Tensor]:
+    """Scratch for swa_prefill_q8 calls of these sizes (None when it needs none). Runs of more than 16 queries: dense bf16 rows for
+    as many keys as a run can see at the most, that is window_left + max_query_len, the width of the block table, or
+    ``max_seq_len``, whichever is least; 256 MiB of them, or one sequence's where that is more. Its contents need no
+    initialisation; calls that can overlap on the GPU need one each."""
+    max_blocks = _prefill_q8_columns(max_blocks, block_size, kvh, max_query_len, window_left, max_seq_len)
     n = _abi.lib.sbk_swa_prefill_q8_workspace_bytes(n_seqs, max_query_len, max_blocks, kvh, D, block_size, window_left)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
@@ -884,10 +898,13 @@ def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    v_scale: torch.Tensor, block_tables: torch.Tensor, query_start_loc: torch.Tensor,
                    context_lens: torch.Tensor, max_query_len: int, *, window_left: int, scale: Optional[float] = None,
                    out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
-                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   status: Optional[torch.Tensor] = None, max_seq_len: Optional[int] = None) -> torch.Tensor:
     """Sliding-window attention of runs of query tokens (q [T, H, D] bf16, token-major) over the 8-bit paged cache, the
     runs' own K/V already appended; arguments as in swa_prefill. ``workspace`` (swa_prefill_q8_workspace): kept by callers
-    that must not allocate."""
+    that must not allocate. ``max_seq_len``: no sequence is longer, its run included. Worth giving with a block table much
+    wider than that and no window: the dense rows of long runs are laid out for what a sequence can hold at the most, and
+    sequences that do not fit 256 MiB together are served one after the other. Tokens behind it are treated like those
+    behind the end of the table."""
     dev = _one_device(q, k_cache, v_cache, k_scale, v_scale, block_tables, query_start_loc, context_lens, out, workspace, status)
     nb, bs, kvh, d, cs, ss = _q8_geometry(k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != d or q.dtype != torch.bfloat16:
@@ -904,6 +921,9 @@ def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not _heads_contiguous(out):
         raise ValueError("out must be bf16 [T, H, D] with contiguous heads")
     max_query_len = int(max_query_len)
+    columns = _prefill_q8_columns(max_blocks, bs, kvh, max_query_len, window_left, max_seq_len)
+    if columns < max_blocks:
+        block_tables, max_blocks = block_tables[:, :columns].contiguous(), columns
     if workspace is None and n_seqs:
         workspace = swa_prefill_q8_workspace(n_seqs, max_query_len, max_blocks, kvh, d, q.device, block_size=bs,
                                              window_left=window_left)

@@ -229,3 +229,67 @@ def test_tokens_of_an_entry_outside_the_pool_take_no_part(ops, new, H, kvh, bs, 
     else:
         out = _attend(ops, q, codes, scales, table, ctx, news, wl, status=2)
         _check(out, None, ref.runs(*dev, ctx, news, wl, SCALE, weights=_weights_of(news)))
+
+
+# ------------------------------------------------------------------------------------- block tables much wider than the sequences
+def test_the_bound_on_the_lengths_bounds_the_workspace(ops):
+    size = lambda mq, mb, wl, kvh=4, **kw: ops.swa_prefill_q8_workspace(3, mq, mb, kvh, 128, "cpu", block_size=16, window_left=wl, **kw).numel()
+    wide, tight = 65536, 20                                                # columns: 2^20 tokens, 320 tokens
+    assert size(17, wide, -1) >= 2 ** 31                                   # one sequence's worth of dense rows
+    assert size(17, wide, -1, max_seq_len=320) == size(17, tight, -1) < 2 ** 22
+    assert size(17, wide, -1, max_seq_len=305) == size(17, tight, -1)
+    assert size(17, wide, 200, max_seq_len=320) == size(17, wide, 200)     # (the window bounds them already)
+    assert size(17, tight, -1, max_seq_len=10 ** 6) == size(17, tight, -1)
+    assert size(4, wide, -1, max_seq_len=320) == size(4, wide, -1)         # short runs need none
+    assert size(4, wide, -1, kvh=3, max_seq_len=320) == size(4, tight, -1, kvh=3)
+
+
+@gpu
+@pytest.mark.parametrize("wl", [-1, 50])
+def test_short_sequences_behind_a_wide_table(ops, wl):
+    """Sequences that do not fit the scratch together are served in turn (two at a time here), or, with a bound on their lengths, at
+    once: the same values."""
+    H, kvh = 28, 4
+    ctx, new = [100, 0, 37, 300, 250], [20, 40, 17, 33, 18]
+    lens = [a + b for a, b in zip(ctx, new)]
+    codes, scales, table = _pool(lens, -1, kvh, 128, 16, seed=250, spread=0.5, n_new=new)
+    table = torch.cat([table, torch.full((5, 4096 - table.shape[1]), -1, dtype=torch.int32)], 1)
+    q = torch.randn(sum(new), H, 128, generator=torch.Generator().manual_seed(251)).bfloat16()
+    plain = _attend(ops, q, codes, scales, table, ctx, new, wl)
+    bound = _attend(ops, q, codes, scales, table, ctx, new, wl, max_seq_len=max(lens))
+    ws = ops.swa_prefill_q8_workspace(5, 40, 4096, kvh, 128, DEV, block_size=16, window_left=wl, max_seq_len=max(lens))
+    given = _attend(ops, q, codes, scales, table, ctx, new, wl, max_seq_len=max(lens), workspace=ws)
+    want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=ref.TWO_BF16)
+    _check(plain, None, want)
+    assert torch.equal(bound, plain) and torch.equal(given, plain)
+    # a bound that does not hold: reported
+    if wl < 0:
+        short = _attend(ops, q, codes, scales, table, ctx, new, wl, max_seq_len=320, status=2)
+        keep = torch.ones(sum(new), dtype=torch.bool, device=DEV)
+        keep[77 + 20:77 + 33] = False                                      # the queries of sequence 3 behind token 320
+        assert torch.equal(short[keep], plain[keep])
+
+
+@gpu
+def test_backend_prompt_behind_a_wide_table_takes_little_memory(ops):
+    from tests.test_kv_q8 import _impl, _meta
+    H, kvh, D, bs = 28, 4, 128, 16
+    ctx, new = [30, 0], [50, 20]
+    impl = _impl(window=None)
+    table = torch.full((2, 8192), -1, dtype=torch.int32, device=DEV)       # room for 131072 tokens each
+    table[0, :6], table[1, :6] = torch.arange(6, device=DEV), torch.arange(6, 12, device=DEV)
+    kv, sc = ops.kv_cache_q8(12, bs, kvh, D, device=DEV)
+    slots = torch.cat([torch.arange(30, 80, device=DEV), 96 + torch.arange(20, device=DEV)])
+    old = torch.cat([torch.arange(30, device=DEV)])
+    k0, v0 = (_rows((30, kvh, D), 260 + i).bfloat16().to(DEV) for i in range(2))
+    ops.kv_append_q8(k0, v0, kv[0], kv[1], sc[0], sc[1], old)
+    q, k, v = (_rows((70, h, D), 262 + i).bfloat16().to(DEV) for i, h in enumerate((H, kvh, kvh)))
+    out = torch.empty(70, H * D, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    impl.forward(None, q, k, v, None, None, None, kv, _meta(ctx, new, 2, table, slots, DEV), output=out, kv_scales=sc)
+    assert torch.cuda.max_memory_allocated() - before < 8 * 2 ** 20
+    assert impl.status() == 0
+    _check(out.view(70, H, D), None, ref.runs(q, kv, sc, table, ctx, new, -1, D ** -0.5, weights=ref.TWO_BF16))
