@@ -80,9 +80,10 @@ struct Cfg {
   static constexpr int kPreOff = kInfoOff + kStages * (int)sizeof(StageInfo);
   static constexpr int kLensOff = kPreOff + (kMaxSeqs + 4) * 4;
   static constexpr int kCntOff = kLensOff + kMaxSeqs * 4;
-  static constexpr int kMlOff = kCntOff + kMaxSeqs;              // (m, l) of every warp's heads at the end of an item
-  static constexpr int kBarOff = kMlOff + kWarps * 64;
-  static constexpr int kMiscOff = kBarOff + 2 * kStages * 8;
+  static constexpr int kMlFloats = NQ > 1 ? 20 : 16;             // (m, l) of a warp's heads at the end of an item, the dims that are NaN
+  static constexpr int kMlOff = kCntOff + kMaxSeqs;
+  static constexpr int kBarOff = kMlOff + kWarps * kMlFloats * 4;
+  static constexpr int kMiscOff = kBarOff + (2 * kStages + 1) * 8;
   static constexpr int kSmemBytes = kMiscOff + 64 + 1024;        // + slack to align the ring to 1 KiB
   static_assert(kSmemBytes * kCtasPerSm <= 230400, "the CTAs of an SM must fit its shared memory");
   static_assert(kWarps * kMergeWarpBytes <= kStageBytes, "the merge scratch lives inside one stage");
@@ -157,8 +158,28 @@ __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
 }
 __device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
-template <int N>
-__device__ __forceinline__ void consumer_bar() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
+
+// mbar_wait_bounded as one statement: as a loop of the language it cost runs of four 7 us of 115, by what the compiler made of the code
+// around it
+__device__ __forceinline__ uint32_t meet_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      " .reg .pred p, q;\n"
+      " .reg .u32 n;\n"
+      " mov.u32 n, 0;\n"
+      "again:\n"
+      " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " add.u32 n, n, 1;\n"
+      " setp.lt.and.u32 q, n, 0x1000000, !p;\n"
+      " @q bra again;\n"
+      " selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
 
 template <typename TO> __device__ __forceinline__ void store2(TO* p, float a, float b);
 template <> __device__ __forceinline__ void store2<float>(float* p, float a, float b) { p[0] = a; p[1] = b; }
@@ -200,7 +221,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   int* pre = reinterpret_cast<int*>(smem + C::kPreOff);
   int* tops = reinterpret_cast<int*>(smem + C::kLensOff);
   uint8_t* cnts = smem + C::kCntOff;
-  const uint32_t bar_full = ring + C::kBarOff, bar_empty = bar_full + 8 * kStages;
+  const uint32_t bar_full = ring + C::kBarOff, bar_empty = bar_full + 8 * kStages, bar_meet = bar_empty + 8 * kStages;
   volatile int* misc = reinterpret_cast<volatile int*>(smem + C::kMiscOff);   // [0] abort, [1] longest, [2..] scan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 kNotCut = make_int4(-1, 0, 0, 0);
@@ -216,6 +237,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       mbar_init(bar_full + 8 * s, 1 + 32);   // the stage's bytes, and each producer lane's exponents
       mbar_init(bar_empty + 8 * s, C::kWarps);
     }
+    mbar_init(bar_meet, C::kWarps);
     misc[0] = 0;
     misc[1] = 0;
     pre[0] = 0;
@@ -491,12 +513,23 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       m[0][0] = x.x; m[0][1] = x.y; rs[0][0] = x.z; rs[0][1] = x.w;
     }
   };
+  auto waited = [&](bool ok) {
+    if (!ok && lane == 0) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); misc[0] = 1; }
+    return ok;
+  };
+  // The consumer warps meet (bounded like every wait: a warp that gave up does not come), an even number of times in an item unless
+  // it has one query and a warp to every kv head: so the phase is known where they meet. Who waited in vain goes on to the end of the
+  // item (in bounds, with values that the status disowns), which costs no registers where leaving at once would.
+  uint32_t met = 1;
+  auto meet = [&](uint32_t phase) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_meet);
+    met &= meet_wait(bar_meet, phase);
+  };
+  uint32_t odd_item = 0;
   for (int it = 0;; ++it) {
     const int s = it % kStages;
-    if (!mbar_wait_bounded(bar_full + 8 * s, (it / kStages) & 1)) {
-      if (lane == 0) { raise_status(P.status, SBK_ST_WAIT_TIMEOUT); misc[0] = 1; }
-      return;
-    }
+    if (!waited(mbar_wait_bounded(bar_full + 8 * s, (it / kStages) & 1))) return;
     const StageInfo si = info[s];
     if (si.flags & kEnd) return;
     const uint32_t stage = ring + s * kStageBytes;
@@ -807,7 +840,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
     // warps that share a kv head (each took other tokens) are added up from there
     uint8_t* mbuf = smem + s * kStageBytes;
     float* wo = reinterpret_cast<float*>(mbuf + warp * kMergeWarpBytes);
-    float* wml = reinterpret_cast<float*>(smem + C::kMlOff) + warp * 16;
+    float* wml = reinterpret_cast<float*>(smem + C::kMlOff) + warp * C::kMlFloats;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int r = C::kShare ? 0 : n;
@@ -820,7 +853,8 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         for (int off = 4; off < 32; off <<= 1) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], off);
         fix[i] = 1.f / rs[r][i];
       }
-      consumer_bar<C::kConsumers>();          // every warp is done reading this stage, or the results of the query before
+      // every warp is done reading this stage, or the results of the query before
+      meet(kSub > 1 ? 0u : (NQ > 1 ? (uint32_t)n & 1u : odd_item));
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
 #pragma unroll
@@ -833,7 +867,9 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
         wml[2 * t] = m[r][0]; wml[2 * t + 1] = m[r][1];
         wml[8 + 2 * t] = l[n][0]; wml[8 + 2 * t + 1] = l[n][1];
       }
-      if constexpr (kSub > 1) consumer_bar<C::kConsumers>(); else __syncwarp();
+      if constexpr (NQ > 1)
+        if (lane < 4) wml[16 + lane] = __uint_as_float(nan_sh[n * 4 + lane]);
+      if (kSub == 1) __syncwarp(); else meet(1u);
       if (n < si.n_q) {
         const int64_t orow = (int64_t)si.row + n;
         const int64_t prow = ((int64_t)(2 * me + (si.part > 0 ? 1 : 0)) * kCap + n) * P.H;
@@ -845,7 +881,7 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           float M = -INFINITY;
 #pragma unroll
           for (int w2 = 0; w2 < kSub; ++w2)
-            M = fmaxf(M, reinterpret_cast<const float*>(smem + C::kMlOff)[(kh + KVH * w2) * 16 + row]);
+            M = fmaxf(M, reinterpret_cast<const float*>(smem + C::kMlOff)[(kh + KVH * w2) * C::kMlFloats + row]);
           const float Ms = fmaxf(M, kNegBig);
           float L = 0.f;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -853,13 +889,13 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
           for (int w2 = 0; w2 < kSub; ++w2) {
             const int src = kh + KVH * w2;
             const float* po = reinterpret_cast<const float*>(mbuf + src * kMergeWarpBytes);
-            const float* ml = reinterpret_cast<const float*>(smem + C::kMlOff) + src * 16;
+            const float* ml = reinterpret_cast<const float*>(smem + C::kMlOff) + src * C::kMlFloats;
             const float wgt = kSub > 1 ? fast_exp2(ml[row] - Ms) : 1.f;
             const float4 o = *reinterpret_cast<const float4*>(po + row * kD + ((4 * lane) ^ ((row & 7) << 2)));
             L += ml[8 + row] * wgt;
             O.x += o.x * wgt; O.y += o.y * wgt; O.z += o.z * wgt; O.w += o.w * wgt;
             if constexpr (NQ > 1) {
-              const uint32_t nan = reinterpret_cast<const uint32_t*>(smem + C::kNanOff)[(src * NQ + n) * 4 + (lane >> 3)] >> (4 * (lane & 7));
+              const uint32_t nan = __float_as_uint(ml[16 + (lane >> 3)]) >> (4 * (lane & 7));
               if (nan & 1u) O.x = __uint_as_float(0x7fffffffu);
               if (nan & 2u) O.y = __uint_as_float(0x7fffffffu);
               if (nan & 4u) O.z = __uint_as_float(0x7fffffffu);
@@ -878,8 +914,10 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
       }
     }
     fence_proxy_async_smem();               // these accesses precede the copies that refill the stage
-    if constexpr (kSub > 1) consumer_bar<C::kConsumers>(); else __syncwarp();
+    if (!waited(met)) return;
+    __syncwarp();
     if (lane == 0) mbar_arrive(bar_empty + 8 * s);
+    odd_item ^= 1u;
   }
 }
 
