@@ -338,8 +338,8 @@ int sbk_kv_gather_q8(const void* k_cache, const void* v_cache, const void* k_sca
  *               max_query_len keys, or max_blocks * block_size where that is less, 512 kvh bytes each. Sequences share 256
  *               MiB, or one sequence's worth where that is more, in turn: without a window, a table no wider than the longest
  *               sequence keeps both the workspace and the number of turns small. Else partial results, as for single tokens.
- * Supported: D == 128, H % kvh == 0, H/kvh <= 8, block_size % 16 == 0; sbk_swa_decode_q8: kvh in {1,2,4}; sbk_swa_prefill_q8:
- * q, out 16-byte aligned with token strides that are multiples of 8 elements.
+ * Supported: D == 128, H % kvh == 0, H/kvh <= 8, block_size % 16 == 0, max_blocks * block_size at most 2^30 tokens; sbk_swa_decode_q8:
+ * kvh in {1,2,4}; sbk_swa_prefill_q8: q, out 16-byte aligned with token strides that are multiples of 8 elements.
  */
 size_t sbk_swa_decode_q8_workspace_bytes(int B, int H, int D);
 int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void* k_cache, const void* v_cache,

@@ -1151,6 +1151,10 @@ extern "C" int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void
     set_error("sbk_swa_decode_q8: block_size=%d must be a positive multiple of 16", block_size);
     return SBK_E_ARG;
   }
+  if ((int64_t)max_blocks * block_size > kMaxWidth) {
+    set_error("sbk_swa_decode_q8: a table of %d blocks of %d tokens spans more than 2^30 tokens", max_blocks, block_size);
+    return SBK_E_ARG;
+  }
   if (out_dtype != SBK_BF16 && out_dtype != SBK_F32) {
     set_error("sbk_swa_decode_q8: out_dtype=%d unsupported", out_dtype);
     return SBK_E_ARG;

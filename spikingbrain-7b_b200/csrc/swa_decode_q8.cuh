@@ -7,6 +7,9 @@
 namespace sbk {
 namespace decode_q8 {
 
+// tokens that a row of the block table may span: positions, and what is added to them, are 32-bit numbers
+constexpr int64_t kMaxWidth = (int64_t)1 << 30;
+
 struct Call {
   const void* q; int64_t q_stride;                       // elements between rows
   const void* k_cache; const void* v_cache; const void* k_scale; const void* v_scale;

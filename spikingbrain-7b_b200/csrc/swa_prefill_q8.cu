@@ -624,6 +624,10 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     set_error("sbk_swa_prefill_q8: null pointer or max_blocks=%d", max_blocks);
     return SBK_E_ARG;
   }
+  if ((int64_t)max_blocks * block_size > decode_q8::kMaxWidth) {
+    set_error("sbk_swa_prefill_q8: a table of %d blocks of %d tokens spans more than 2^30 tokens", max_blocks, block_size);
+    return SBK_E_ARG;
+  }
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_scale) || !aligned16(v_scale) ||
       cache_block_stride_bytes % 16 || scale_block_stride_bytes % 16 || !aligned16(q) || !aligned16(out) || q_tok_stride % 8 ||
       out_tok_stride % 8) {

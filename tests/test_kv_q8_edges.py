@@ -293,3 +293,41 @@ def test_backend_prompt_behind_a_wide_table_takes_little_memory(ops):
     assert torch.cuda.max_memory_allocated() - before < 8 * 2 ** 20
     assert impl.status() == 0
     _check(out.view(70, H, D), None, ref.runs(q, kv, sc, table, ctx, new, -1, D ** -0.5, weights=ref.TWO_BF16))
+
+
+A = 1 << 20          # an aligned address that is never dereferenced: the calls below are refused on the host
+
+
+@pytest.mark.parametrize("blocks,block", [(2 ** 26 + 1, 16), (32768, 65536), (2 ** 31 - 1, 16), (2 ** 30 // 48 + 1, 48)])
+def test_tables_beyond_32_bit_positions_are_refused(sb, blocks, block):
+    from spikingbrain_7b_b200 import _abi
+    scale, cs, ss = ctypes.c_float(0.1), 4 * 128 * block, 4 * block
+    assert _abi.lib.sbk_swa_decode_q8(A, 3584, A, A, A, A, A, blocks, A, 2, 28, 4, 128, 8, block, cs, ss, 15, scale, A, 0, 3584, None, A,
+                                      1 << 40, None, None) == -1
+    assert b"2^30" in _abi.lib.sbk_last_error()
+    for most in (5, 40):
+        assert _abi.lib.sbk_swa_prefill_q8(A, 3584, A, A, A, A, A, blocks, A, A, 2, most, 28, 4, 128, 8, block, cs, ss, 15, scale, A, 3584, A,
+                                           1 << 40, None, None) == -1
+        assert b"2^30" in _abi.lib.sbk_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("new", [None, 3, 20])
+def test_the_last_positions_of_the_widest_table(ops, new):
+    """2^30 tokens of room; one sequence that fills it, one that claims 2^31 - 1 (clamped to 2^30 tokens of context in runs)."""
+    H, kvh, bs, n, wl = 7, 1, 65536, new or 1, 40
+    g = torch.Generator().manual_seed(270)
+    codes = torch.randn(2, 2, bs, kvh, 128, generator=g).to(torch.float8_e4m3fn)
+    scales = torch.full((2, 2, kvh, bs), 126, dtype=torch.uint8)
+    table = torch.full((2, 16384), -1, dtype=torch.int32)
+    table[:, -1] = 1
+    ctx = [2 ** 30 - n, 2 ** 31 - 1 - n]
+    q = torch.randn(2 * n, H, 128, generator=g).bfloat16()
+    dev = [t.to(DEV) for t in (q, codes, scales, table)]
+    if new is None:
+        out = _attend(ops, q, codes, scales, table, [2 ** 30, 2 ** 31 - 1], None, wl, status=2)
+        want = ref.decode(*dev, [2 ** 30, 2 ** 31 - 1], wl, SCALE, ref.FP16)
+    else:
+        out = _attend(ops, q, codes, scales, table, ctx, [n, n], wl, status=2)
+        want = ref.runs(*dev, [ctx[0], 2 ** 30], [n, n], wl, SCALE, weights=_weights_of([n]))
+    _check(out, None, want)
