@@ -1174,6 +1174,10 @@ extern "C" int sbk_swa_decode_q8(const void* q, int64_t q_seq_stride, const void
     set_error("sbk_swa_decode_q8: a block stride is smaller than the block it spans");
     return SBK_E_ARG;
   }
+  if (B > 1 && out_seq_stride < (int64_t)H * D) {
+    set_error("sbk_swa_decode_q8: the rows of out overlap");
+    return SBK_E_ARG;
+  }
   const size_t need = sbk_swa_decode_q8_workspace_bytes(B, H, D);
   if (!workspace || workspace_bytes < need) {
     set_error("sbk_swa_decode_q8: workspace of %zu bytes given, %zu needed", workspace ? workspace_bytes : 0, need);

@@ -638,6 +638,10 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     set_error("sbk_swa_prefill_q8: a block stride is smaller than the block it spans");
     return SBK_E_ARG;
   }
+  if (out_tok_stride < (int64_t)H * D) {
+    set_error("sbk_swa_prefill_q8: the rows of out overlap");
+    return SBK_E_ARG;
+  }
   const size_t need = sbk_swa_prefill_q8_workspace_bytes(n_seqs, max_query_len, max_blocks, kvh, D, block_size, window_left);
   if (!workspace || workspace_bytes < need) {
     set_error("sbk_swa_prefill_q8: workspace of %zu bytes given, %zu needed", workspace ? workspace_bytes : 0, need);

@@ -331,3 +331,15 @@ def test_the_last_positions_of_the_widest_table(ops, new):
         out = _attend(ops, q, codes, scales, table, ctx, [n, n], wl, status=2)
         want = ref.runs(*dev, [ctx[0], 2 ** 30], [n, n], wl, SCALE, weights=_weights_of([n]))
     _check(out, None, want)
+
+
+def test_overlapping_output_rows_are_refused(sb):
+    from spikingbrain_7b_b200 import _abi
+    decode = lambda B, stride: _abi.lib.sbk_swa_decode_q8(A, 3584, A, A, A, A, A, 4, A, B, 28, 4, 128, 8, 16, 8192, 64, 15, ctypes.c_float(0.1), A, 0,
+                                                          stride, None, None, 0, None, None)
+    assert decode(2, 0) == decode(2, 3576) == -1 and b"overlap" in _abi.lib.sbk_last_error()
+    assert decode(1, 0) == decode(2, 3584) == -3                           # (the next check: no workspace)
+    for most in (5, 40):
+        assert _abi.lib.sbk_swa_prefill_q8(A, 3584, A, A, A, A, A, 4, A, A, 2, most, 28, 4, 128, 8, 16, 8192, 64, 15, ctypes.c_float(0.1), A, 0,
+                                           None, 0, None, None) == -1
+        assert b"overlap" in _abi.lib.sbk_last_error()
