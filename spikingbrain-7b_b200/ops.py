@@ -920,6 +920,8 @@ def swa_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         out = q.new_empty((T, H, d))
     elif out.shape != (T, H, d) or out.dtype != torch.bfloat16 or not _heads_contiguous(out):
         raise ValueError("out must be bf16 [T, H, D] with contiguous heads")
+    if not T:                                    # (every run is empty)
+        return out
     max_query_len = int(max_query_len)
     columns = _prefill_q8_columns(max_blocks, bs, kvh, max_query_len, window_left, max_seq_len)
     if columns < max_blocks:

@@ -343,3 +343,14 @@ def test_overlapping_output_rows_are_refused(sb):
         assert _abi.lib.sbk_swa_prefill_q8(A, 3584, A, A, A, A, A, 4, A, A, 2, most, 28, 4, 128, 8, 16, 8192, 64, 15, ctypes.c_float(0.1), A, 0,
                                            None, 0, None, None) == -1
         assert b"overlap" in _abi.lib.sbk_last_error()
+
+
+@gpu
+def test_calls_without_queries_give_empty_outputs(ops):
+    kv, sc = ops.kv_cache_q8(4, 16, 4, 128, device=DEV)
+    table = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+    q = torch.zeros(0, 28, 128, dtype=torch.bfloat16, device=DEV)
+    for most in (0, 1, 40):
+        out = ops.swa_prefill_q8(q, kv[0], kv[1], sc[0], sc[1], table, _i32(0, 0, 0), _i32(3, 5), most, window_left=-1)
+        assert out.shape == (0, 28, 128)
+    assert ops.swa_decode_q8(q, kv[0], kv[1], sc[0], sc[1], table[:0], _i32(), window_left=-1).shape == (0, 28, 128)
