@@ -354,3 +354,41 @@ def test_calls_without_queries_give_empty_outputs(ops):
         out = ops.swa_prefill_q8(q, kv[0], kv[1], sc[0], sc[1], table, _i32(0, 0, 0), _i32(3, 5), most, window_left=-1)
         assert out.shape == (0, 28, 128)
     assert ops.swa_decode_q8(q, kv[0], kv[1], sc[0], sc[1], table[:0], _i32(), window_left=-1).shape == (0, 28, 128)
+
+
+@gpu
+@pytest.mark.parametrize("new", [None, 4, 40])
+def test_repeated_calls_on_two_streams_and_from_two_graphs_give_the_same_bits(ops, new):
+    """No atomics whose order changes a sum, no workspace shared between calls that may overlap."""
+    H, kvh, n = 28, 4, new or 1
+    ctx = [3000, 200, 5000, 0, 1111]
+    lens = [c + n for c in ctx]
+    codes, scales, table = (t.to(DEV) for t in _pool(lens, 2000, kvh, 128, 16, seed=280, n_new=[n] * 5))
+    qs = [_rows((5 * n, H, 128), 281 + i).bfloat16().to(DEV) for i in range(2)]
+    lens_d, ctx_d, start = _i32(*lens), _i32(*ctx), _starts([n] * 5)
+
+    def call(i):
+        if new is None:
+            return ops.swa_decode_q8(qs[i], *codes, *scales, table, lens_d, window_left=2000)
+        return ops.swa_prefill_q8(qs[i], *codes, *scales, table, start, ctx_d, n, window_left=2000)
+    want = [call(i).clone() for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    for i in range(2):
+        streams[i].wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i]):
+            outs.append(call(i))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        eager = []
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+                eager.append(call(i))
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[i]) and torch.equal(eager[i], want[i])
+            outs[i].fill_(0.0)
+        torch.cuda.synchronize()
