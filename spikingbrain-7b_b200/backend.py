@@ -489,7 +489,8 @@ class MetaAttentionImpl:
         if layer is not None:
             assert (getattr(layer, "_k_scale_float", 1.0) == 1.0
                     and getattr(layer, "_v_scale_float", 1.0) == 1.0), (
-                "key/v_scale is only supported with an fp8 cache, which this path does not have")
+                "calibrated key/value scales belong to a cache with one scale per tensor, which this backend does not have (with "
+                "kv_cache_dtype \"fp8_e4m3\" the append makes an exponent per token and head, in kv_scales)")
         if (key2 is None) != (value2 is None):
             raise ValueError("key2 and value2 come together")
         q8 = self.kv_cache_dtype == "fp8_e4m3"

@@ -392,3 +392,14 @@ def test_repeated_calls_on_two_streams_and_from_two_graphs_give_the_same_bits(op
             assert torch.equal(outs[i], want[i]) and torch.equal(eager[i], want[i])
             outs[i].fill_(0.0)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["auto", "fp8_e4m3"])
+def test_backend_says_why_it_takes_no_calibrated_scales(sb, dtype):
+    from types import SimpleNamespace
+    from tests.test_kv_q8 import _impl, _meta
+    q, k = torch.zeros(1, 28, 128).bfloat16(), torch.zeros(1, 4, 128).bfloat16()
+    md = _meta([3], [1], 0, torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int64), "cpu")
+    with pytest.raises(AssertionError, match="one scale per tensor"):
+        _impl(dtype).forward(SimpleNamespace(_k_scale_float=0.5, _v_scale_float=1.0), q, k, k, None, None, None,
+                             torch.zeros(2, 4, 16, 4, 128, dtype=torch.uint8), md, output=torch.empty_like(q))
