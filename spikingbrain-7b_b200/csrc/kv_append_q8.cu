@@ -15,11 +15,6 @@ namespace sbk {
 namespace q8 {
 
 using namespace tc5;                  // packed fp32 pairs
-__device__ __forceinline__ f32x2 fmul2(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 template <typename T> struct Vec8;   // eight elements of a row
 template <> struct Vec8<__nv_bfloat16> {

@@ -134,11 +134,6 @@ __device__ __forceinline__ void widen(uint32_t (&a)[4], uint32_t lo, uint32_t hi
   a[0] = q8::e4m3x2_to_f16x2(lo & 0xffffu); a[1] = q8::e4m3x2_to_f16x2(hi & 0xffffu);
   a[2] = q8::e4m3x2_to_f16x2(lo >> 16); a[3] = q8::e4m3x2_to_f16x2(hi >> 16);
 }
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 // two 16 x 16 byte matrices, transposed: lane 4g + t gets column g (r0) and g + 8 (r1) of the first, rows 4t ... 4t+3, and the
 // same of the second (r2, r3); lanes 0-15 name the rows of the first matrix, 16-31 those of the second
 __device__ __forceinline__ void ldmatrix_b8_trans(uint32_t (&r)[4], uint32_t addr) {
@@ -198,11 +193,6 @@ __device__ __forceinline__ float row_lse(float m, float l) { return l != 0.f ? (
 __device__ __forceinline__ float inverse(float l) { return l != 0.f ? 1.f / l : 0.f; }
 
 using namespace tc5;                  // packed fp32 pairs
-__device__ __forceinline__ f32x2 fmul2(f32x2 a, f32x2 b) {
-  f32x2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 template <int KVH, int NQ, typename TO>
 __global__ void __launch_bounds__(Cfg<NQ>::kThreads, Cfg<NQ>::kCtasPerSm)
