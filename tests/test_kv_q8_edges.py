@@ -403,3 +403,29 @@ def test_backend_says_why_it_takes_no_calibrated_scales(sb, dtype):
     with pytest.raises(AssertionError, match="one scale per tensor"):
         _impl(dtype).forward(SimpleNamespace(_k_scale_float=0.5, _v_scale_float=1.0), q, k, k, None, None, None,
                              torch.zeros(2, 4, 16, 4, 128, dtype=torch.uint8), md, output=torch.empty_like(q))
+
+
+@gpu
+@pytest.mark.parametrize("lens,wl,H,kvh", [([1, 17, 300, 2050, 0], 1024, 28, 4), ([30011, 6000], -1, 7, 1), ([8193] * 3, 4096, 14, 2),
+                                           ([1500] * 160, 1000, 28, 4)])
+def test_single_tokens_hold_their_weights_in_fp16(ops, lens, wl, H, kvh):
+    codes, scales, table = _pool(lens, wl, kvh, 128, 16, seed=290, spread=0.5)
+    q = torch.randn(len(lens), H, 128, generator=torch.Generator().manual_seed(291)).bfloat16()
+    want = ref.decode(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), lens, wl, SCALE, ref.FP16)
+    for dtype in (torch.float32, torch.bfloat16):
+        lse = torch.empty(len(lens), H, device=DEV)
+        out = _attend(ops, q, codes, scales, table, lens, None, wl, out_dtype=dtype, lse=lse)
+        _check(out, lse, want)
+        assert mean_rel(out.float(), want[0].to(dtype).float()) <= MEAN_REL
+
+
+@gpu
+@pytest.mark.parametrize("ctx,new,wl,H,kvh", [([4200] * 8, [4] * 8, 4096, 28, 4), ([30000, 7], [16, 5], -1, 7, 1), ([900, 0, 2000], [2, 1, 2], 700, 14, 2)])
+def test_short_runs_hold_their_weights_in_fp16(ops, ctx, new, wl, H, kvh):
+    lens = [a + b for a, b in zip(ctx, new)]
+    codes, scales, table = _pool(lens, wl, kvh, 128, 16, seed=292, spread=0.5, n_new=new)
+    q = torch.randn(sum(new), H, 128, generator=torch.Generator().manual_seed(293)).bfloat16()
+    out = _attend(ops, q, codes, scales, table, ctx, new, wl)
+    want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=ref.FP16)
+    _check(out, None, want)
+    assert mean_rel(out.float(), want[0].bfloat16().float()) <= MEAN_REL
