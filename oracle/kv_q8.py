@@ -57,8 +57,9 @@ class Weights(NamedTuple):
 # One number in fp16 (half a step: 2^-11). The largest one of a query is at least 2^6 when its offset is chosen, so half of
 # fp16's smallest step, 2^-25, is 2^-31 of it at the most.
 FP16 = Weights(2.0 ** -11, 2.0 ** -31, 17)
-# Two bf16 numbers: the first is off by 2^-8 of the weight, the second by 2^-8 of that rest. No floor (bf16 has fp32's exponents).
-TWO_BF16 = Weights(2.0 ** -16, 0.0, 34)
+# Two bf16 numbers: the first is cut off, so the rest is under 2^-7 of the weight; the second is rounded, off by 2^-8 of that rest. No
+# floor (bf16 has fp32's exponents).
+TWO_BF16 = Weights(2.0 ** -15, 0.0, 34)
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seen: torch.Tensor, scale: float, weights: Optional[Weights] = None):

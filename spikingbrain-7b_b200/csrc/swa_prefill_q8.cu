@@ -12,7 +12,7 @@
 //        warps 0-3  :  softmax A(0)  |                 | softmax A(1)    ...
 //        warps 4-7  :                | softmax B(0)    |                 ...
 //    Unlike there V is bf16 (a V row may have any exponent, which fp16 does not hold), and P goes in as a bf16 head and a bf16 remainder,
-//    two products, so that it loses 2^-16 of itself (the head alone loses 2^-8, as much as the output's own rounding: mean relative
+//    two products, so that it loses 2^-15 of itself (the head alone loses 2^-8, as much as the output's own rounding: mean relative
 //    error 1.6e-3 against 64 bits, over the 1e-3 that the framework's attention kernels keep). Nothing has to be converted, and a tile of
 //    128 keys is one copy per 64 dims.
 //    Tensor memory (512 columns): S_A / P_A [0,128), S_B / P_B [128,256), O_A [256,384), O_B [384,512). The softmax offset of a row
@@ -175,6 +175,16 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(r));
   return r != 0;
+}
+
+// Two weights as packed bf16 heads and packed bf16 remainders: the heads are cut off (one instruction for both), not rounded, so
+// a remainder is under 2^-7 of the weight, and its rounding under 2^-15. (Rounded heads: 714 us against 702 on 8192 queries.)
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+  float ra, rb;
+  unpack2(ffma2(pack2(__uint_as_float(__float_as_uint(a) & 0xffff0000u), __uint_as_float(__float_as_uint(b) & 0xffff0000u)),
+                pack2(-1.f, -1.f), pack2(a, b)), ra, rb);
+  lo = pack_bf16x2(ra, rb);
 }
 
 // ---- 2. attention of the runs over the dense rows ----
@@ -479,8 +489,8 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                 const float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
                 la = fadd2(la, pack2(e0, e1));
                 lb = fadd2(lb, pack2(e2, e3));
-                split_bf16x2(e0, e1, ph[i >> 1], ph[16 + (i >> 1)]);
-                split_bf16x2(e2, e3, ph[(i >> 1) + 1], ph[17 + (i >> 1)]);
+                split2(e0, e1, ph[i >> 1], ph[16 + (i >> 1)]);
+                split2(e2, e3, ph[(i >> 1) + 1], ph[17 + (i >> 1)]);
               }
               float a0, a1, b0, b1;
               unpack2(la, a0, a1);
@@ -495,7 +505,7 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
                 if (__uint_as_float(sr[i + 1]) == -INFINITY) pb = 0.f;
                 ls[i & 3] += pa;
                 ls[(i + 1) & 3] += pb;
-                split_bf16x2(pa, pb, ph[i >> 1], ph[16 + (i >> 1)]);
+                split2(pa, pb, ph[i >> 1], ph[16 + (i >> 1)]);
               }
             }
             tmem_st32(s_col + col0, ph);
@@ -564,8 +574,9 @@ attend_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
 }
 
 // Runs of at most kFew queries go through the kernel of the single tokens, which reads the cache once for four queries and
-// expands nothing. Measured there against here, us, window 4096 on 8190 cached tokens: 64 runs of 8 187 / 375, of 16 336 / 384, of
-// 20 407 / 390; 256 runs of 16 1160, of 20 1495 / 1346; 8 of 20 76 / 89; one of 20 34 / 70.
+// expands nothing. Measured there against here, us, window 4096 on 8190 cached tokens: 256 runs of 16 1170 / 1348, of 17 1483 / 1348;
+// 64 of 8 197 / 401, of 16 348 / 410, of 20 410 / 428, of 24 481 / 430. With fewer sequences the border lies higher, and what is in
+// between loses here: 8 runs of 20 84 / 109, of 32 113 / 111; one of 20 51 / 94, of 128 74 / 92, of 300 125 / 96.
 constexpr int kFew = 16;
 static bool few_queries(int max_query_len, int kvh) { return max_query_len <= kFew && (kvh == 1 || kvh == 2 || kvh == 4); }
 
@@ -723,7 +734,8 @@ extern "C" int sbk_swa_prefill_q8(const void* q, int64_t q_tok_stride, const voi
     if (rc != SBK_OK) return rc;
     P.seq0 = s0;
     // What is left for the last, partly filled round of CTAs takes one tile to a CTA if the SMs have room for twice as many: half
-    // the queries take less than a pair, though more than half of it
+    // the queries take less than a pair, though more than half of it. Against pairs throughout, us, 28 + 4 heads: 8192 queries 621 / 631,
+    // 1500 184 / 195, 4 x 700 274 / 287.
     const int64_t total = (int64_t)n * pairs * kvh;
     const int rest = (int)(total % sms);
     P.pairs_per_head = n * pairs;
