@@ -303,9 +303,13 @@ stream_kernel(const Params P, const __grid_constant__ CUtensorMap map_k, const _
   const int total = pre[P.B], n_cta = (int)gridDim.x, me = (int)blockIdx.x;
   int per = (total + n_cta - 1) / n_cta;
   if (per < 1) per = 1;
-  // A batch of near-equal items that fills the CTAs evenly streams fastest as whole items: no partials to write and fold.
+  // A batch of near-equal items that fills the CTAs evenly streams fastest as whole items: no partials to write and fold. Against
+  // cutting, us: 256 sequences of 8193, window 4096, 170 / 183; 592 equal ones 215 / 221, 10 % apart 211 / 215. Limits: rounds that are
+  // filled to 10/11 (to 10/13: 309 against 283 on 1024 items), the longest item 9/8 of the mean (11/8: 78 against 74 on 148 items 30 %
+  // apart, 166 against 158 on 592). A lone round leaves CTAs empty: it pays, whole against cut, on 200 equal items of four kv heads 96 / 102,
+  // not on 160 (86 / 84); of two on 220 (102 / 104), not on 180 (94 / 90); of one not on 148 (84 / 64) nor 220 (88 / 85).
   const int rounds = (P.B + n_cta - 1) / n_cta;
-  const bool whole = 2 * P.B >= n_cta && ((P.B <= n_cta && !C::kShare) || 10 * rounds * n_cta <= 11 * P.B) &&
+  const bool whole = (KVH == 4 ? 8 * P.B >= 5 * n_cta : 4 * P.B >= 3 * n_cta) && ((P.B <= n_cta && !C::kShare) || 10 * rounds * n_cta <= 11 * P.B) &&
                      (int64_t)misc[1] * P.B <= ((int64_t)total - (int64_t)C::kItemCost * P.B) / 8 * 9;
   auto first_row = [&](int b) {
     if (P.seq_lens) return P.item0 + b;
@@ -1021,9 +1025,12 @@ static int launch(const char* who, const Params& P0, int64_t items, int sms, con
     // no more CTAs than there can be units of work
     const int64_t most = (int64_t)P.B * per_item;
     int grid = (int)(most < n_ctas ? most : n_ctas);
-    // a batch between one and two items per SM: one CTA each, so that every SM has work either way of cutting (four queries
-    // to an item are bound by instructions, not by the copies that a lone CTA can keep up: there both CTAs of an SM share)
-    if (!C::kShare && 2 * P.B >= n_ctas && P.B < n_ctas) grid = P.B;
+    // A batch that nearly fills the CTAs, one item each: as many CTAs as items, so that every SM has work where near-equal items stay
+    // whole. Measured against all CTAs, us, equal items: 256 items 111 / 115, 290 123 / 127; where lengths differ by up to half 90 / 92. With
+    // fewer items it may only stay off: 148 equal ones 80 / 84, but 74 / 57 and 64 / 51 where lengths differ by a third and by half (7 + 1
+    // heads). (Four queries to an item are bound by instructions, not by the copies that a lone CTA can keep up: there both CTAs of an SM
+    // share.)
+    if (!C::kShare && 4 * P.B >= 3 * n_ctas && P.B < n_ctas) grid = P.B;
     P.cut_by_item = P.B < grid;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
