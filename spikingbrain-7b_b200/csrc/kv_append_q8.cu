@@ -62,7 +62,7 @@ constexpr int kAppendThreads = 128;
 // V = D / 8 vectors per row, V / 2 lanes, two vectors each: a rotated pair (j, j + half) lies in one lane, so the rotation needs
 // no exchange and its cosines are read once for both. Rows of a token: kvh of K, kvh of V, H of the query. CTAs past the
 // last row retire blocks. Bound by the latency of position -> cosines and slot -> cache (a third of the DRAM
-// rate; the issue slots are 60 % busy), so by the rows in flight: twelve CTAs of 128 threads per SM. Measured on 8192 tokens,
+// rate; the issue slots are 72 % busy), so by the rows in flight: twelve CTAs of 128 threads per SM. Measured on 8192 tokens,
 // 28 + 4 heads of 128 (142 MB, 22 us at the copy rate): 29 us; 31 us at the 47 registers the compiler takes when it may; 58 us
 // with one vector per lane and the partner's values by shuffles; 48 us with four query heads per lane group (fewer address
 // and table reads, a quarter of the threads).

@@ -4,11 +4,12 @@
 //
 // Single tokens are bound by HBM: 2 kvh (D + 1) bytes per visible token, at 14 flops a byte. 28 + 4 heads of 128, window 4096:
 //   256 sequences of 8193 tokens 170 us (1.08 GB, 6.4 TB/s); 64 of 1025 ... 32769 54 us (4.9 TB/s; 11 us of it until the first
-//   bytes come and from the last ones to the folded rows); 4 of 131072, no window, 87 us (5.8 TB/s).
+//   bytes come and from the last ones to the folded rows); 4 of 100003 ... 131072, no window, 87 us (5.8
+//   TB/s).
 // Runs of up to four queries to an item read the cache once for them, and are bound by the instructions around the products: 64 x 4
-//   queries 109 us (2.5 TB/s; 0.35 instructions issued per cycle and scheduler, eight consumer warps an SM being all that the
-//   accumulators leave room for). Two groups of four warps with two queries each, every code converted twice, took
-//   124 us; the weights of all four queries before one vote on the offsets, not query by query, 122 us.
+//   queries 115 us (2.4 TB/s; 0.35 instructions issued per cycle and scheduler, eight consumer warps an SM being all that the
+//   accumulators leave room for; 109 before values that a query does not see were kept from it). Against those 109: two groups of
+//   four warps with two queries each, every code converted twice, 124 us; the weights of all four queries before one vote on the offsets, not query by query, 122 us.
 //
 // Products. Both run on mma.sync m16n8k16 in fp16, the codes converted in registers on their way into the A operand (exact, two codes
 //   per instruction), K and V taking the 16-row side and the query heads of a kv group (at most eight) the other:

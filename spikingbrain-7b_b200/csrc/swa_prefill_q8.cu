@@ -3,8 +3,9 @@
 // 1. unpack: the keys that a run sees become dense bf16 rows, K and V [head][row][128], once. Every value of the cache is
 //    a bf16 number, so nothing is rounded. A run's rows start at a multiple of 128 and its last 128 are filled up with
 //    zeros. Each key serves (window / queries of a tile) query tiles, so expanding it in every CTA that reads it would repeat that work
-//    a hundred times over in the kernel that is short of instructions; written out once it is 3 (D + 1) kvh bytes a token,
-//    under 2 % of the time of a long run.
+//    a hundred times over in the kernel that is short of instructions; written out once it is (6 D + 2) kvh bytes a
+//    token, under 2 % of the time of a long run. What must not meet a weight of zero is kept from the second step here: NaN codes of V
+//    become a mark, tokens that the pool does not hold a bit of their tile, and a flag per tile says whether there are any.
 // 2. attend: tcgen05, two query tiles per CTA taking turns, as in swa_prefill_tc2.cu: a CTA owns 2 x (128 / G) consecutive queries of a
 //    run and one kv head as two MMA tiles A and B of 128 rows (row = query * G + head); both read the same K / V tiles in shared
 //    memory; one thread owns one row, and while the warps of A work on their scores the tensor core computes for B:
@@ -13,18 +14,18 @@
 //        warps 4-7  :                | softmax B(0)    |                 ...
 //    Unlike there V is bf16 (a V row may have any exponent, which fp16 does not hold), and P goes in as a bf16 head and a bf16 remainder,
 //    two products, so that it loses 2^-15 of itself (the head alone loses 2^-8, as much as the output's own rounding: mean relative
-//    error 1.6e-3 against 64 bits, over the 1e-3 that the framework's attention kernels keep). Nothing has to be converted, and a tile of
+//    error 1.7e-3, over the 1e-3 that the framework's attention kernels keep). Nothing has to be converted, and a tile of
 //    128 keys is one copy per 64 dims.
 //    Tensor memory (512 columns): S_A / P_A [0,128), S_B / P_B [128,256), O_A [256,384), O_B [384,512). The softmax offset of a row
 //    moves only when its maximum has grown by more than 2^8, so O is rescaled in tensor memory almost only on the first tile.
 //    Roles (384 threads): warps 0-3 softmax / epilogue of tile A, 4-7 of tile B, 8 producer of the K ring, 9 of the V ring, 10 tensor
 //    memory and MMA issue; 11 looks through the tiles' flags, and is there for its registers: the softmax warps hold a row's 128 scores
 //    at once, with what the last four warps give up. Every wait is bounded.
-// Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 725 us, 664 TFLOP/s of useful products (4 H D
-//    a visible pair; with the heads of P alone it took 578). Then a tile pair took about 4000 cycles per 128 keys, of which the tensor
-//    core worked 2050: the rest is the way from a tile's last P over the MMAs still to be issued to its next scores, and the
-//    softmax (two warps per scheduler, 1900 cycles alone, 2700 when A's and B's overlap). Tried and slower (us, the first form of this
-//    kernel being 624): scores read twice instead of held 598 against 581; tiles of 64 keys with two S buffers each 711; two
+// Measured, 28 + 4 heads of 128, window 4096, 8192 queries on 8192 cached tokens: 685 us, 704 TFLOP/s of useful products (4 H D
+//    a visible pair), the tensor core at work 60 % of the time. With the heads of P alone it took 578: then a tile pair took about 4000
+//    cycles per 128 keys, of which the tensor core worked 2050 (now 3070): the rest is the way from a tile's last P over the MMAs
+//    still to be issued to its next scores, and the softmax (two warps per scheduler, 1900 cycles alone, 2700 when A's and B's
+//    overlap). Tried and slower, with the heads alone (us, the first form of this kernel being 624): scores read twice instead of held 598 against 581; tiles of 64 keys with two S buffers each 711; two
 //    threads per row 592; part of the exponentials as a polynomial 0 to 5 % more; P in halves 581; MMAs issued
 //    under `lane == 0` 618 against 598; a warp of its own to issue each tile's MMAs 662.
 #include <math.h>

@@ -429,3 +429,32 @@ def test_short_runs_hold_their_weights_in_fp16(ops, ctx, new, wl, H, kvh):
     want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, wl, SCALE, weights=ref.FP16)
     _check(out, None, want)
     assert mean_rel(out.float(), want[0].bfloat16().float()) <= MEAN_REL
+
+
+@gpu
+@pytest.mark.parametrize("H,kvh", [(6, 3), (5, 5), (64, 8), (12, 6)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 0, 9], [40, 3, 300]])
+def test_runs_with_other_numbers_of_kv_heads(ops, H, kvh, new):
+    ctx = [100, 7, 0]
+    codes, scales, table = _pool([a + b for a, b in zip(ctx, new)], 90, kvh, 128, 32, seed=300, spread=0.5, n_new=new)
+    q = torch.randn(sum(new), H, 128, generator=torch.Generator().manual_seed(301)).bfloat16()
+    out = _attend(ops, q, codes, scales, table, ctx, new, 90)
+    want = ref.runs(q.to(DEV), codes.to(DEV), scales.to(DEV), table.to(DEV), ctx, new, 90, SCALE, weights=ref.TWO_BF16)
+    _check(out, None, want)
+
+
+@gpu
+@pytest.mark.parametrize("new", [None, 4, 40])
+def test_infinite_queries_spoil_their_own_rows_only(ops, new):
+    """Scores of +-inf and NaN stay in the rows whose query makes them, the other heads and queries of their tiles keep their values."""
+    H, kvh, n = 14, 2, new or 1
+    ctx, lens = [60, 300], [60 + n, 300 + n]
+    codes, scales, table = _pool(lens, 100, kvh, 128, 16, seed=302, spread=0.5, n_new=[n, n])
+    q = torch.randn(2 * n, H, 128, generator=torch.Generator().manual_seed(303)).bfloat16()
+    clean = q.clone()
+    q[0, 3, 5], q[n, 9, 127], q[2 * n - 1, 0, 0] = math.inf, -math.inf, math.nan
+    spoilt = torch.zeros(2 * n, H, dtype=torch.bool, device=DEV)
+    spoilt[0, 3] = spoilt[n, 9] = spoilt[2 * n - 1, 0] = True
+    args = (codes, scales, table, lens if new is None else ctx, None if new is None else [n, n], 100)
+    a, b = _attend(ops, q, *args), _attend(ops, clean, *args)
+    assert torch.equal(a[~spoilt], b[~spoilt]) and not torch.isfinite(a.float()[spoilt]).all(-1).any()
