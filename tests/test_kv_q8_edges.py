@@ -233,7 +233,7 @@ def test_tokens_of_an_entry_outside_the_pool_take_no_part(ops, new, H, kvh, bs, 
 
 # ------------------------------------------------------------------------------------- block tables much wider than the sequences
 def test_the_bound_on_the_lengths_bounds_the_workspace(ops):
-    size = lambda mq, mb, wl, kvh=4, **kw: ops.swa_prefill_q8_workspace(3, mq, mb, kvh, 128, "cpu", block_size=16, window_left=wl, **kw).numel()
+    size = lambda mq, mb, wl, kvh=4, **kw: ops.swa_prefill_q8_workspace(3, mq, mb, kvh, 128, "meta", block_size=16, window_left=wl, **kw).numel()
     wide, tight = 65536, 20                                                # columns: 2^20 tokens, 320 tokens
     assert size(17, wide, -1) >= 2 ** 31                                   # one sequence's worth of dense rows
     assert size(17, wide, -1, max_seq_len=320) == size(17, tight, -1) < 2 ** 22
