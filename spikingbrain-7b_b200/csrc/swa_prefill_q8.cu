@@ -25,9 +25,10 @@
 //    a visible pair), the tensor core at work 60 % of the time. With the heads of P alone it took 578: then a tile pair took about 4000
 //    cycles per 128 keys, of which the tensor core worked 2050 (now 3070): the rest is the way from a tile's last P over the MMAs
 //    still to be issued to its next scores, and the softmax (two warps per scheduler, 1900 cycles alone, 2700 when A's and B's
-//    overlap). Tried and slower, with the heads alone (us, the first form of this kernel being 624): scores read twice instead of held 598 against 581; tiles of 64 keys with two S buffers each 711; two
-//    threads per row 592; part of the exponentials as a polynomial 0 to 5 % more; P in halves 581; MMAs issued
-//    under `lane == 0` 618 against 598; a warp of its own to issue each tile's MMAs 662.
+//    overlap). Tried and slower, with the heads alone (us, the first form of this kernel being 624): scores read twice instead of held
+//    598 against 581; tiles of 64 keys with two S buffers each 711; two threads per row 592; part of the exponentials as a
+//    polynomial 0 to 5 % more; P in halves 581; MMAs issued under `lane == 0` 618 against 598; a warp of its own to issue
+//    each tile's MMAs 662.
 #include <math.h>
 
 #include "kv_q8.cuh"
